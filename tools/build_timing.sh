@@ -6,7 +6,7 @@ cd "$(dirname "$0")/../paccmann_polymer_amd/csrc"
 make -s -j8
 mkdir -p /tmp/ppk_timing
 for f in ppk_seq_persist ppk_seq_persist_bwd; do
-  [ -f $f.hip ] && /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -fno-gpu-rdc -Wno-unused-function -DPPK_SEQ_TIMING -c $f.hip -o /tmp/ppk_timing/$f.o
+  [ -f $f.hip ] && /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -fno-gpu-rdc -Wno-unused-function -DPPK_SEQ_TIMING -c $f.hip -o /tmp/ppk_timing/$f.o
 done
 objs=""
 for o in ppk_*.o; do
