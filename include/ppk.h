@@ -43,6 +43,7 @@ extern "C" {
 
 #define PPK_F32 0
 #define PPK_F64 1
+#define PPK_BF16 2
 
 typedef void* ppk_stream_t;   /* hipStream_t */
 
@@ -297,6 +298,33 @@ int ppk_ce_fwd(const float* logits, int64_t ldl, const int64_t* targets, int64_t
                float* loss, void* workspace, size_t ws_bytes, ppk_stream_t stream);
 int ppk_ce_bwd(const float* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
                const float* dloss, float* dlogits, int64_t ldd, const void* workspace, size_t ws_bytes, ppk_stream_t stream);
+
+/* ---- K8: log-probabilities of taken tokens, clipped policy loss --------------
+ * The losses that train a generator from rewards, beside K2 on the same packed logits (no counterpart in the reference: its
+ * only objective is the likelihood of paccmann_encoder.py:168).  logits [rows, V] of dtype PPK_F32 or PPK_BF16, row stride
+ * ldl in elements, any alignment; targets [rows]; a row whose target is ignore_index counts nowhere: its log-probability is
+ * 0 and its gradient row is zero, whatever stands in its logits.  A target that is neither ignore_index nor in [0, V) makes its
+ * log-probability, and the loss, NaN.  log-probabilities are of softmax(logits / temperature).
+ *   ppk_token_logp_fwd  logp [rows]; saved [rows, 2] (NULL where no backward follows) is what ppk_token_logp_bwd takes
+ *   ppk_token_logp_bwd  dlogits = dlogp / temperature (onehot - softmax), in the type of the logits, row stride ldd
+ *   ppk_policy_loss     ratio = exp(logp - old); per row -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *                       + kl_coef (e^d - d - 1), d = ref - logp (ref_logp may be NULL where kl_coef is 0);
+ *                       loss [1] is the mean over the rows that count (0 where none does), stats [3] the means of the policy
+ *                       term, of the KL term and of the rows whose clipped side is the smaller one.  dlogits (NULL: not wanted)
+ *                       receives the gradient of the loss in the same pass over the logits.
+ *   ppk_scale_unless_one  g *= scale[0] (a device scalar), nothing where that is 1: the upstream gradient of a loss whose
+ *                       gradient has been written already
+ * Sums over rows are in 64 bits and of a fixed order. */
+int ppk_token_logp_fwd(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                       float temperature, float* logp, float* saved, ppk_stream_t stream);
+int ppk_token_logp_bwd(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                       float temperature, const float* saved, const float* dlogp, void* dlogits, int64_t ldd, ppk_stream_t stream);
+size_t ppk_policy_loss_workspace_bytes(int64_t rows);
+int ppk_policy_loss(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                    float temperature, const float* old_logp, const float* advantages, const float* ref_logp,
+                    float clip_low, float clip_high, float kl_coef, float* loss, float* stats, void* dlogits, int64_t ldd,
+                    void* workspace, size_t ws_bytes, ppk_stream_t stream);
+int ppk_scale_unless_one(int dtype, void* g, int64_t n, const float* scale, ppk_stream_t stream);
 
 /* ---- K3: reparameterise + KL ------------------------------------------------
  * TeacherVAE.reparameterize (paccmann_encoder.py:167; in-tree twin

@@ -67,6 +67,12 @@ SIGNATURES = {
     'ppk_ce_workspace_bytes': (c_sz, [c_i64]),
     'ppk_ce_fwd': (c_int, [ptr, c_i64, ptr, c_i64, c_i64, c_i64, ptr, ptr, c_sz, ptr]),
     'ppk_ce_bwd': (c_int, [ptr, c_i64, ptr, c_i64, c_i64, c_i64, ptr, ptr, c_i64, ptr, c_sz, ptr]),
+    'ppk_token_logp_fwd': (c_int, [c_int, ptr, c_i64, ptr, c_i64, c_i64, c_i64, c_f32, ptr, ptr, ptr]),
+    'ppk_token_logp_bwd': (c_int, [c_int, ptr, c_i64, ptr, c_i64, c_i64, c_i64, c_f32, ptr, ptr, ptr, c_i64, ptr]),
+    'ppk_policy_loss_workspace_bytes': (c_sz, [c_i64]),
+    'ppk_policy_loss': (c_int, [c_int, ptr, c_i64, ptr, c_i64, c_i64, c_i64, c_f32, ptr, ptr, ptr, c_f32, c_f32, c_f32,
+                                ptr, ptr, ptr, c_i64, ptr, c_sz, ptr]),
+    'ppk_scale_unless_one': (c_int, [c_int, ptr, c_i64, ptr, ptr]),
     'ppk_reparam_workspace_bytes': (c_sz, [c_i64]),
     'ppk_reparam_fwd': (c_int, [ptr, ptr, ptr, c_i64, ptr, ptr, ptr, c_sz, ptr]),
     'ppk_reparam_bwd': (c_int, [ptr, ptr, ptr, c_i64, ptr, ptr, ptr, ptr, ptr]),
@@ -95,6 +101,8 @@ SIGNATURES = {
 
 
 PPK_ERR_UNSUP = -4        # include/ppk.h
+PPK_F32, PPK_BF16 = 0, 2
+DTYPES = {torch.float32: PPK_F32, torch.bfloat16: PPK_BF16}
 
 
 class PPKError(RuntimeError):
@@ -138,6 +146,22 @@ def p(t):
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def dtype_code(t, what):
+    """The library's code of a tensor's element type; a type that the kernels do not take is refused."""
+    if t.dtype not in DTYPES:
+        raise TypeError(f'{what}: {t.dtype} is not supported (float32 and bfloat16 are)')
+    return DTYPES[t.dtype]
+
+
+def one_device(*tensors):
+    """The GPU that all of these tensors (None: left out) are on; anything else is refused."""
+    require_gpu(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise PPKError(f'tensors on different devices: {sorted(map(str, devices))}')
+    return devices.pop()
 
 
 def require_gpu(*tensors):

@@ -14,6 +14,9 @@
 
 #define PPK_F32 0
 #define PPK_F64 1
+#define PPK_BF16 2
+
+typedef void* ppk_stream_t;   // hipStream_t
 
 void ppk_set_error(const char* fmt, ...);
 

@@ -1,0 +1,445 @@
+// Log-probabilities of the tokens a generator took, and the clipped policy loss on them with a KL term towards a reference,
+// from logits [rows, V] in fp32 or bf16.  With v = logits / temperature, m = max v, s = sum exp(v - m):
+//   lp    = v[token] - m - log s
+//   ratio = exp(lp - old);  pg = -min(ratio A, clip(ratio, 1 - lo, 1 + hi) A);  d = ref - lp;  kl = e^d - d - 1
+//   loss  = sum over rows that count of (pg + beta kl) / n
+//   dloss / dlp = (-ratio A where ratio A is the smaller side, else 0) + beta (1 - e^d);  dlp / dlogits = (onehot - softmax) / temperature
+// All of it is bound by HBM: the logits are read once and held in registers, and a training call writes their gradient in the
+// same pass.  A row belongs to a group of TG threads that hold it as NV 16-byte chunks each.
+#include "ppk_common.h"
+#include "ppk_vec.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int COUNT_BLOCK = 4096;                // targets per partial count
+constexpr int MAX_BLOCKS = 4096;                 // row blocks of a launch, and rows of its partial sums
+
+// What a row of logits meets.  `old` etc. are read only in the policy modes.
+struct RowArgs {
+    const void* logits; long long ld;            // row stride in elements
+    const int64_t* targets;
+    long long rows;
+    int V;
+    long long ignore;
+    float inv_t;                                 // 1 / temperature
+    const float* old; const float* adv; const float* ref;
+    float low, high, beta;                       // 1 - clip_low, 1 + clip_high
+    const int* counts; int ncounts;              // partial counts of the rows that count
+    void* grad; long long ldg;
+    float* logp; float* saved;                   // [rows]; [rows, 2]: max logit and 1 / s
+    double* part;                                // [blocks, 3]
+};
+
+enum { MODE_LOGP = 0, MODE_POLICY = 1, MODE_POLICY_GRAD = 2 };
+
+__global__ __launch_bounds__(256) void k_count_rows(const int64_t* __restrict__ tgt, long long rows, long long ignore, int* __restrict__ counts)
+{
+    __shared__ int sc[4];
+    const long long r0 = (long long)blockIdx.x * COUNT_BLOCK;
+    int c = 0;
+    for (int i = threadIdx.x; i < COUNT_BLOCK && r0 + i < rows; i += 256) c += tgt[r0 + i] != ignore;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    if ((threadIdx.x & 63) == 0) sc[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = sc[0] + sc[1] + sc[2] + sc[3];
+}
+
+// the number of rows that count, the same in every thread of a block; `red` is LDS of one int per wave
+__device__ __forceinline__ int total_count(const int* counts, int n, int* red)
+{
+    int c = 0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) c += counts[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    int t = 0;
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) t += red[w];
+    return t;
+}
+
+template <int TG> __device__ __forceinline__ float group_max(float v, float* red)
+{
+#pragma unroll
+    for (int o = (TG < 64 ? TG : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if (TG > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TG / 64; ++w) v = fmaxf(v, red[w]);
+    }
+    return v;
+}
+template <int TG> __device__ __forceinline__ float group_sum(float v, float* red)
+{
+#pragma unroll
+    for (int o = (TG < 64 ? TG : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (TG > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TG / 64; ++w) v += red[w];
+    }
+    return v;
+}
+
+// The terms of one row in fp64: e^d - d - 1 of a small d and the border of the clip both need more than 24 bits, and a row
+// costs one lane a few hundred cycles beside V exponentials.  Returns dloss / dlp of the row (before the division by n).
+__device__ __forceinline__ double policy_terms(const RowArgs& a, long long row, double lp, double& pg, double& kl, double& clipped)
+{
+    double em[2];                                  // expm1 of lp - old and of ref - lp: exp(u) = expm1(u) + 1 to an absolute 2^-53
+    const double u[2] = {lp - (double)a.old[row], a.ref ? (double)a.ref[row] - lp : 0.0};
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) em[k] = expm1(u[k]);
+    const double adv = a.adv[row], ratio = em[0] + 1.0;
+    const double held_r = ratio < (double)a.low ? (double)a.low : (ratio > (double)a.high ? (double)a.high : ratio);
+    const double free_ = ratio * adv, held = held_r * adv;
+    pg = -(free_ <= held ? free_ : (free_ != free_ ? free_ : held));
+    clipped = held < free_ ? 1.0 : 0.0;
+    double g = free_ <= held ? -free_ : 0.0;
+    kl = 0.0;
+    if (a.ref) {
+        kl = em[1] - u[1];
+        g -= (double)a.beta * em[1];
+    }
+    return g;
+}
+
+// One group of TG threads a row (TG <= 64: 256 / TG rows a workgroup at once; above, one), NV chunks of 16 bytes a thread.
+// NV = 0: the row does not fit in registers and is read again for its gradient.
+template <typename T, int TG, int NV, int MODE>
+__global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
+{
+    constexpr int E = 16 / (int)sizeof(T), THREADS = TG > 256 ? TG : 256, GROUPS = THREADS / TG;
+    __shared__ float red[THREADS / 64];
+    __shared__ int redc[THREADS / 64];
+    __shared__ double acc_s[GROUPS][3];
+    const int g = threadIdx.x / TG, l = threadIdx.x % TG;
+    double inv_n = 1.0;
+    if (MODE == MODE_POLICY_GRAD) {
+        const int n = total_count(a.counts, a.ncounts, redc);
+        inv_n = 1.0 / (double)(n > 0 ? n : 1);
+    }
+    const float k2 = a.inv_t * LOG2E;
+    double s_pg = 0, s_kl = 0, s_cl = 0;
+    for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < a.rows; row0 += (long long)gridDim.x * GROUPS) {
+        const long long row = row0 + g;
+        const bool live = row < a.rows;                                   // TG <= 64: whole groups idle, no barrier inside
+        const T* x = (const T*)a.logits + (live ? row : 0) * a.ld;
+        const RowChunks<T> rc(x, live ? a.V : 0);
+        uint4 raw[NV > 0 ? NV : 1];
+        float m = -INFINITY;
+        if (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = rc.load(l + i * TG, -INFINITY);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float v[E];
+                unpack<T>(raw[i], v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+            }
+        } else {
+            for (int c = l; c < rc.chunks; c += TG) {
+                float v[E];
+                unpack<T>(rc.load(c, -INFINITY), v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+            }
+        }
+        m = group_max<TG>(m, red);
+        float s = 0.f;
+        if (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float v[E];
+                unpack<T>(raw[i], v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * k2);
+            }
+        } else {
+            for (int c = l; c < rc.chunks; c += TG) {
+                float v[E];
+                unpack<T>(rc.load(c, -INFINITY), v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * k2);
+            }
+        }
+        s = group_sum<TG>(s, red);
+        if (!live) continue;                                              // no barrier below; the whole group leaves together
+        const long long t = a.targets[row];
+        const bool counts = t != a.ignore, good = t >= 0 && t < a.V;
+        double lp = 0.0;
+        if (counts) lp = good ? ((double)to_f32(x[t]) - (double)m) * (double)a.inv_t - log((double)s) : (double)NAN;   // an id outside the vocabulary: NaN, never a guess
+        if (MODE == MODE_LOGP) {
+            if (l == 0) {
+                a.logp[row] = (float)lp;
+                if (a.saved) { a.saved[2 * row] = m; a.saved[2 * row + 1] = 1.0f / s; }
+            }
+            continue;
+        }
+        double gr = 0.0;
+        if (counts) {
+            double pg, kl, cl;
+            gr = policy_terms(a, row, lp, pg, kl, cl);
+            s_pg += pg; s_kl += kl; s_cl += cl;
+        }
+        if (MODE == MODE_POLICY_GRAD) {
+            const float gt = (float)(gr * inv_n * (double)a.inv_t);
+            const float gp = -gt / s;
+            T* out = (T*)a.grad + row * a.ldg;
+            const RowChunks<T> oc(out, a.V);
+            const bool same = oc.shift == rc.shift;
+            const auto emit = [&](int c, uint4 r) {
+                float v[E];
+                unpack<T>(r, v);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float p = counts ? gp * __builtin_amdgcn_exp2f((v[e] - m) * k2) : 0.f;
+                    if (counts && rc.at(c, e) == t) p += gt;
+                    v[e] = p;
+                }
+                if (same) oc.store(out, c, v);
+                else if (c < rc.chunks)
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (rc.has(c, e)) out[rc.at(c, e)] = from_f32<T>(v[e]);
+            };
+            if (NV > 0) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) emit(l + i * TG, raw[i]);
+            } else {
+                for (int c = l; c < rc.chunks; c += TG) emit(c, rc.load(c, -INFINITY));
+            }
+        }
+    }
+    if (MODE != MODE_LOGP) {
+        if (l == 0) { acc_s[g][0] = s_pg; acc_s[g][1] = s_kl; acc_s[g][2] = s_cl; }
+        __syncthreads();
+        if (threadIdx.x < 3) {
+            double t = 0;
+            for (int q = 0; q < GROUPS; ++q) t += acc_s[q][threadIdx.x];
+            a.part[(long long)blockIdx.x * 3 + threadIdx.x] = t;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__ part, int nparts, const int* __restrict__ counts, int ncounts,
+                                                      float beta, float* __restrict__ loss, float* __restrict__ stats)
+{
+    __shared__ int redc[4];
+    __shared__ double red[4][3];
+    const int n = total_count(counts, ncounts, redc);
+    double a[3] = {0, 0, 0};
+    for (int p = threadIdx.x; p < nparts; p += 256)
+        for (int k = 0; k < 3; ++k) a[k] += part[(long long)p * 3 + k];
+    for (int k = 0; k < 3; ++k) {
+        a[k] = ppk_wave_sum_d(a[k]);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][k] = a[k];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double inv = 1.0 / (double)(n > 0 ? n : 1);
+        double t[3];
+        for (int k = 0; k < 3; ++k) t[k] = ((red[0][k] + red[1][k]) + (red[2][k] + red[3][k])) * inv;
+        loss[0] = (float)(t[0] + (double)beta * t[1]);
+        for (int k = 0; k < 3; ++k) stats[k] = (float)t[k];
+    }
+}
+
+// d logits = g / temperature (onehot - softmax) from what the forward kept of each row: its max and 1 / s
+template <typename T>
+__global__ __launch_bounds__(256) void k_logp_bwd(RowArgs a, const float* __restrict__ saved, const float* __restrict__ dlogp, int per_row)
+{
+    constexpr int E = 16 / (int)sizeof(T);
+    const float k2 = a.inv_t * LOG2E;
+    const long long tasks = a.rows * per_row;
+    for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
+        const long long row = task / per_row;
+        const int c = (int)(task - row * per_row) * 256 + threadIdx.x;
+        const T* x = (const T*)a.logits + row * a.ld;
+        const RowChunks<T> rc(x, a.V);
+        if (c >= rc.chunks) continue;
+        T* out = (T*)a.grad + row * a.ldg;
+        const RowChunks<T> oc(out, a.V);
+        const long long t = a.targets[row];
+        const bool counts = t != a.ignore;
+        const float g = t >= 0 && t < a.V ? dlogp[row] * a.inv_t : NAN, m = saved[2 * row], gp = -g * saved[2 * row + 1];
+        float v[E];
+        unpack<T>(rc.load(c, -INFINITY), v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float p = counts ? gp * __builtin_amdgcn_exp2f((v[e] - m) * k2) : 0.f;
+            if (counts && rc.at(c, e) == t) p += g;
+            v[e] = p;
+        }
+        if (oc.shift == rc.shift) oc.store(out, c, v);
+        else
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (rc.has(c, e)) out[rc.at(c, e)] = from_f32<T>(v[e]);
+    }
+}
+
+// grad *= scale[0], and nothing at all where that is 1 (the upstream gradient of a loss that is the root of the backward pass)
+template <typename T>
+__global__ __launch_bounds__(256) void k_scale_unless_one(T* __restrict__ g, long long n, const float* __restrict__ scale)
+{
+    const float s = scale[0];
+    if (s == 1.0f) return;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) g[e] = from_f32<T>(to_f32(g[e]) * s);
+}
+
+template <typename T, int TG, int NV>
+void launch_rows(const RowArgs& a, int mode, int blocks, hipStream_t st)
+{
+    const dim3 block(TG > 256 ? TG : 256);
+    if (mode == MODE_LOGP) k_rows_lp<T, TG, NV, MODE_LOGP><<<blocks, block, 0, st>>>(a);
+    else if (mode == MODE_POLICY) k_rows_lp<T, TG, NV, MODE_POLICY><<<blocks, block, 0, st>>>(a);
+    else k_rows_lp<T, TG, NV, MODE_POLICY_GRAD><<<blocks, block, 0, st>>>(a);
+}
+
+// group width of a row of `chunks` 16-byte chunks, and the blocks of a launch over `rows`
+int group_width(long long chunks) { return chunks <= 64 ? 16 : chunks <= 512 ? 64 : chunks <= 2048 ? 256 : 1024; }
+int row_blocks(long long rows, int tg)
+{
+    const int groups = tg >= 256 ? 1 : 256 / tg;
+    const long long b = (rows + groups - 1) / groups;
+    return (int)(b < MAX_BLOCKS ? b : MAX_BLOCKS);
+}
+
+template <typename T>
+void dispatch_rows(const RowArgs& a, int mode, int blocks, long long chunks, hipStream_t st)
+{
+    if (chunks <= 16) launch_rows<T, 16, 1>(a, mode, blocks, st);
+    else if (chunks <= 64) launch_rows<T, 16, 4>(a, mode, blocks, st);
+    else if (chunks <= 128) launch_rows<T, 64, 2>(a, mode, blocks, st);
+    else if (chunks <= 256) launch_rows<T, 64, 4>(a, mode, blocks, st);
+    else if (chunks <= 512) launch_rows<T, 64, 8>(a, mode, blocks, st);
+    else if (chunks <= 1024) launch_rows<T, 256, 4>(a, mode, blocks, st);
+    else if (chunks <= 2048) launch_rows<T, 256, 8>(a, mode, blocks, st);
+    else if (chunks <= 4096) launch_rows<T, 1024, 4>(a, mode, blocks, st);
+    else if (chunks <= 8192) launch_rows<T, 1024, 8>(a, mode, blocks, st);
+    else if (chunks <= 16384) launch_rows<T, 1024, 16>(a, mode, blocks, st);
+    else launch_rows<T, 1024, 0>(a, mode, blocks, st);
+}
+
+int elem_bytes(int dtype) { return dtype == PPK_F32 ? 4 : 2; }
+// chunks of a row at worst: one more than its bytes need where it begins inside a chunk
+long long row_chunks(long long V, int dtype) { return (V * elem_bytes(dtype) + 15) / 16 + 1; }
+
+int check_rows(const char* what, int dtype, long long rows, long long V, const void* logits, long long ld, const void* targets, float temperature)
+{
+    if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "%s: logits of type %d (fp32 and bf16 are supported)", what, dtype);
+    if (rows < 0 || V < 1 || ld < V || V > (1LL << 30)) PPK_FAIL(PPK_ERR_SHAPE, "%s: rows=%lld V=%lld row stride=%lld", what, rows, V, ld);
+    if (!(temperature > 0.f) || temperature > 3.0e38f) PPK_FAIL(PPK_ERR_SHAPE, "%s: temperature %g", what, (double)temperature);
+    if (rows > 0 && (!logits || !targets)) PPK_FAIL(PPK_ERR_NULL, "%s: null pointer", what);
+    if ((uintptr_t)logits % (unsigned)elem_bytes(dtype)) PPK_FAIL(PPK_ERR_ALIGN, "%s: logits not aligned to their elements", what);
+    return PPK_OK;
+}
+
+struct PolicyWs { int* counts; double* part; };
+int count_blocks(long long rows) { return (int)((rows + COUNT_BLOCK - 1) / COUNT_BLOCK); }
+size_t policy_ws_bytes(long long rows) { return ppk_align_up((size_t)count_blocks(rows) * 4, 256) + ppk_align_up((size_t)MAX_BLOCKS * 24, 256); }
+
+}  // namespace
+
+extern "C" {
+
+int ppk_token_logp_fwd(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                       float temperature, float* logp, float* saved, ppk_stream_t stream)
+{
+    int rc = check_rows("token_logp_fwd", dtype, rows, V, logits, ldl, targets, temperature);
+    if (rc) return rc;
+    if (rows == 0) return PPK_OK;
+    if (!logp) PPK_FAIL(PPK_ERR_NULL, "token_logp_fwd: null pointer");
+    RowArgs a = {};
+    a.logits = logits; a.ld = ldl; a.targets = targets; a.rows = rows; a.V = (int)V; a.ignore = ignore_index; a.inv_t = 1.0f / temperature;
+    a.logp = logp; a.saved = saved;
+    const long long ch = row_chunks(V, dtype);
+    const int blocks = row_blocks(rows, group_width(ch));
+    if (dtype == PPK_F32) dispatch_rows<float>(a, MODE_LOGP, blocks, ch, (hipStream_t)stream);
+    else dispatch_rows<bf16_t>(a, MODE_LOGP, blocks, ch, (hipStream_t)stream);
+    PPK_CHECK_LAUNCH("token_logp_fwd");
+    return PPK_OK;
+}
+
+int ppk_token_logp_bwd(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                       float temperature, const float* saved, const float* dlogp, void* dlogits, int64_t ldd, ppk_stream_t stream)
+{
+    int rc = check_rows("token_logp_bwd", dtype, rows, V, logits, ldl, targets, temperature);
+    if (rc) return rc;
+    if (ldd < V) PPK_FAIL(PPK_ERR_SHAPE, "token_logp_bwd: row stride %lld < V", (long long)ldd);
+    if (rows == 0) return PPK_OK;
+    if (!saved || !dlogp || !dlogits) PPK_FAIL(PPK_ERR_NULL, "token_logp_bwd: null pointer");
+    RowArgs a = {};
+    a.logits = logits; a.ld = ldl; a.targets = targets; a.rows = rows; a.V = (int)V; a.ignore = ignore_index; a.inv_t = 1.0f / temperature;
+    a.grad = dlogits; a.ldg = ldd;
+    const int per_row = (int)((row_chunks(V, dtype) + 255) / 256);
+    const long long tasks = rows * per_row;
+    const unsigned blocks = (unsigned)(tasks < 16384 ? tasks : 16384);
+    if (dtype == PPK_F32) k_logp_bwd<float><<<blocks, 256, 0, (hipStream_t)stream>>>(a, saved, dlogp, per_row);
+    else k_logp_bwd<bf16_t><<<blocks, 256, 0, (hipStream_t)stream>>>(a, saved, dlogp, per_row);
+    PPK_CHECK_LAUNCH("token_logp_bwd");
+    return PPK_OK;
+}
+
+size_t ppk_policy_loss_workspace_bytes(int64_t rows) { return rows < 0 ? 0 : policy_ws_bytes(rows); }
+
+int ppk_policy_loss(int dtype, const void* logits, int64_t ldl, const int64_t* targets, int64_t rows, int64_t V, int64_t ignore_index,
+                    float temperature, const float* old_logp, const float* advantages, const float* ref_logp,
+                    float clip_low, float clip_high, float kl_coef, float* loss, float* stats, void* dlogits, int64_t ldd,
+                    void* workspace, size_t ws_bytes, ppk_stream_t stream)
+{
+    int rc = check_rows("policy_loss", dtype, rows, V, logits, ldl, targets, temperature);
+    if (rc) return rc;
+    if (!(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f)) PPK_FAIL(PPK_ERR_SHAPE, "policy_loss: clip range [%g, %g]", (double)clip_low, (double)clip_high);
+    if (!loss || !stats || !workspace || (rows > 0 && (!old_logp || !advantages))) PPK_FAIL(PPK_ERR_NULL, "policy_loss: null pointer");
+    if (rows > 0 && kl_coef != 0.f && !ref_logp) PPK_FAIL(PPK_ERR_NULL, "policy_loss: a KL term needs the reference's log-probabilities");
+    if (dlogits && ldd < V) PPK_FAIL(PPK_ERR_SHAPE, "policy_loss: row stride %lld < V", (long long)ldd);
+    if (rows > (1LL << 31) - 1) PPK_FAIL(PPK_ERR_UNSUP, "policy_loss: %lld rows", (long long)rows);
+    if (ws_bytes < policy_ws_bytes(rows)) PPK_FAIL(PPK_ERR_WS, "policy_loss: workspace of %zu bytes, %zu needed", ws_bytes, policy_ws_bytes(rows));
+    hipStream_t st = (hipStream_t)stream;
+    char* cur = (char*)workspace;
+    const int nc = count_blocks(rows);
+    int* counts = (int*)ppk_carve(cur, (size_t)nc * 4);
+    RowArgs a = {};
+    a.logits = logits; a.ld = ldl; a.targets = targets; a.rows = rows; a.V = (int)V; a.ignore = ignore_index; a.inv_t = 1.0f / temperature;
+    a.old = old_logp; a.adv = advantages; a.ref = ref_logp;
+    a.low = 1.0f - clip_low; a.high = 1.0f + clip_high; a.beta = kl_coef;
+    a.counts = counts; a.ncounts = nc; a.grad = dlogits; a.ldg = ldd;
+    a.part = (double*)cur;
+    const long long ch = row_chunks(V, dtype);
+    const int blocks = row_blocks(rows, group_width(ch));
+    if (nc) k_count_rows<<<nc, 256, 0, st>>>(targets, rows, ignore_index, counts);
+    const int mode = dlogits ? MODE_POLICY_GRAD : MODE_POLICY;
+    if (rows > 0) {
+        if (dtype == PPK_F32) dispatch_rows<float>(a, mode, blocks, ch, st);
+        else dispatch_rows<bf16_t>(a, mode, blocks, ch, st);
+    }
+    k_policy_final<<<1, 256, 0, st>>>(a.part, rows > 0 ? blocks : 0, counts, nc, kl_coef, loss, stats);
+    PPK_CHECK_LAUNCH("policy_loss");
+    return PPK_OK;
+}
+
+int ppk_scale_unless_one(int dtype, void* g, int64_t n, const float* scale, ppk_stream_t stream)
+{
+    if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "scale_unless_one: type %d", dtype);
+    if (n < 0) PPK_FAIL(PPK_ERR_SHAPE, "scale_unless_one: n=%lld", (long long)n);
+    if (n == 0) return PPK_OK;
+    if (!g || !scale) PPK_FAIL(PPK_ERR_NULL, "scale_unless_one: null pointer");
+    const long long b = (n + 2047) / 2048;
+    const unsigned blocks = (unsigned)(b < 2048 ? b : 2048);
+    if (dtype == PPK_F32) k_scale_unless_one<float><<<blocks, 256, 0, (hipStream_t)stream>>>((float*)g, n, scale);
+    else k_scale_unless_one<bf16_t><<<blocks, 256, 0, (hipStream_t)stream>>>((bf16_t*)g, n, scale);
+    PPK_CHECK_LAUNCH("scale_unless_one");
+    return PPK_OK;
+}
+
+}  // extern "C"

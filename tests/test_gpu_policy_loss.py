@@ -1,0 +1,242 @@
+"""`token_log_probs` and `policy_loss` against their definitions in 64 bits.
+
+Tolerances, in half-steps of fp32 (H = 2^-24).  The exponent of a term is (v - m) times a rounded constant: three roundings, so a
+term e^-u is off by at most 3u + 2 (the exponential itself) halves relative, and since sum e^-u u <= log(V) sum e^-u the sum s by
+3 log V + 2, plus one half for each addition on a value's way (at most 64 in a thread, 6 across lanes, 16 across waves).  With
+V <= 2^18 that is below 130 H: lp is off by at most 130 H, and by one rounding of itself when it is stored.  A gradient
+g (onehot - p) has p off by that and by its own exponent's error 3u + 2, where p u <= u e^-u <= 0.37: below |g| (p 140 + 8) H.  bf16
+results add one half-step of theirs, 2^-8 relative."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+H = 2.0 ** -24
+
+
+def make(rows, V, dtype, seed, scale=2.0, ignored=0.2, ld=None, offset=0):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    ld = V if ld is None else ld
+    store = torch.randn(rows * ld + offset, generator=g, device='cuda') * scale
+    logits = store.to(dtype)[offset:].view(rows, ld)[:, :V]
+    tgt = torch.randint(1 if V > 1 else 0, V, (rows,), generator=g, device='cuda')
+    tgt[torch.rand(rows, generator=g, device='cuda') < ignored] = 0
+    return logits, tgt, g
+
+
+def definition(logits, tgt, temperature):
+    v = logits.double() / temperature
+    lp = torch.log_softmax(v, 1)
+    return lp.gather(1, tgt.clamp(0, logits.shape[1] - 1)[:, None])[:, 0], lp.exp()
+
+
+def close(got, want, tol, dtype):
+    if dtype == torch.bfloat16:
+        tol = tol * (1 + 2.0 ** -8) + want.abs() * 2.0 ** -8
+    bad = (got.double() - want).abs() > tol
+    assert not bool(bad.any()), (int(bad.sum()), float((got.double() - want).abs().max()))
+
+
+CASES = [(1, 1), (1, 2), (3, 5), (7, 64), (33, 65), (130, 257), (5, 575), (9, 1025), (4, 2050), (3, 8199), (3, 16391), (2, 33001), (2, 70001), (1, 131073)]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,V', CASES)
+def test_token_log_probs(rows, V, dtype):
+    from paccmann_polymer_amd.policy_loss import token_log_probs
+    for temperature, ld, offset in ((1.0, V, 0), (0.7, V + 3, 1)):
+        logits, tgt, g = make(rows, V, dtype, rows + V, ld=ld, offset=offset)
+        use = tgt != 0
+        want, p = definition(logits, tgt, temperature)
+        x = logits.detach().requires_grad_()
+        lp = token_log_probs(x, tgt, temperature=temperature)
+        want = torch.where(use, want, 0.0)
+        close(lp.detach(), want, 130 * H + H * want.abs(), torch.float32)
+        assert torch.equal(lp.detach(), token_log_probs(logits, tgt, temperature=temperature))        # the same with and without a backward
+        up = torch.randn(rows, generator=g, device='cuda')
+        (d,) = torch.autograd.grad(lp, x, up)
+        gr = (torch.where(use, up, 0.0) / temperature).double()[:, None]
+        dwant = -p * gr
+        dwant.scatter_add_(1, tgt[:, None], gr)
+        assert d.dtype == dtype and d.shape == logits.shape
+        close(d, dwant, gr.abs() * (140 * p + 8) * H, dtype)
+
+
+def policy_definition(logits, tgt, old, adv, ref, lo, hi, beta, temperature):
+    x = logits.double().requires_grad_()
+    use = tgt != 0
+    lp = torch.log_softmax(x / temperature, 1).gather(1, tgt[:, None])[:, 0][use]
+    A = adv.double()[use]
+    ratio = torch.exp(lp - old.double()[use])
+    free, held = ratio * A, ratio.clamp(1 - lo, 1 + hi) * A
+    pg = -torch.minimum(free, held)
+    kl = torch.zeros_like(pg)
+    if ref is not None:
+        d = ref.double()[use] - lp
+        kl = torch.expm1(d) - d
+    n = max(1, int(use.sum()))
+    loss = (pg.sum() + beta * kl.sum()) / n
+    (grad,) = torch.autograd.grad(loss, x) if x.numel() else (x,)
+    return loss.detach(), torch.stack([pg.sum() / n, kl.sum() / n, (held < free).sum() / n]).detach(), grad, (pg.abs().sum() / n).detach()
+
+
+def policy_inputs(logits, tgt, g, lo, hi):
+    """Ratios on both sides of the clip's borders, none within 1e-3 of one (a ratio on a border has no gradient to compare)."""
+    rows = logits.shape[0]
+    lp, _ = definition(logits, tgt, 1.0)
+    u = 0.3 * torch.randn(rows, generator=g, device='cuda', dtype=torch.float64)
+    for edge in (math.log(1 - lo), math.log(1 + hi)):
+        u = torch.where((u - edge).abs() < 1e-3, u + 3e-3, u)
+    return (lp - u).float(), torch.randn(rows, generator=g, device='cuda'), (lp + 0.3 * torch.randn(rows, generator=g, device='cuda', dtype=torch.float64)).float()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,V', CASES + [(5000, 40), (20011, 3)])
+def test_policy_loss(rows, V, dtype):
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    lo, hi, beta = 0.2, 0.28, 0.05
+    logits, tgt, g = make(rows, V, dtype, rows * 3 + V)
+    old, adv, ref = policy_inputs(logits, tgt, g, lo, hi)
+    use = (tgt != 0)[:, None]
+    for r, b in ((ref, beta), (None, 0.0)):
+        loss_w, stats_w, grad_w, size = policy_definition(logits, tgt, old, adv, r, lo, hi, b, 1.0)
+        x = logits.detach().requires_grad_()
+        loss, stats = policy_loss(x, tgt, old, adv, r, clip_low=lo, clip_high=hi, kl_coef=b)
+        # a ratio is off by 130 H relative, a KL term by |e^d - 1| 130 H; each mean is rounded once
+        tol = 130 * H * (size + 0.5 + 2 * b) + H
+        assert abs(float(loss.detach() - loss_w)) <= float(tol) + H * abs(float(loss_w))
+        assert bool(((stats.double() - stats_w).abs() <= tol + H * stats_w.abs()).all()), (stats, stats_w)
+        with torch.no_grad():
+            again, st2 = policy_loss(logits, tgt, old, adv, r, clip_low=lo, clip_high=hi, kl_coef=b)
+        assert torch.equal(again, loss.detach()) and torch.equal(st2, stats)
+        (d,) = torch.autograd.grad(loss, x)
+        assert d.dtype == dtype and d.shape == logits.shape
+        # the row's factor: |ratio A| + b |e^d - 1| over n, off by 130 H of each and two roundings
+        n = max(1, int(use.sum()))
+        lp, p = definition(logits, tgt, 1.0)
+        gmax = torch.exp(lp - old.double()) * adv.double().abs() + (b * torch.exp(ref.double() - lp) if r is not None else 0.0)
+        close(d, grad_w, torch.where(use, gmax[:, None] / n * (p * 272 + 140) * H, 0.0), dtype)
+
+
+def test_policy_loss_upstream_gradient_and_second_backward():
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(50, 70, torch.float32, 1)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    x = logits.detach().requires_grad_()
+    loss, _ = policy_loss(x, tgt, old, adv, ref, kl_coef=0.1)
+    (d1,) = torch.autograd.grad(loss, x, retain_graph=True)
+    keep = d1.clone()
+    (d3,) = torch.autograd.grad(loss * -3.0, x, retain_graph=True)
+    assert torch.equal(d1, keep)                                    # what was handed out is not touched again
+    assert torch.equal(d3, keep * -3.0)
+    (d0,) = torch.autograd.grad(loss * 0.0, x)
+    assert not bool(d0.any())
+
+
+def test_rows_that_do_not_count_leak_nothing():
+    """NaN and infinities in every input of an ignored row, and infinite logits in a row that counts."""
+    from paccmann_polymer_amd.policy_loss import policy_loss, token_log_probs
+    inf, nan = float('inf'), float('nan')
+    logits, tgt, g = make(12, 33, torch.float32, 2, ignored=0.0)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    tgt[3] = tgt[7] = 0
+    logits, old, adv, ref = logits.clone(), old.clone(), adv.clone(), ref.clone()
+    logits[5, :20] = -inf                                           # tokens that may not be taken
+    tgt[5] = 30
+    lp5 = torch.log_softmax(logits[5].double(), 0)[30]
+    old[5] = ref[5] = float(lp5)
+    want = policy_definition(logits, tgt, old, adv, ref, 0.2, 0.2, 0.1, 1.0)
+    logits[3] = nan
+    logits[7] = inf
+    for t in (old, adv, ref):
+        t[3], t[7] = nan, -inf
+    x = logits.detach().requires_grad_()
+    loss, stats = policy_loss(x, tgt, old, adv, ref, kl_coef=0.1)
+    (d,) = torch.autograd.grad(loss, x)
+    assert abs(float(loss.detach() - want[0])) <= 130 * H * float(want[3] + 1) + H
+    keep = torch.tensor([i for i in range(12) if i not in (3, 7)], device='cuda')
+    assert not bool(d[3].any()) and not bool(d[7].any()) and bool(torch.isfinite(d).all())
+    assert float((d[keep].double() - want[2][keep]).abs().max()) <= 1e-6
+    assert not bool(d[5, :20].any())
+    y = logits.detach().requires_grad_()
+    lp = token_log_probs(y, tgt)
+    assert float(lp[3].detach()) == 0.0 and float(lp[7].detach()) == 0.0
+    up = torch.ones(12, device='cuda')
+    up[3], up[7] = nan, inf
+    (dl,) = torch.autograd.grad(lp, y, up)
+    assert not bool(dl[3].any()) and not bool(dl[7].any()) and bool(torch.isfinite(dl).all())
+
+
+def test_no_row_counts_and_no_rows():
+    from paccmann_polymer_amd.policy_loss import policy_loss, token_log_probs
+    for rows in (0, 4):
+        x = torch.randn(rows, 9, device='cuda', requires_grad=True)
+        tgt = torch.zeros(rows, dtype=torch.int64, device='cuda')
+        z = torch.zeros(rows, device='cuda')
+        loss, stats = policy_loss(x, tgt, z, z, z, kl_coef=0.1)
+        assert float(loss.detach()) == 0.0 and not bool(stats.any())
+        (d,) = torch.autograd.grad(loss, x)
+        assert d.shape == x.shape and not bool(d.any())
+        assert not bool(token_log_probs(x, tgt).any())
+
+
+def test_target_outside_the_vocabulary_is_nan():
+    from paccmann_polymer_amd.policy_loss import policy_loss, token_log_probs
+    x = torch.randn(4, 9, device='cuda')
+    z = torch.zeros(4, device='cuda')
+    for bad in (9, -1, 1 << 40):
+        tgt = torch.tensor([1, bad, 2, 0], device='cuda')
+        lp = token_log_probs(x, tgt)
+        assert torch.isnan(lp).tolist() == [False, True, False, False]
+        assert bool(torch.isnan(policy_loss(x, tgt, z, z)[0]))
+    assert not bool(torch.isnan(token_log_probs(x, torch.tensor([1, -100, 2, 3], device='cuda'), ignore_index=-100)).any())
+
+
+def test_gradient_against_differences():
+    """Central differences of the 64-bit definition at fp32 logits: the gradient is the derivative of this loss and no other's."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(6, 11, torch.float32, 5)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    x = logits.detach().requires_grad_()
+    (d,) = torch.autograd.grad(policy_loss(x, tgt, old, adv, ref, kl_coef=0.3)[0], x)
+    step = 1e-4
+    for i in range(6):
+        for j in range(0, 11, 3):
+            e = torch.zeros(6, 11, device='cuda', dtype=torch.float64)
+            e[i, j] = step
+            up = policy_definition(logits.double() + e, tgt, old, adv, ref, 0.2, 0.2, 0.3, 1.0)[0]
+            dn = policy_definition(logits.double() - e, tgt, old, adv, ref, 0.2, 0.2, 0.3, 1.0)[0]
+            assert abs(float((up - dn) / (2 * step)) - float(d[i, j])) <= 1e-6      # third derivatives below 10, times step^2 / 6; and fp32
+
+
+def test_other_stream_and_graph_replays():
+    """On a side stream, and captured: every replay sees the inputs of its time; eager work runs between the replays."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(300, 575, torch.float32, 8)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    x = logits.clone().requires_grad_()
+
+    def step():
+        loss, stats = policy_loss(x, tgt, old, adv, ref, kl_coef=0.1)
+        return loss.detach(), stats, torch.autograd.grad(loss, x)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = step()
+    torch.cuda.current_stream().wait_stream(s)
+    eager = step()
+    for a, b in zip(side, eager):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(logits * (1.0 + 0.1 * k))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
