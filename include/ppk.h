@@ -261,6 +261,52 @@ int ppk_stackgru_seq_bwd(int64_t T, const int64_t* batch_sizes_host, int64_t B, 
                          const float* dHtop, float* dXS, int64_t ks, float* DGI, float* DGH, float* DCS,
                          float* dh0, const float* drop, void* workspace, size_t ws_bytes, ppk_stream_t stream);
 
+/* ---- K9: causal convolution and selective state space scan ------------------
+ * A sequence layer for packed batches beside K1 (no counterpart in the reference, whose only sequence operator is the StackGRU of
+ * paccmann_encoder.py:166,168), with forms for single tokens.  dtype of activations: PPK_F32 or PPK_BF16; parameters, states of the
+ * scan and their gradients are fp32.
+ * A batch is packed — step_off [T + 1] and lengths [B] (device): step t owns rows step_off[t] .. step_off[t + 1], sequence b its row
+ * step_off[t] + b, lengths do not increase with b; states are in that order — or rectangular (both NULL): T steps of B sequences.
+ * Tensors are addressed by strides in elements, given as HOST arrays of a step's and a sequence's (a packed tensor: its row stride,
+ * twice; its elements of a row next to each other).  Sequences of no steps keep their state.
+ *
+ * Convolution of K <= 8 taps:  pre_t = bias + sum_k w[d, k] x_{t-K+1+k},  y = silu ? pre sigmoid(pre) : pre.  state, new_state [B, K - 1, D]
+ * (the inputs before the first step and the last ones; state NULL: zeros; either may be NULL, but not the same memory), weight [D, K].
+ * strides_host: fwd x, y; bwd x, dy, dx (two each).  bwd overwrites dx, dweight, dbias (or NULL), dstate (or NULL).
+ * step: x rows of stride ldx, y [B, D]; new_state may be state. */
+int ppk_causal_conv_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
+                        const void* x, const float* weight, const float* bias, const void* state, int silu, void* y, void* new_state,
+                        const int64_t* strides_host, ppk_stream_t stream);
+size_t ppk_causal_conv_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t K);
+int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
+                        const void* x, const float* weight, const float* bias, const void* state, int silu, const void* dy, const void* dnew_state,
+                        void* dx, float* dweight, float* dbias, void* dstate, const int64_t* strides_host,
+                        void* workspace, size_t ws_bytes, ppk_stream_t stream);
+int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void* x, int64_t ldx, const void* state, const float* weight,
+                         const float* bias, int silu, void* y, void* new_state, ppk_stream_t stream);
+/* Scan of N <= 64 states a channel, B and C shared by the D / G channels of a group:
+ *   dt = softplus ? log(1 + e^(raw + bias)) : raw + bias;  h_n = exp(dt A[d, n]) h_n' + dt x B[g, n];  y = (sum_n C[g, n] h_n + skip x) z sigmoid(z)
+ * skip, bias, z and state may be NULL (z: y is not gated).  state, last_state [B, D, N].  kept [tiles, D, N] (NULL: no backward follows)
+ * receives the state before every ppk_selective_scan_tile() steps of each sequence; tiles [B + 1] (device; NULL for a rectangular batch):
+ * the first of them of each sequence and their number.
+ * strides_host [16]: x, raw (two each), B, C (step, sequence, group), z (two), the outputs in ROWS of their width (two), dy (two).
+ * y, dx, draw, dz [rows, D], dB, dC [rows, G, N].  bwd overwrites all its outputs; dskip, dbias, dstate may be NULL. */
+int64_t ppk_selective_scan_tile(void);
+int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, const int64_t* step_off, const int64_t* lengths,
+                           const int64_t* tiles, const void* x, const void* raw, const float* A, const void* Bm, const void* Cm, const float* skip,
+                           const void* z, const float* bias, const float* state, int softplus, void* y, float* last_state, float* kept,
+                           const int64_t* strides_host, ppk_stream_t stream);
+size_t ppk_selective_scan_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows);
+int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows, const int64_t* step_off,
+                           const int64_t* lengths, const int64_t* tiles, const void* x, const void* raw, const float* A, const void* Bm, const void* Cm,
+                           const float* skip, const void* z, const float* bias, int softplus, const float* kept, const void* dy, const float* dlast_state,
+                           void* dx, void* draw, float* dA, void* dB, void* dC, float* dskip, void* dz, float* dbias, float* dstate,
+                           const int64_t* strides_host, void* workspace, size_t ws_bytes, ppk_stream_t stream);
+/* One token of each of B sequences (strides_host as above, the steps' unused); new_state may be state. */
+int ppk_selective_scan_step(int dtype, int64_t B, int64_t D, int64_t N, int64_t G, const void* x, const void* raw, const float* A, const void* Bm,
+                            const void* Cm, const float* skip, const void* z, const float* bias, const float* state, int softplus, void* y,
+                            float* new_state, const int64_t* strides_host, ppk_stream_t stream);
+
 /* ---- row gather / scatter, column sums, embedding gradient ----------------
  * (index_select / index_put / sum(0) / nn.Embedding backward in the reference's
  * torch graph.)  All deterministic. */

@@ -1,0 +1,405 @@
+// Short causal convolution of each channel over packed or rectangular batches of sequences, with the K - 1 inputs before the first
+// step as its state:  pre_t = bias + sum_k w_k x_{t-K+1+k},  y = pre or pre sigmoid(pre).
+//   backward: dpre = dy act'(pre);  dx_t = sum_k w_k dpre_{t+K-1-k};  dw_k = sum_t dpre_t x_{t-K+1+k};  db = sum_t dpre_t
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx.  A wave takes RUN steps of a sequence with the
+// window in registers, VEC channels a lane in 16-byte accesses; its neighbours' K - 1 rows come from the L2.
+#include "ppk_seq_rows.h"
+
+namespace ppk {
+
+namespace {
+// grid (column block of 256, chunk of PS_ROWS rows)
+__global__ __launch_bounds__(256) void k_ps_part(const float* __restrict__ part, long long P, long long C, double* __restrict__ out)
+{
+    const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    const long long p0 = (long long)blockIdx.y * PS_ROWS, p1 = p0 + PS_ROWS < P ? p0 + PS_ROWS : P;
+    double s = 0;
+    long long p = p0;
+    for (; p + 8 <= p1; p += 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = part[(p + k) * C + c];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += (double)v[k];
+    }
+    for (; p < p1; ++p) s += (double)part[p * C + c];
+    out[(long long)blockIdx.y * C + c] = s;
+}
+__global__ __launch_bounds__(256) void k_ps_final(const double* __restrict__ part, int n, long long C, float* __restrict__ out)
+{
+    const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    double s = 0;
+    for (int p = 0; p < n; ++p) s += part[p * C + c];
+    out[c] = (float)s;
+}
+}  // namespace
+
+size_t partial_sum_ws_bytes(long long P, long long C) { return ppk_align_up((size_t)((P + PS_ROWS - 1) / PS_ROWS) * (size_t)C * 8, 256); }
+int partial_sum(const float* part, long long P, long long C, float* out, void* ws, hipStream_t stream)
+{
+    if (C <= 0) return PPK_OK;
+    const unsigned cb = (unsigned)((C + 255) / 256), chunks = (unsigned)((P + PS_ROWS - 1) / PS_ROWS);
+    if (chunks) k_ps_part<<<dim3(cb, chunks), 256, 0, stream>>>(part, P, C, (double*)ws);
+    k_ps_final<<<cb, 256, 0, stream>>>((const double*)ws, (int)chunks, C, out);
+    PPK_CHECK_LAUNCH("partial_sum");
+    return PPK_OK;
+}
+
+}  // namespace ppk
+
+namespace {
+
+using ppk::SeqBatch;
+using ppk::Stride;
+using ppk::at;
+
+constexpr int RUN = 16;                       // steps a wave takes at a time
+constexpr int MAX_SUM_BLOCKS = 512;           // blocks of a backward launch in the sequence direction: rows of its partial sums
+
+struct ConvArgs {
+    SeqBatch q;
+    int D, K, runs;                           // runs: of the longest sequence
+    const void *x, *state, *dy, *dlast;
+    const float *weight, *bias;
+    void *y, *last, *dx, *dstate;
+    float* part;                              // [blocks, K + 1, D]
+    Stride xs, ys, dys;                       // ys: of y or dx
+    int silu;
+};
+
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC])
+{
+    if (VEC == 1) v[0] = to_f32(*p);
+    else unpack<T>(*reinterpret_cast<const uint4*>(p), v);
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC])
+{
+    if (VEC == 1) *p = from_f32<T>(v[0]);
+    else *reinterpret_cast<uint4*>(p) = pack<T>(v);
+}
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+
+// the input of step t, which is of the state before the first step; r = row of step t where t >= 0
+template <typename T, int VEC>
+__device__ __forceinline__ void input_at(const ConvArgs& a, long long t, long long b, int c, float (&v)[VEC])
+{
+    if (t >= 0) { load_vec<T, VEC>((const T*)a.x + at(a.xs, a.q.row(t), b) + c, v); return; }
+    const long long i = t + a.K - 1;
+    if (i >= 0 && a.state) { load_vec<T, VEC>((const T*)a.state + (b * (a.K - 1) + i) * a.D + c, v); return; }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 0.f;
+}
+// KP taps, K of them the operator's: the first KP - K are zero
+template <int VEC, int KP> __device__ __forceinline__ void load_taps(const ConvArgs& a, int c, float (&w)[KP][VEC], float (&bias)[VEC])
+{
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        bias[e] = a.bias ? a.bias[c + e] : 0.f;
+#pragma unroll
+        for (int j = 0; j < KP; ++j) w[j][e] = j >= KP - a.K ? a.weight[(long long)(c + e) * a.K + j - (KP - a.K)] : 0.f;
+    }
+}
+
+// block 256 = 256 / CL items (a run of a sequence) x CL lanes of VEC channels
+template <typename T, int VEC, int KP, int CL>
+__global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a)
+{
+    const int c = (blockIdx.y * CL + threadIdx.x % CL) * VEC;
+    const long long item = (long long)blockIdx.x * (256 / CL) + threadIdx.x / CL;
+    const long long b = item / a.runs, t0 = (item % a.runs) * RUN;
+    if (c >= a.D || b >= a.q.B) return;
+    const long long len = a.q.length(b);
+    if (t0 >= len && t0 > 0) return;
+    const long long t1 = t0 + RUN < len ? t0 + RUN : len;
+    float w[KP][VEC], bias[VEC], win[KP][VEC];
+    load_taps<VEC, KP>(a, c, w, bias);
+#pragma unroll
+    for (int j = 0; j < KP - 1; ++j) input_at<T, VEC>(a, t0 - (KP - 1) + j, b, c, win[j]);
+#pragma unroll 4
+    for (long long t = t0; t < t1; ++t) {
+        const long long r = a.q.row(t);
+        load_vec<T, VEC>((const T*)a.x + at(a.xs, r, b) + c, win[KP - 1]);
+        float out[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float s = bias[e];
+#pragma unroll
+            for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+            out[e] = a.silu ? s * sigmoid(s) : s;
+#pragma unroll
+            for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+        }
+        store_vec<T, VEC>((T*)a.y + at(a.ys, r, b) + c, out);
+    }
+    if (t1 == len && a.last)
+#pragma unroll
+        for (int j = 0; j < KP - 1; ++j)
+            if (j >= KP - a.K) store_vec<T, VEC>((T*)a.last + (b * (a.K - 1) + j - (KP - a.K)) * a.D + c, win[j]);
+}
+
+template <typename T, int VEC, int KP, int CL>
+__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a)
+{
+    constexpr int IL = 256 / CL;
+    __shared__ float red[IL][CL][VEC];
+    const int cl = threadIdx.x % CL, il = threadIdx.x / CL, c = (blockIdx.y * CL + cl) * VEC;
+    float dw[KP][VEC] = {}, db[VEC] = {};
+    if (c < a.D) {
+        float w[KP][VEC], bias[VEC];
+        load_taps<VEC, KP>(a, c, w, bias);
+        const long long items = a.q.B * a.runs;
+        for (long long item = (long long)blockIdx.x * IL + il; item < items; item += (long long)gridDim.x * IL) {
+            const long long b = item / a.runs, t0 = (item % a.runs) * RUN, len = a.q.length(b);
+            if (t0 >= len && t0 > 0) continue;
+            const long long t1 = t0 + RUN < len ? t0 + RUN : len, first = t0 == 0 ? -(long long)(a.K - 1) : t0;
+            float win[KP][VEC], dp[KP][VEC];                 // inputs t - KP + 1 .. t; dp[j] = dpre of step t - j
+#pragma unroll
+            for (int j = 0; j < KP - 1; ++j) input_at<T, VEC>(a, t0 - (KP - 1) + j, b, c, win[j]);
+#pragma unroll
+            for (int j = 0; j < KP; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) dp[j][e] = 0.f;
+#pragma unroll 4
+            for (long long t = t0; t < t1 + KP - 1; ++t) {
+#pragma unroll
+                for (int j = KP - 1; j > 0; --j)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
+                if (t < len) {
+                    const long long r = a.q.row(t);
+                    float dy[VEC];
+                    load_vec<T, VEC>((const T*)a.x + at(a.xs, r, b) + c, win[KP - 1]);
+                    load_vec<T, VEC>((const T*)a.dy + at(a.dys, r, b) + c, dy);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        float s = bias[e];
+#pragma unroll
+                        for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+                        if (a.silu) { const float g = sigmoid(s); dy[e] *= g * fmaf(s, 1.0f - g, 1.0f); }
+                        dp[0][e] = dy[e];
+                        if (t < t1) {
+                            db[e] += dy[e];
+#pragma unroll
+                            for (int j = 0; j < KP; ++j) dw[j][e] = fmaf(dy[e], win[j][e], dw[j][e]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) dp[0][e] = 0.f;
+                }
+                const long long tt = t - (KP - 1);           // the step whose input's gradient is complete
+                if (tt < first || tt >= t1) continue;
+                float dx[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    dx[e] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < KP; ++j) dx[e] = fmaf(w[j][e], dp[j][e], dx[e]);
+                }
+                const long long i = tt - (len - (a.K - 1));
+                if (i >= 0 && a.dlast) {                     // the last K - 1 inputs are the new state too
+                    float g[VEC];
+                    load_vec<T, VEC>((const T*)a.dlast + (b * (a.K - 1) + i) * a.D + c, g);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) dx[e] += g[e];
+                }
+                if (tt >= 0) store_vec<T, VEC>((T*)a.dx + at(a.ys, a.q.row(tt), b) + c, dx);
+                else if (a.dstate) store_vec<T, VEC>((T*)a.dstate + (b * (a.K - 1) + tt + a.K - 1) * a.D + c, dx);
+            }
+        }
+    }
+    // the items of a block, in order, one column of the partial sums at a time
+#pragma unroll
+    for (int j = 0; j <= KP; ++j) {
+        if (j < KP && j < KP - a.K) continue;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) red[il][cl][e] = j < KP ? dw[j < KP ? j : 0][e] : db[e];
+        __syncthreads();
+        if (il == 0 && c < a.D) {
+            const int col = j < KP ? j - (KP - a.K) : a.K;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float s = red[0][cl][e];
+                for (int i = 1; i < IL; ++i) s += red[i][cl][e];
+                a.part[((long long)blockIdx.x * (a.K + 1) + col) * a.D + c + e] = s;
+            }
+        }
+    }
+}
+
+// [K + 1, D] -> dweight [D, K], dbias [D]
+__global__ __launch_bounds__(256) void k_conv_unpack(const float* __restrict__ sums, int D, int K, float* __restrict__ dw, float* __restrict__ db)
+{
+    const int e = blockIdx.x * 256 + threadIdx.x;
+    if (e >= D * (K + 1)) return;
+    const int k = e / D, d = e % D;
+    if (k < K) dw[(long long)d * K + k] = sums[e];
+    else if (db) db[d] = sums[e];
+}
+
+template <typename T, int KP>
+__global__ __launch_bounds__(256) void k_conv_step(long long B, int D, int K, const T* __restrict__ x, long long ldx, const T* state,
+                                                   const float* __restrict__ weight, const float* __restrict__ bias, int silu, T* __restrict__ y, T* next)
+{
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= B * D) return;
+    const long long b = e / D;
+    const int d = (int)(e % D);
+    T in[KP];                                  // all of a channel's state is read before any of it is written: next may be the state itself
+#pragma unroll
+    for (int j = 0; j < KP - 1; ++j)
+        if (j >= KP - K) in[j] = state[(b * (K - 1) + j - (KP - K)) * D + d];
+    in[KP - 1] = x[b * ldx + d];
+    float s = bias ? bias[d] : 0.f;
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+        if (j >= KP - K) s = fmaf(weight[(long long)d * K + j - (KP - K)], to_f32(in[j]), s);
+    y[e] = from_f32<T>(silu ? s * sigmoid(s) : s);
+#pragma unroll
+    for (int j = 0; j < KP - 1; ++j)
+        if (j >= KP - K) next[(b * (K - 1) + j - (KP - K)) * D + d] = in[j + 1];
+}
+
+int taps(long long K) { return K <= 2 ? 2 : K <= 4 ? 4 : 8; }
+
+template <typename T, int VEC, int KP, int CL> void launch_conv(const ConvArgs& a, bool bwd, unsigned blocks, hipStream_t st)
+{
+    const dim3 grid(blocks, (unsigned)((a.D + CL * VEC - 1) / (CL * VEC)));
+    if (bwd) k_conv_bwd<T, VEC, KP, CL><<<grid, 256, 0, st>>>(a);
+    else k_conv_fwd<T, VEC, KP, CL><<<grid, 256, 0, st>>>(a);
+}
+template <typename T, int VEC, int KP> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
+{
+    if (cl == 16) launch_conv<T, VEC, KP, 16>(a, bwd, blocks, st);
+    else launch_conv<T, VEC, KP, 64>(a, bwd, blocks, st);
+}
+template <typename T, int VEC> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
+{
+    switch (taps(a.K)) {
+        case 2: launch_conv<T, VEC, 2>(a, bwd, cl, blocks, st); break;
+        case 4: launch_conv<T, VEC, 4>(a, bwd, cl, blocks, st); break;
+        default: launch_conv<T, VEC, 8>(a, bwd, cl, blocks, st);
+    }
+}
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// 16-byte accesses where every row that a lane touches begins on one; single elements otherwise
+bool conv_vec(const ConvArgs& a, int elem)
+{
+    const int E = 16 / elem;
+    const long long s = a.xs.t | a.xs.b | a.ys.t | a.ys.b | a.dys.t | a.dys.b | a.D;
+    return s % E == 0 && aligned16(a.x) && aligned16(a.state) && aligned16(a.dy) && aligned16(a.dlast) && aligned16(a.y) && aligned16(a.last) &&
+           aligned16(a.dx) && aligned16(a.dstate);
+}
+long long conv_items(long long T, long long B) { const long long r = (T + RUN - 1) / RUN; return B * (r > 0 ? r : 1); }
+int conv_lanes(long long D, int vec) { return D <= 16 * vec ? 16 : 64; }
+long long conv_blocks(long long items, int cl) { return (items + 256 / cl - 1) / (256 / cl); }
+unsigned conv_sum_blocks(long long items, int cl) { const long long b = conv_blocks(items, cl); return (unsigned)(b < MAX_SUM_BLOCKS ? b : MAX_SUM_BLOCKS); }
+
+int conv_check(const char* what, int dtype, long long T, long long B, long long D, long long K, const void* x, const float* w, const int64_t* strides)
+{
+    if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "%s: type %d (fp32 and bf16 are supported)", what, dtype);
+    if (T < 0 || B < 0 || D < 1 || D > (1 << 20) || K < 1) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld K=%lld", what, T, B, D, K);
+    if (K > 8) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld taps (at most 8)", what, K);
+    if (!strides || !w || (B > 0 && T > 0 && !x)) PPK_FAIL(PPK_ERR_NULL, "%s: null pointer", what);
+    if (conv_blocks(conv_items(T, B), 64) > 0x7fffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "%s: T=%lld B=%lld", what, T, B);
+    return PPK_OK;
+}
+
+template <typename T> int conv_run(const ConvArgs& a, bool bwd, long long items, hipStream_t st)
+{
+    constexpr int E = 16 / (int)sizeof(T);
+    const bool vec = conv_vec(a, (int)sizeof(T));
+    const int cl = conv_lanes(a.D, vec ? E : 1);
+    const unsigned blocks = bwd ? conv_sum_blocks(items, cl) : (unsigned)conv_blocks(items, cl);
+    if (vec) launch_conv<T, E>(a, bwd, cl, blocks, st);
+    else launch_conv<T, 1>(a, bwd, cl, blocks, st);
+    return (int)blocks;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ppk_causal_conv_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
+                        const void* x, const float* weight, const float* bias, const void* state, int silu, void* y, void* new_state,
+                        const int64_t* strides_host, ppk_stream_t stream)
+{
+    int rc = conv_check("causal_conv_fwd", dtype, T, B, D, K, x, weight, strides_host);
+    if (rc) return rc;
+    if (B == 0) return PPK_OK;
+    if (T > 0 && !y) PPK_FAIL(PPK_ERR_NULL, "causal_conv_fwd: null pointer");
+    ConvArgs a = {};
+    a.q = {step_off, lengths, T, B};
+    a.D = (int)D; a.K = (int)K; a.runs = (int)(conv_items(T, 1));
+    a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.y = y; a.last = K > 1 ? new_state : nullptr; a.silu = silu;
+    a.xs = {strides_host[0], strides_host[1]}; a.ys = {strides_host[2], strides_host[3]};
+    if (dtype == PPK_F32) conv_run<float>(a, false, conv_items(T, B), (hipStream_t)stream);
+    else conv_run<bf16_t>(a, false, conv_items(T, B), (hipStream_t)stream);
+    PPK_CHECK_LAUNCH("causal_conv_fwd");
+    return PPK_OK;
+}
+
+size_t ppk_causal_conv_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t K)
+{
+    if (T < 0 || B < 0 || D < 1 || K < 1) return 0;
+    const size_t cols = (size_t)(K + 1) * (size_t)D;
+    return ppk_align_up((size_t)MAX_SUM_BLOCKS * cols * 4, 256) + ppk::partial_sum_ws_bytes(MAX_SUM_BLOCKS, (long long)cols) + ppk_align_up(cols * 4, 256);
+}
+
+int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
+                        const void* x, const float* weight, const float* bias, const void* state, int silu, const void* dy, const void* dnew_state,
+                        void* dx, float* dweight, float* dbias, void* dstate, const int64_t* strides_host,
+                        void* workspace, size_t ws_bytes, ppk_stream_t stream)
+{
+    int rc = conv_check("causal_conv_bwd", dtype, T, B, D, K, x, weight, strides_host);
+    if (rc) return rc;
+    if (!dweight || !workspace || (B > 0 && T > 0 && (!dy || !dx))) PPK_FAIL(PPK_ERR_NULL, "causal_conv_bwd: null pointer");
+    if (ws_bytes < ppk_causal_conv_bwd_workspace_bytes(T, B, D, K)) PPK_FAIL(PPK_ERR_WS, "causal_conv_bwd: workspace of %zu bytes", ws_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    const long long cols = (K + 1) * D;
+    char* cur = (char*)workspace;
+    ConvArgs a = {};
+    a.part = (float*)ppk_carve(cur, (size_t)MAX_SUM_BLOCKS * (size_t)cols * 4);
+    void* sum_ws = ppk_carve(cur, ppk::partial_sum_ws_bytes(MAX_SUM_BLOCKS, cols));
+    float* sums = (float*)cur;
+    a.q = {step_off, lengths, T, B};
+    a.D = (int)D; a.K = (int)K; a.runs = (int)(conv_items(T, 1));
+    a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.dy = dy; a.silu = silu; a.dx = dx;
+    a.dlast = K > 1 ? dnew_state : nullptr; a.dstate = K > 1 ? dstate : nullptr;
+    a.xs = {strides_host[0], strides_host[1]}; a.dys = {strides_host[2], strides_host[3]}; a.ys = {strides_host[4], strides_host[5]};
+    int blocks = 0;
+    if (B > 0) blocks = dtype == PPK_F32 ? conv_run<float>(a, true, conv_items(T, B), st) : conv_run<bf16_t>(a, true, conv_items(T, B), st);
+    rc = ppk::partial_sum(a.part, blocks, cols, sums, sum_ws, st);
+    if (rc) return rc;
+    k_conv_unpack<<<(unsigned)((cols + 255) / 256), 256, 0, st>>>(sums, (int)D, (int)K, dweight, dbias);
+    PPK_CHECK_LAUNCH("causal_conv_bwd");
+    return PPK_OK;
+}
+
+int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void* x, int64_t ldx, const void* state, const float* weight,
+                         const float* bias, int silu, void* y, void* new_state, ppk_stream_t stream)
+{
+    if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: type %d (fp32 and bf16 are supported)", dtype);
+    if (B < 0 || D < 1 || K < 1 || ldx < 0) PPK_FAIL(PPK_ERR_SHAPE, "causal_conv_step: B=%lld D=%lld K=%lld", (long long)B, (long long)D, (long long)K);
+    if (K > 8) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: %lld taps (at most 8)", (long long)K);
+    if (B * D > 0xffffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: B=%lld D=%lld", (long long)B, (long long)D);
+    if (B == 0) return PPK_OK;
+    if (!x || !weight || !y || (K > 1 && (!state || !new_state))) PPK_FAIL(PPK_ERR_NULL, "causal_conv_step: null pointer");
+    const unsigned blocks = (unsigned)((B * D + 255) / 256);
+    hipStream_t st = (hipStream_t)stream;
+#define STEP(T, KP) k_conv_step<T, KP><<<blocks, 256, 0, st>>>(B, (int)D, (int)K, (const T*)x, ldx, (const T*)state, weight, bias, silu, (T*)y, (T*)new_state)
+    const int kp = taps(K);
+    if (dtype == PPK_F32) { if (kp == 2) STEP(float, 2); else if (kp == 4) STEP(float, 4); else STEP(float, 8); }
+    else { if (kp == 2) STEP(bf16_t, 2); else if (kp == 4) STEP(bf16_t, 4); else STEP(bf16_t, 8); }
+#undef STEP
+    PPK_CHECK_LAUNCH("causal_conv_step");
+    return PPK_OK;
+}
+
+}  // extern "C"

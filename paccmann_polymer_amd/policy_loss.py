@@ -41,6 +41,10 @@ def _rows_of(logits):
     return logits.contiguous()
 
 
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _ld(logits):
     return max(logits.stride(0), logits.shape[1])
 
@@ -48,14 +52,14 @@ def _ld(logits):
 class _TokenLogProbs(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, logits, targets, ignore_index, temperature):
+    def forward(ctx, logits, targets, ignore_index, temperature, want_grad):
         code = _check_logits('token_log_probs', logits, targets, temperature)
         dev = _C.one_device(logits, targets)
         x, t = _rows_of(logits), targets.contiguous()
         rows, V = x.shape
         with torch.cuda.device(dev):
             logp = torch.empty(rows, dtype=torch.float32, device=dev)
-            saved = torch.empty(rows, 2, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+            saved = torch.empty(rows, 2, dtype=torch.float32, device=dev) if want_grad else None
             _C.check(_lib.ppk_token_logp_fwd(code, _C.p(x), _ld(x), _C.p(t), rows, V, ignore_index, temperature, _C.p(logp), _C.p(saved), _C.stream()))
         if saved is not None:
             ctx.save_for_backward(x, t, saved)
@@ -72,7 +76,7 @@ class _TokenLogProbs(torch.autograd.Function):
             d = torch.empty(rows, V, dtype=x.dtype, device=x.device)
             g = dlogp.to(torch.float32).contiguous()
             _C.check(_lib.ppk_token_logp_bwd(code, _C.p(x), _ld(x), _C.p(t), rows, V, ignore_index, temperature, _C.p(saved), _C.p(g), _C.p(d), V, _C.stream()))
-        return d, None, None, None
+        return d, None, None, None, None
 
 
 def token_log_probs(logits, targets, ignore_index=0, temperature=1.0):
@@ -80,7 +84,7 @@ def token_log_probs(logits, targets, ignore_index=0, temperature=1.0):
 
     logits [rows, V] fp32 or bf16 (rows may be strided), targets [rows] int64.  Differentiable in the logits.  A target that is
     neither `ignore_index` nor in [0, V) gives NaN (nothing is read through it, and nothing synchronises)."""
-    return _TokenLogProbs.apply(logits, targets, int(ignore_index), float(temperature))
+    return _TokenLogProbs.apply(logits, targets, int(ignore_index), float(temperature), _wants_grad(logits))
 
 
 def _policy_call(code, x, t, old, adv, ref, args, want_grad):
@@ -103,10 +107,10 @@ class _PolicyLoss(torch.autograd.Function):
     gradient, which costs nothing but a look where that is 1."""
 
     @staticmethod
-    def forward(ctx, logits, targets, old, adv, ref, args):
+    def forward(ctx, logits, targets, old, adv, ref, args, want_grad):
         code = _C.dtype_code(logits, 'policy_loss')
         x = _rows_of(logits)
-        loss, stats, d = _policy_call(code, x, targets, old, adv, ref, args, ctx.needs_input_grad[0])
+        loss, stats, d = _policy_call(code, x, targets, old, adv, ref, args, want_grad)
         if d is not None:
             ctx.save_for_backward(x, targets, old, adv, ref)
             ctx.grad, ctx.code, ctx.args = d, code, args
@@ -123,7 +127,7 @@ class _PolicyLoss(torch.autograd.Function):
         with torch.cuda.device(x.device):
             s = dloss.to(torch.float32).reshape(1).contiguous()
             _C.check(_lib.ppk_scale_unless_one(ctx.code, _C.p(d), d.numel(), _C.p(s), _C.stream()))
-        return d, None, None, None, None, None
+        return d, None, None, None, None, None, None
 
 
 def policy_loss(logits, targets, old_log_probs, advantages, ref_log_probs=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
@@ -151,4 +155,4 @@ def policy_loss(logits, targets, old_log_probs, advantages, ref_log_probs=None, 
     ref = None if ref_log_probs is None else _row_values(what, 'ref_log_probs', ref_log_probs, rows)
     _C.one_device(logits, targets, old, adv, ref)
     args = (float(clip_low), float(clip_high), float(kl_coef), int(ignore_index), float(temperature))
-    return _PolicyLoss.apply(logits, targets.contiguous(), old, adv, ref, args)
+    return _PolicyLoss.apply(logits, targets.contiguous(), old, adv, ref, args, _wants_grad(logits))

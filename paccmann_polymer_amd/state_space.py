@@ -1,0 +1,435 @@
+"""Causal convolution and selective state space scan: the operators of a sequence layer beside the StackGRU of K1
+(`stack_gru_vae`), for packed batches, for rectangular ones, and for single tokens while generating.  The reference's only sequence
+operator is the recurrent one (paccmann_polymer/models/paccmann_encoder.py:166-168); these have no counterpart in it.
+
+Batches.  `x` is a `PackedSequence` (its `.data` [rows, D]), rows [rows, D] of a packed batch with the `plan` that `packed_rows` made of
+its batch sizes, or a rectangular tensor [T, B, D] of any strides (a batch-first one goes in as `x.transpose(0, 1)`).  The other
+per-step tensors come in the same form.  States [B, ...] are in packed (sorted) order, as K1's `h0` is: permute them with the
+PackedSequence's `sorted_indices`.  A program that works on the same packing again keeps the plan: making one copies a few
+integers to the device, which cannot be captured into a graph.
+
+Types.  Activations are fp32 or bf16 (all of a call the same); parameters, scan states and their gradients are fp32.  The
+convolution's state holds inputs, in their type.  Kernels: csrc/ppk_causal_conv.hip, csrc/ppk_selective_scan.hip.
+
+A backward pass inside a graph capture needs leaves that no eager autograd graph holds at that time (autograd would make the
+capturing stream wait for the eager one, which ends the process): take `torch.autograd.grad` of fresh detached leaves, or capture first.
+"""
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+from torch.nn.utils.rnn import PackedSequence
+
+from . import _C
+
+_lib = _C.lib
+MAX_TAPS = 8
+MAX_STATES = 64
+
+
+class PackedRows(NamedTuple):
+    """What the kernels need of a packed batch; `packed_rows` makes it."""
+    offsets: torch.Tensor            # [T + 1] int64, device: step t owns rows offsets[t] .. offsets[t + 1]
+    lengths: torch.Tensor            # [B] int64, device
+    tiles: torch.Tensor              # [B + 1] int64, device: first kept state of each sequence
+    steps: int
+    sequences: int
+    rows: int
+    kept: int                        # kept states in all
+
+
+def packed_rows(batch_sizes, device, sequences: Optional[int] = None) -> PackedRows:
+    """The plan of a packed batch from its `PackedSequence.batch_sizes` (or the PackedSequence itself).  `sequences`: how many there
+    are, where some have no steps at all (they are the last ones, and keep their states)."""
+    if isinstance(batch_sizes, PackedSequence):
+        batch_sizes = batch_sizes.batch_sizes
+    bs = torch.as_tensor(batch_sizes).to('cpu', torch.int64).reshape(-1)
+    T = bs.numel()
+    B = int(bs[0]) if T else 0
+    if T and (int(bs.min()) < 1 or bool((bs[1:] > bs[:-1]).any())):
+        raise ValueError('packed_rows: batch sizes must be positive and must not increase')
+    if sequences is not None:
+        if int(sequences) < B:
+            raise ValueError(f'packed_rows: {int(sequences)} sequences, but {B} have a first step')
+        B = int(sequences)
+    tile = int(_lib.ppk_selective_scan_tile())
+    off = torch.zeros(T + 1, dtype=torch.int64)
+    off[1:] = torch.cumsum(bs, 0)
+    # length of sequence b: how many steps have more than b rows
+    lengths = torch.zeros(B, dtype=torch.int64)
+    if T:
+        lengths[:int(bs[0])] = T - torch.searchsorted(bs.flip(0), torch.arange(int(bs[0])), right=True)
+    tiles = torch.zeros(B + 1, dtype=torch.int64)
+    tiles[1:] = torch.cumsum((lengths + tile - 1) // tile, 0)
+    sent = torch.cat([off, lengths, tiles]).to(device)
+    return PackedRows(sent[:T + 1], sent[T + 1:T + 1 + B], sent[T + 1 + B:], T, B, int(off[-1]), int(tiles[-1]))
+
+
+def _data(t):
+    return t.data if isinstance(t, PackedSequence) else t
+
+
+class _Batch:
+    """The layout of a call: packed or rectangular, and how its tensors are addressed."""
+
+    def __init__(self, what, x, plan):
+        if isinstance(x, PackedSequence) and plan is None:
+            plan = packed_rows(x.batch_sizes, x.data.device)
+        data = _data(x)
+        if not torch.is_tensor(data):
+            raise TypeError(f'{what}: x must be a tensor or a PackedSequence')
+        self.what, self.plan = what, plan
+        if plan is not None:
+            if not isinstance(plan, PackedRows):
+                raise TypeError(f'{what}: plan must be what packed_rows gives')
+            if data.dim() != 2 or data.shape[0] != plan.rows:
+                raise ValueError(f'{what}: x must be [{plan.rows}, D] for this plan')
+            self.T, self.B, self.rows = plan.steps, plan.sequences, plan.rows
+            self.lead, self.out_rows = (plan.rows,), (1, 1)
+        else:
+            if data.dim() != 3:
+                raise ValueError(f'{what}: x must be [T, B, D], or the rows of a packed batch with its plan')
+            self.T, self.B = data.shape[:2]
+            self.rows = self.T * self.B
+            self.lead = (self.T, self.B)
+            # outputs lie as x does: batch-first where a sequence's steps are next to each other
+            self.batch_first = data.stride(0) < data.stride(1)
+            self.out_rows = (1, self.T) if self.batch_first else (self.B, 1)
+        self.D = data.shape[-1]
+        if self.D < 1:
+            raise ValueError(f'{what}: x has no channels')
+
+    def take(self, name, t, tail, dtype):
+        """A per-step tensor [lead, tail], the elements of its last dimension next to each other."""
+        t = _data(t)
+        if not torch.is_tensor(t) or tuple(t.shape) != (*self.lead, *tail):
+            raise ValueError(f'{self.what}: {name} must be {[*self.lead, *tail]}, not {list(t.shape) if torch.is_tensor(t) else t}')
+        if t.dtype != dtype:
+            raise TypeError(f'{self.what}: {name} must be {dtype}, as x is')
+        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+    def strides(self, t):
+        """Of a step and of a sequence, in elements."""
+        if t is None:
+            return (0, 0)
+        return (t.stride(0), t.stride(0)) if self.plan is not None else (t.stride(0), t.stride(1))
+
+    def new(self, tail, dtype, device):
+        if self.plan is None and self.batch_first:
+            return torch.empty(self.B, self.T, *tail, dtype=dtype, device=device).transpose(0, 1)
+        return torch.empty(*self.lead, *tail, dtype=dtype, device=device)
+
+    def pointers(self):
+        p = self.plan
+        return (None, None) if p is None else (_C.p(p.offsets), _C.p(p.lengths))
+
+    def tensors(self):
+        return () if self.plan is None else (self.plan.offsets, self.plan.lengths, self.plan.tiles)
+
+
+def _param(what, name, t, shape):
+    if not torch.is_tensor(t) or tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{what}: {name} must be {list(shape)}')
+    if t.dtype != torch.float32:
+        raise TypeError(f'{what}: {name} must be float32')
+
+
+def _ints(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
+
+
+def _ws(nbytes, device):
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+def _like(x, y):
+    """y in the form that x came in."""
+    return PackedSequence(y, x.batch_sizes, x.sorted_indices, x.unsorted_indices) if isinstance(x, PackedSequence) else y
+
+
+# ------------------------------------------------------------------------------------------------------- causal convolution
+class _CausalConv(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, batch, silu, x, weight, bias, state):
+        dev = x.device
+        weight, bias, state = weight.contiguous(), _contiguous(bias), _contiguous(state)
+        D, K = weight.shape
+        with torch.cuda.device(dev):
+            y = batch.new((D,), x.dtype, dev)
+            last = torch.empty(batch.B, K - 1, D, dtype=x.dtype, device=dev)
+            off, lengths = batch.pointers()
+            _C.check(_lib.ppk_causal_conv_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.p(x), _C.p(weight), _C.p(bias), _C.p(state),
+                                              silu, _C.p(y), _C.p(last), _ints(*batch.strides(x), *batch.strides(y)), _C.stream()))
+        ctx.save_for_backward(x, weight, bias, state)
+        ctx.batch, ctx.silu = batch, silu
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, weight, bias, state = ctx.saved_tensors
+        batch, dev = ctx.batch, x.device
+        D, K = weight.shape
+        with torch.cuda.device(dev):
+            dy = torch.zeros(*batch.lead, D, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (D,), x.dtype)
+            dlast = _contiguous(dlast)
+            dx = batch.new((D,), x.dtype, dev)
+            dw = torch.empty_like(weight)
+            db = None if bias is None else torch.empty_like(bias)
+            ds = None if state is None else torch.empty_like(state)
+            off, lengths = batch.pointers()
+            wsb = _lib.ppk_causal_conv_bwd_workspace_bytes(batch.T, batch.B, D, K)
+            ws = _ws(wsb, dev)
+            _C.check(_lib.ppk_causal_conv_bwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.p(x), _C.p(weight), _C.p(bias), _C.p(state), ctx.silu,
+                                              _C.p(dy), _C.p(dlast), _C.p(dx), _C.p(dw), _C.p(db), _C.p(ds),
+                                              _ints(*batch.strides(x), *batch.strides(dy), *batch.strides(dx)), _C.p(ws), wsb, _C.stream()))
+        return None, None, dx, dw, db, ds
+
+
+def _conv_params(what, weight, bias, D, activation):
+    if not torch.is_tensor(weight) or weight.dim() != 2 or weight.shape[0] != D or weight.shape[1] < 1:
+        raise ValueError(f'{what}: weight must be [{D}, taps]')
+    if weight.shape[1] > MAX_TAPS:
+        raise ValueError(f'{what}: at most {MAX_TAPS} taps')
+    _param(what, 'weight', weight, weight.shape)
+    if bias is not None:
+        _param(what, 'bias', bias, (D,))
+    if activation not in (None, 'silu'):
+        raise ValueError(f"{what}: activation must be None or 'silu'")
+    return int(activation == 'silu')
+
+
+def causal_conv(x, weight, bias=None, plan: Optional[PackedRows] = None, state=None, activation='silu'):
+    """Each channel's causal convolution over its sequence: y_t = act(bias + sum_k weight[:, k] x_{t - K + 1 + k}), and the new state.
+
+    weight [D, K] fp32 (K <= 8, the last tap is the current step's), bias [D] fp32.  state [B, K - 1, D] in x's type: the inputs
+    before the first step, the oldest first (None: zeros).  Returns (y like x, new state [B, K - 1, D]: each sequence's last inputs).
+    Differentiable in x, weight, bias and state."""
+    what = 'causal_conv'
+    batch = _Batch(what, x, plan)
+    data = _data(x)
+    _C.dtype_code(data, what)
+    data = batch.take('x', data, (batch.D,), data.dtype)
+    silu = _conv_params(what, weight, bias, batch.D, activation)
+    K = weight.shape[1]
+    if state is not None:
+        if not torch.is_tensor(state) or tuple(state.shape) != (batch.B, K - 1, batch.D):
+            raise ValueError(f'{what}: state must be {[batch.B, K - 1, batch.D]}')
+        if state.dtype != data.dtype:
+            raise TypeError(f'{what}: state must be {data.dtype}, as x is')
+    _C.one_device(data, weight, bias, state, *batch.tensors())
+    y, last = _CausalConv.apply(batch, silu, data, weight, bias, state)
+    return _like(x, y), last
+
+
+def _extent(t):
+    """The addresses that a tensor's elements lie between."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a, b):
+    """Whether the memory that two tensors span has a part in common."""
+    if a is None or b is None or not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a0 < b1 and b0 < a1
+
+
+def _step_out(what, state, out, others):
+    """Where a step writes its new state: `out`, or fresh memory.  `out` may be the state itself, but share memory with nothing else."""
+    if out is None:
+        return torch.empty(state.shape, dtype=state.dtype, device=state.device)
+    if not torch.is_tensor(out) or out.shape != state.shape or out.dtype != state.dtype or out.device != state.device or not out.is_contiguous():
+        raise ValueError(f'{what}: out must be a contiguous tensor like state')
+    if out.data_ptr() != state.data_ptr() and _overlap(out, state):
+        raise ValueError(f'{what}: out overlaps state without being it')
+    for t in others:
+        if _overlap(t, out):
+            raise ValueError(f'{what}: out shares memory with an input')
+    return out
+
+
+def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
+    """One token of each of B sequences: x [B, D], state [B, K - 1, D] -> (y [B, D], new state).  `out`: where the new state goes
+    (it may be `state`: updated in place).  Inference only: training goes through `causal_conv`."""
+    what = 'causal_conv_step'
+    if not torch.is_tensor(x) or x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f'{what}: x must be [B, D]')
+    code = _C.dtype_code(x, what)
+    B, D = x.shape
+    silu = _conv_params(what, weight, bias, D, activation)
+    K = weight.shape[1]
+    if not torch.is_tensor(state) or tuple(state.shape) != (B, K - 1, D):
+        raise ValueError(f'{what}: state must be {[B, K - 1, D]}')
+    if state.dtype != x.dtype:
+        raise TypeError(f'{what}: state must be {x.dtype}, as x is')
+    dev = _C.one_device(x, state, weight, bias)
+    with torch.no_grad(), torch.cuda.device(dev):
+        x = x.detach()
+        x = x if x.stride(1) == 1 or D == 1 else x.contiguous()
+        weight, bias = weight.contiguous(), _contiguous(bias)
+        new = _step_out(what, state, out, (x, weight, bias))
+        state = state.contiguous()
+        y = torch.empty(B, D, dtype=x.dtype, device=dev)
+        _C.check(_lib.ppk_causal_conv_step(code, B, D, K, _C.p(x), x.stride(0), _C.p(state), _C.p(weight), _C.p(bias), silu, _C.p(y), _C.p(new), _C.stream()))
+    return y, new
+
+
+# ------------------------------------------------------------------------------------------------------------ selective scan
+def _scan_strides(batch, x, raw, B, C, z, rows, dy):
+    bt, bb = batch.strides(B)
+    ct, cb = batch.strides(C)
+    return _ints(*batch.strides(x), *batch.strides(raw), bt, bb, B.stride(-2), ct, cb, C.stride(-2), *batch.strides(z), *rows, *batch.strides(dy))
+
+
+class _SelectiveScan(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, batch, softplus, want_grad, x, dt, A, B, C, D, z, dt_bias, state):
+        dev = x.device
+        A, D, dt_bias, state = A.contiguous(), _contiguous(D), _contiguous(dt_bias), _contiguous(state)
+        N, G, width = A.shape[1], B.shape[-2], batch.D
+        tiles = None if batch.plan is None else batch.plan.tiles
+        with torch.cuda.device(dev):
+            y = batch.new((width,), x.dtype, dev)
+            last = torch.empty(batch.B, width, N, dtype=torch.float32, device=dev)
+            kept = None
+            if want_grad:
+                tile = int(_lib.ppk_selective_scan_tile())
+                n = batch.plan.kept if batch.plan is not None else batch.B * ((batch.T + tile - 1) // tile)
+                kept = torch.empty(n, width, N, dtype=torch.float32, device=dev)
+            off, lengths = batch.pointers()
+            _C.check(_lib.ppk_selective_scan_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, off, lengths, _C.p(tiles), _C.p(x), _C.p(dt), _C.p(A),
+                                                 _C.p(B), _C.p(C), _C.p(D), _C.p(z), _C.p(dt_bias), _C.p(state), softplus, _C.p(y), _C.p(last), _C.p(kept),
+                                                 _scan_strides(batch, x, dt, B, C, z, batch.out_rows, None), _C.stream()))
+        if kept is not None:
+            ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, kept)
+            ctx.batch, ctx.softplus, ctx.has_state = batch, softplus, state is not None
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, dt, A, B, C, D, z, dt_bias, kept = ctx.saved_tensors
+        batch, dev = ctx.batch, x.device
+        N, G, width = A.shape[1], B.shape[-2], batch.D
+        tiles = None if batch.plan is None else batch.plan.tiles
+        with torch.cuda.device(dev):
+            dy = torch.zeros(*batch.lead, width, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (width,), x.dtype)
+            dlast = _contiguous(dlast)
+            dx, draw = batch.new((width,), x.dtype, dev), batch.new((width,), x.dtype, dev)
+            dz = None if z is None else batch.new((width,), x.dtype, dev)
+            dB, dC = batch.new((G, N), x.dtype, dev), batch.new((G, N), x.dtype, dev)
+            dA = torch.empty_like(A)
+            dD = None if D is None else torch.empty_like(D)
+            dbias = None if dt_bias is None else torch.empty_like(dt_bias)
+            dstate = torch.empty(batch.B, width, N, dtype=torch.float32, device=dev) if ctx.has_state else None
+            off, lengths = batch.pointers()
+            wsb = _lib.ppk_selective_scan_bwd_workspace_bytes(batch.T, batch.B, width, N, G, batch.rows)
+            ws = _ws(wsb, dev)
+            _C.check(_lib.ppk_selective_scan_bwd(
+                _C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, batch.rows, off, lengths, _C.p(tiles), _C.p(x), _C.p(dt), _C.p(A), _C.p(B), _C.p(C),
+                _C.p(D), _C.p(z), _C.p(dt_bias), ctx.softplus, _C.p(kept), _C.p(dy), _C.p(dlast), _C.p(dx), _C.p(draw), _C.p(dA), _C.p(dB), _C.p(dC),
+                _C.p(dD), _C.p(dz), _C.p(dbias), _C.p(dstate), _scan_strides(batch, x, dt, B, C, z, batch.out_rows, dy), _C.p(ws), wsb, _C.stream()))
+        return None, None, None, dx, draw, dA, dB, dC, dD, dz, dbias, dstate
+
+
+def _scan_params(what, A, D, dt_bias, width):
+    if not torch.is_tensor(A) or A.dim() != 2 or A.shape[0] != width or A.shape[1] < 1:
+        raise ValueError(f'{what}: A must be [{width}, states]')
+    if A.shape[1] > MAX_STATES:
+        raise ValueError(f'{what}: at most {MAX_STATES} states a channel')
+    _param(what, 'A', A, A.shape)
+    if D is not None:
+        _param(what, 'D', D, (width,))
+    if dt_bias is not None:
+        _param(what, 'dt_bias', dt_bias, (width,))
+    return A.shape[1]
+
+
+def _grouped(what, name, t, lead, width, N):
+    """B or C as [..., groups, N]."""
+    t = _data(t)
+    if not torch.is_tensor(t) or t.dim() not in (len(lead) + 1, len(lead) + 2) or t.shape[-1] != N:
+        raise ValueError(f'{what}: {name} must be [..., groups, {N}] or [..., {N}]')
+    t = t.unsqueeze(-2) if t.dim() == len(lead) + 1 else t
+    if t.shape[-2] < 1 or width % t.shape[-2]:
+        raise ValueError(f'{what}: {t.shape[-2]} groups of {width} channels')
+    return t
+
+
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, plan: Optional[PackedRows] = None, state=None, dt_softplus=True):
+    """Selective state space scan: per channel d, with its group's B and C,
+
+      s_t = softplus(dt_t + dt_bias) (or the plain sum);  h_t = exp(s_t A) h_{t-1} + s_t x_t B_t;  y_t = (C_t . h_t + D x_t) silu(z_t)
+
+    x, dt, z [.., channels]; B, C [.., groups, N] or [.., N]; A [channels, N], D, dt_bias [channels] fp32; state [B, channels, N] fp32 (None:
+    zeros).  D, z, dt_bias may be None.  Returns (y like x, last state [B, channels, N] fp32).  N <= 64.
+    Differentiable in x, dt, A, B, C, D, z, dt_bias and state."""
+    what = 'selective_scan'
+    batch = _Batch(what, x, plan)
+    data, width = _data(x), batch.D
+    _C.dtype_code(data, what)
+    data = batch.take('x', data, (width,), data.dtype)
+    N = _scan_params(what, A, D, dt_bias, width)
+    raw = batch.take('dt', dt, (width,), data.dtype)
+    gate = None if z is None else batch.take('z', z, (width,), data.dtype)
+    Bg, Cg = _grouped(what, 'B', B, batch.lead, width, N), _grouped(what, 'C', C, batch.lead, width, N)
+    if Bg.shape != Cg.shape:
+        raise ValueError(f'{what}: B has {Bg.shape[-2]} groups, C has {Cg.shape[-2]}')
+    Bg, Cg = batch.take('B', Bg, Bg.shape[-2:], data.dtype), batch.take('C', Cg, Cg.shape[-2:], data.dtype)
+    if state is not None:
+        _param(what, 'state', state, (batch.B, width, N))
+    _C.one_device(data, raw, A, Bg, Cg, D, gate, dt_bias, state, *batch.tensors())
+    inputs = (data, raw, A, Bg, Cg, D, gate, dt_bias, state)
+    want_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    y, last = _SelectiveScan.apply(batch, int(bool(dt_softplus)), want_grad, *inputs)
+    return _like(x, y), last
+
+
+def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=True, out=None):
+    """One token of each of B sequences: x, dt, z [B, channels], B, C [B, groups, N] or [B, N], state [B, channels, N] fp32 -> (y [B, channels],
+    new state).  `out`: where the new state goes (it may be `state`: updated in place).  Inference only: training goes through
+    `selective_scan`."""
+    what = 'selective_scan_step'
+    if not torch.is_tensor(x) or x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f'{what}: x must be [B, channels]')
+    code = _C.dtype_code(x, what)
+    n, width = x.shape
+    N = _scan_params(what, A, D, dt_bias, width)
+
+    def row(name, t, tail):
+        if not torch.is_tensor(t) or tuple(t.shape) != (n, *tail):
+            raise ValueError(f'{what}: {name} must be {[n, *tail]}')
+        if t.dtype != x.dtype:
+            raise TypeError(f'{what}: {name} must be {x.dtype}, as x is')
+        t = t.detach()
+        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+    Bg, Cg = _grouped(what, 'B', B, (n,), width, N), _grouped(what, 'C', C, (n,), width, N)
+    if Bg.shape != Cg.shape:
+        raise ValueError(f'{what}: B has {Bg.shape[-2]} groups, C has {Cg.shape[-2]}')
+    data, raw = row('x', x, (width,)), row('dt', dt, (width,))
+    gate = None if z is None else row('z', z, (width,))
+    Bg, Cg = row('B', Bg, Bg.shape[1:]), row('C', Cg, Cg.shape[1:])
+    _param(what, 'state', state, (n, width, N))
+    dev = _C.one_device(data, raw, A, Bg, Cg, D, gate, dt_bias, state)
+    with torch.no_grad(), torch.cuda.device(dev):
+        A, D, dt_bias = A.contiguous(), _contiguous(D), _contiguous(dt_bias)
+        new = _step_out(what, state, out, (data, raw, A, Bg, Cg, D, gate, dt_bias))
+        state = state.contiguous()
+        y = torch.empty(n, width, dtype=x.dtype, device=dev)
+        pair = lambda t: (0, 0) if t is None else (0, t.stride(0))      # noqa: E731
+        strides = _ints(*pair(data), *pair(raw), 0, Bg.stride(0), Bg.stride(1), 0, Cg.stride(0), Cg.stride(1), *pair(gate), 0, 1, 0, 0)
+        _C.check(_lib.ppk_selective_scan_step(code, n, width, N, Bg.shape[1], _C.p(data), _C.p(raw), _C.p(A), _C.p(Bg), _C.p(Cg), _C.p(D), _C.p(gate),
+                                              _C.p(dt_bias), _C.p(state), int(bool(dt_softplus)), _C.p(y), _C.p(new), strides, _C.stream()))
+    return y, new

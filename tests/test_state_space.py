@@ -1,0 +1,164 @@
+"""What the sequence operators refuse, and the plan of a packed batch (no GPU needed)."""
+import pytest
+import torch
+from torch.nn.utils.rnn import pack_sequence
+
+from paccmann_polymer_amd import _C
+from paccmann_polymer_amd import state_space as S
+
+T, B, D, K, N = 5, 3, 8, 4, 6
+
+
+def plan():
+    return S.packed_rows(torch.tensor([3, 3, 2, 1]), 'cpu')
+
+
+@pytest.mark.parametrize('lengths', [[1], [5], [3, 3, 2, 1], [40, 17, 16, 16, 1], [7] * 9])
+def test_packed_rows_matches_pack_sequence(lengths):
+    seqs = [torch.arange(n) for n in lengths]
+    packed = pack_sequence(seqs)
+    p = S.packed_rows(packed, 'cpu', sequences=len(lengths) + 2)
+    assert p.rows == sum(lengths) and p.steps == max(lengths) and p.sequences == len(lengths) + 2
+    assert p.lengths.tolist() == lengths + [0, 0]
+    assert p.offsets.tolist() == [0] + torch.cumsum(packed.batch_sizes, 0).tolist()
+    for b, n in enumerate(lengths):
+        for t in range(n):
+            assert int(packed.data[p.offsets[t] + b]) == t
+    tiles = [-(-n // 16) for n in lengths] + [0, 0]
+    assert p.kept == sum(tiles) and (p.tiles[1:] - p.tiles[:-1]).tolist() == tiles
+
+
+@pytest.mark.parametrize('sizes', [[2, 3], [1, 0], [-1]])
+def test_packed_rows_refuses(sizes):
+    with pytest.raises(ValueError):
+        S.packed_rows(torch.tensor(sizes), 'cpu')
+    with pytest.raises(ValueError):
+        S.packed_rows(torch.tensor([4, 2]), 'cpu', sequences=3)
+
+
+def conv_args(**change):
+    a = dict(x=torch.zeros(T, B, D), weight=torch.zeros(D, K), bias=torch.zeros(D))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=torch.zeros(T, D)), ValueError),                                     # rows without a plan
+    (dict(x=torch.zeros(8, D), plan=plan()), ValueError),                        # rows that the plan does not have
+    (dict(x=torch.zeros(T, B, D), plan=plan()), ValueError),
+    (dict(x=torch.zeros(9, D), plan=torch.tensor([3])), TypeError),
+    (dict(x=[1.0]), TypeError),
+    (dict(x=torch.zeros(T, B, 0)), ValueError),
+    (dict(x=torch.zeros(T, B, D, dtype=torch.float16)), TypeError),
+    (dict(x=torch.zeros(T, B, D, dtype=torch.float64)), TypeError),
+    (dict(weight=torch.zeros(D + 1, K)), ValueError),
+    (dict(weight=torch.zeros(D, 1, K)), ValueError),
+    (dict(weight=torch.zeros(D, 0)), ValueError),
+    (dict(weight=torch.zeros(D, 9)), ValueError),
+    (dict(weight=torch.zeros(D, K, dtype=torch.bfloat16)), TypeError),
+    (dict(bias=torch.zeros(D + 1)), ValueError),
+    (dict(state=torch.zeros(B, K, D)), ValueError),
+    (dict(state=torch.zeros(B, K - 1, D, dtype=torch.bfloat16)), TypeError),
+    (dict(activation='relu'), ValueError),
+    (dict(), _C.PPKError),                                                       # all in order, but on the CPU
+    (dict(x=torch.zeros(9, D), plan=plan()), _C.PPKError),
+])
+def test_causal_conv_refuses(change, error):
+    with pytest.raises(error):
+        S.causal_conv(**conv_args(**change))
+
+
+def scan_args(**change):
+    a = dict(x=torch.zeros(T, B, D), dt=torch.zeros(T, B, D), A=torch.zeros(D, N), B=torch.zeros(T, B, N), C=torch.zeros(T, B, N))
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(dt=torch.zeros(T, B, D + 1)), ValueError),
+    (dict(dt=torch.zeros(T, B, D, dtype=torch.bfloat16)), TypeError),
+    (dict(x=torch.zeros(T, B, D, dtype=torch.bfloat16)), TypeError),
+    (dict(A=torch.zeros(D, 65), B=torch.zeros(T, B, 65), C=torch.zeros(T, B, 65)), ValueError),
+    (dict(A=torch.zeros(D, N, dtype=torch.bfloat16)), TypeError),
+    (dict(A=torch.zeros(D + 1, N)), ValueError),
+    (dict(B=torch.zeros(T, B, N + 1)), ValueError),
+    (dict(B=torch.zeros(T, B, 3, N), C=torch.zeros(T, B, 3, N)), ValueError),    # 3 groups of 8 channels
+    (dict(B=torch.zeros(T, B, 2, N), C=torch.zeros(T, B, 4, N)), ValueError),
+    (dict(B=torch.zeros(T + 1, B, N)), ValueError),
+    (dict(D=torch.zeros(D + 1)), ValueError),
+    (dict(z=torch.zeros(T, B, 1)), ValueError),
+    (dict(dt_bias=torch.zeros(D, dtype=torch.float64)), TypeError),
+    (dict(state=torch.zeros(B, D, N + 1)), ValueError),
+    (dict(state=torch.zeros(B, D, N, dtype=torch.bfloat16)), TypeError),
+    (dict(), _C.PPKError),
+])
+def test_selective_scan_refuses(change, error):
+    with pytest.raises(error):
+        S.selective_scan(**scan_args(**change))
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=torch.zeros(B, 1, D)), ValueError),
+    (dict(state=torch.zeros(B, D, N + 1)), ValueError),
+    (dict(state=torch.zeros(B, D, N, dtype=torch.float64)), TypeError),
+    (dict(dt=torch.zeros(B + 1, D)), ValueError),
+    (dict(B=torch.zeros(B, N, dtype=torch.bfloat16)), TypeError),
+    (dict(), _C.PPKError),
+])
+def test_selective_scan_step_refuses(change, error):
+    a = dict(x=torch.zeros(B, D), dt=torch.zeros(B, D), A=torch.zeros(D, N), B=torch.zeros(B, N), C=torch.zeros(B, N), state=torch.zeros(B, D, N))
+    a.update(change)
+    with pytest.raises(error):
+        S.selective_scan_step(**a)
+
+
+def test_step_out_may_be_the_state_and_nothing_else():
+    state = torch.zeros(4, 3, D)
+    assert S._step_out('f', state, None, ()).shape == state.shape
+    assert S._step_out('f', state, state, ()) is state
+    whole = torch.zeros(5, 3, D)
+    for bad in (torch.zeros(4, 3, D + 1), torch.zeros(4, 3, D, dtype=torch.bfloat16), torch.zeros(4, D, 3).transpose(1, 2)):
+        with pytest.raises(ValueError):
+            S._step_out('f', state, bad, ())
+    with pytest.raises(ValueError):
+        S._step_out('f', whole[:4], whole[1:], ())                               # shifted by one sequence
+    with pytest.raises(ValueError):
+        S._step_out('f', state, whole[:4], (whole[3, 0],))
+    assert S._step_out('f', state, whole[:4], (whole[4],)).data_ptr() == whole.data_ptr()    # beside each other in one allocation
+
+
+@pytest.mark.parametrize('change,error', [
+    (dict(x=torch.zeros(B, D, 1)), ValueError),
+    (dict(state=torch.zeros(B, K, D)), ValueError),
+    (dict(state=torch.zeros(B, K - 1, D, dtype=torch.bfloat16)), TypeError),
+    (dict(), _C.PPKError),
+])
+def test_causal_conv_step_refuses(change, error):
+    a = dict(x=torch.zeros(B, D), state=torch.zeros(B, K - 1, D), weight=torch.zeros(D, K))
+    a.update(change)
+    with pytest.raises(error):
+        S.causal_conv_step(**a)
+
+
+def strides(n):
+    import ctypes
+    return (ctypes.c_int64 * n)()
+
+
+@pytest.mark.parametrize('call,code', [
+    (lambda L: L.ppk_causal_conv_fwd(1, 1, 1, 8, 4, None, None, 16, 16, None, None, 1, 16, None, strides(4), None), -4),
+    (lambda L: L.ppk_causal_conv_fwd(0, 1, 1, 8, 9, None, None, 16, 16, None, None, 1, 16, None, strides(4), None), -4),
+    (lambda L: L.ppk_causal_conv_fwd(0, 1, 1, 0, 4, None, None, 16, 16, None, None, 1, 16, None, strides(4), None), -1),
+    (lambda L: L.ppk_causal_conv_fwd(0, 1, 1, 8, 4, None, None, None, 16, None, None, 1, 16, None, strides(4), None), -6),
+    (lambda L: L.ppk_causal_conv_fwd(0, 5, 0, 8, 4, None, None, None, 16, None, None, 1, None, None, strides(4), None), 0),
+    (lambda L: L.ppk_causal_conv_bwd(0, 1, 1, 8, 4, None, None, 16, 16, None, None, 1, 16, None, 16, 16, None, None, strides(6), 256, 8, None), -3),
+    (lambda L: L.ppk_causal_conv_step(0, 1, 8, 4, 16, 8, None, 16, None, 1, 16, None, None), -6),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 65, 1, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -4),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 3, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -1),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 1, 16, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -6),
+    (lambda L: L.ppk_selective_scan_bwd(0, 2, 1, 8, 4, 1, 2, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 8, None), -3),
+    (lambda L: L.ppk_selective_scan_bwd(0, 2, 1, 8, 4, 1, 3, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 8, None), -1),
+    (lambda L: L.ppk_selective_scan_step(0, 1, 8, 4, 1, *[16] * 5, *[None] * 4, 1, 16, 16, strides(16), None), -6),
+])
+def test_c_entries_return_codes(call, code):
+    assert call(_C.lib) == code
