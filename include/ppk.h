@@ -292,10 +292,11 @@ int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void*
  * strides_host [16]: x, raw (two each), B, C (step, sequence, group), z (two), the outputs in ROWS of their width (two), dy (two).
  * y, dx, draw, dz [rows, D], dB, dC [rows, G, N].  bwd overwrites all its outputs; dskip, dbias, dstate may be NULL. */
 int64_t ppk_selective_scan_tile(void);
+size_t ppk_selective_scan_fwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G);      /* 0 where none is needed */
 int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, const int64_t* step_off, const int64_t* lengths,
                            const int64_t* tiles, const void* x, const void* raw, const float* A, const void* Bm, const void* Cm, const float* skip,
                            const void* z, const float* bias, const float* state, int softplus, void* y, float* last_state, float* kept,
-                           const int64_t* strides_host, ppk_stream_t stream);
+                           const int64_t* strides_host, void* workspace, size_t ws_bytes, ppk_stream_t stream);
 size_t ppk_selective_scan_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows);
 int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows, const int64_t* step_off,
                            const int64_t* lengths, const int64_t* tiles, const void* x, const void* raw, const float* A, const void* Bm, const void* Cm,

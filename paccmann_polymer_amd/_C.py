@@ -64,7 +64,8 @@ SIGNATURES = {
     'ppk_causal_conv_step': (c_int, [c_int, c_i64, c_i64, c_i64, ptr, c_i64, ptr, ptr, ptr, c_int, ptr, ptr, ptr]),
     'ppk_selective_scan_tile': (c_i64, []),
     'ppk_selective_scan_fwd': (c_int, [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr,
-                                       ptr, ptr, ptr, c_int, ptr, ptr, ptr, ptr, ptr]),
+                                       ptr, ptr, ptr, c_int, ptr, ptr, ptr, ptr, ptr, c_sz, ptr]),
+    'ppk_selective_scan_fwd_workspace_bytes': (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     'ppk_selective_scan_bwd_workspace_bytes': (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
     'ppk_selective_scan_bwd': (c_int, [c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr,
                                        ptr, ptr, ptr, c_int, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr,

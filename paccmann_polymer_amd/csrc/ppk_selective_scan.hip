@@ -14,6 +14,7 @@ using ppk::Stride;
 using ppk::at;
 
 constexpr int TILE = 16;                     // steps between two kept states
+constexpr long long MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 1024;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScanArgs {
@@ -21,6 +22,8 @@ struct ScanArgs {
     const int64_t* tiles;                    // device [B + 1]: first tile of each sequence, or null: rectangular
     int D, N, G, per;                        // per = D / G channels of a group
     int blocks_per_group;                    // channel blocks of a launch in a group
+    int splits;                              // of the time axis, each of span steps (a multiple of TILE)
+    long long span;
     const void *x, *raw, *Bm, *Cm, *z, *dy;
     const float *A, *skip, *bias, *state, *dlast;
     Stride xs, raws, Bs, Cs, zs, dys, rows;  // rows: of the outputs, in rows of their width
@@ -28,69 +31,270 @@ struct ScanArgs {
     int softplus;
     void *y, *dx, *draw, *dz;
     float *last, *kept, *dstate;             // kept: [tiles, D, N]
-    float *pA, *pD, *pBC;                    // partial sums: [items, D, N], [2, items, D], [blocks_per_group, rows, G, 2, N]
+    float *carry, *sdt;                      // [B, splits, D, N], [B, splits, D]: what enters a split, and the sum of its dt
+    float *pA, *pD, *pBC;                    // partial sums: [B splits, D, N], [2, B splits, D], [blocks_per_group, rows, G, 2, N]
     long long nrows;
 };
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_(-LOG2E * x)); }
-__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(__expf(x)); }
+// log(1 + e^x) = max(x, 0) + log1p(u), u = e^-|x|.  w = 1 + u is rounded; log1p(u) = log(w) + (u - (w - 1)) / w to first order in what
+// the rounding lost, which keeps a small dt (softplus of -7 is 1e-3) as exact as a large one.
+__device__ __forceinline__ float softplus(float x)
+{
+    const float u = exp2_(-LOG2E * fabsf(x)), w = 1.0f + u;
+    const float l = fmaf(u - (w - 1.0f), __builtin_amdgcn_rcpf(w), LN2 * __builtin_amdgcn_logf(w));
+    return fmaxf(x, 0.0f) + l;                                 // a NaN comes through l
+}
 __device__ __forceinline__ float lane_value(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 
-// One wave: 64 channels of a group of one sequence, every lane a channel with its NP >= N states in registers.  B and C of a step are
-// loaded by the lanes n < N and handed to the multiplications as scalars.
-template <typename T, int NP>
+// memory that the kernel does not write, at an address that all lanes share: loaded into scalar registers
+#define UNIFORM __attribute__((address_space(4)))
+template <typename T> __device__ __forceinline__ const UNIFORM T* uniform(const void* p) { return (const UNIFORM T*)(uintptr_t)p; }
+__device__ __forceinline__ long long uni_row(const SeqBatch& q, long long t) { return q.off ? uniform<long long>(q.off)[t] : t; }
+__device__ __forceinline__ long long uni_len(const SeqBatch& q, long long b) { return q.len ? uniform<long long>(q.len)[b] : q.T; }
+__device__ __forceinline__ long long first_tile(const ScanArgs& a, long long b) { return a.tiles ? uniform<long long>(a.tiles)[b] : b * ((a.q.T + TILE - 1) / TILE); }
+
+// N consecutive elements at a uniform address, 4-byte aligned, as scalars
+template <typename T, int N> struct Scalars;
+template <int N> struct Scalars<float, N> {
+    float v[N];
+    __device__ __forceinline__ void load(const float* p) { const UNIFORM float* u = uniform<float>(p);
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = u[n]; }
+    __device__ __forceinline__ float at(int n) const { return v[n]; }
+};
+template <int N> struct Scalars<bf16_t, N> {
+    unsigned v[N / 2];
+    __device__ __forceinline__ void load(const bf16_t* p) { const UNIFORM unsigned* u = uniform<unsigned>(p);
+#pragma unroll
+        for (int n = 0; n < N / 2; ++n) v[n] = u[n]; }
+    __device__ __forceinline__ float at(int n) const { return __uint_as_float(n & 1 ? v[n / 2] & 0xffff0000u : v[n / 2] << 16); }
+};
+// ... or any N at any alignment: lane n holds element n, zero from `count` on
+template <typename T, int N> struct Lanes {
+    float v;
+    __device__ __forceinline__ void load(const T* p, int lane, int count) { v = lane < count ? to_f32(p[lane]) : 0.f; }
+    __device__ __forceinline__ float at(int n) const { return lane_value(v, n); }
+};
+// SCALAR: a row's N == NP elements begin on 4 bytes everywhere
+template <typename T, int NP, bool SCALAR> struct RowVec {
+    Scalars<T, NP> s;
+    Lanes<T, NP> l;
+    __device__ __forceinline__ void load(const T* p, int lane, int count) { if constexpr (SCALAR) s.load(p); else l.load(p, lane, count); }
+    __device__ __forceinline__ float at(int n) const { if constexpr (SCALAR) return s.at(n); else return l.at(n); }
+};
+
+template <int NP> __device__ __forceinline__ void load_states(const float* p, int N, float (&h)[NP])
+{
+#pragma unroll
+    for (int n = 0; n < NP; ++n) h[n] = n < N ? p[n] : 0.f;
+}
+template <int NP> __device__ __forceinline__ void store_states(float* p, int N, const float (&h)[NP])
+{
+    if (N == NP && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+        for (int n = 0; n < NP; n += 4) *reinterpret_cast<float4*>(p + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+        if (n < N) p[n] = h[n];
+}
+
+// What a wave of the kernels with a lane a channel works on: 64 channels of a group of one sequence, one split of its steps
+struct Item {
+    long long b, t0, t1, len;
+    int s, g, d;                               // split, group, this lane's channel (a channel of the group where it has none of its own)
+    bool live;
+    __device__ __forceinline__ Item(const ScanArgs& a)
+    {
+        const int nb = a.G * a.blocks_per_group, cb = (int)(blockIdx.x % nb);
+        const long long rest = blockIdx.x / nb;
+        s = (int)(rest % a.splits);
+        b = rest / a.splits;
+        g = cb / a.blocks_per_group;
+        const int dl = (cb % a.blocks_per_group) * 64 + (int)threadIdx.x;
+        live = dl < a.per;
+        d = g * a.per + (live ? dl : 0);
+        len = uni_len(a.q, b);
+        t0 = s * a.span;
+        t1 = t0 + a.span < len ? t0 + a.span : len;
+    }
+};
+__device__ __forceinline__ long long carry_at(const ScanArgs& a, long long b, int s, int d) { return (b * a.splits + s) * a.D + d; }
+
+constexpr int AHEAD = 8;                       // steps whose elements are loaded before those of the steps before them are used
+
+// The forward pass: a lane a channel with its NP >= N states in registers, B and C of a step in scalar registers (SCALAR) or handed over
+// from lanes.  PART: only the state at the end of a split that begins with none, and the sum of its dt.
+template <typename T, int NP, bool SCALAR, bool PART>
 __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 {
-    const int lane = threadIdx.x;
-    const int nb = a.G * a.blocks_per_group;
-    const long long b = blockIdx.x / nb;
-    const int cb = (int)(blockIdx.x % nb), g = cb / a.blocks_per_group;
-    const int dl = (cb % a.blocks_per_group) * 64 + lane;
-    const bool live = dl < a.per;
-    const int d = g * a.per + (live ? dl : 0), N = a.N;
-    const long long len = a.q.length(b);
+    const Item it(a);
+    const int lane = threadIdx.x, N = a.N;
+    const long long len = it.len, t0 = it.t0, t1 = it.t1;
+    if (t0 >= len && it.s > 0) return;
+    if (PART && t1 >= len) return;             // nothing enters a split behind the last
     float A2[NP], h[NP];
+    load_states<NP>(a.A + (long long)it.d * N, N, A2);
+    if (PART || (a.splits == 1 && !a.state)) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) {
-        A2[n] = n < N ? a.A[(long long)d * N + n] * LOG2E : 0.f;
-        h[n] = n < N && a.state ? a.state[(b * a.D + d) * N + n] : 0.f;
-    }
-    const float skip = a.skip ? a.skip[d] : 0.f, bias = a.bias ? a.bias[d] : 0.f;
-    const long long tile0 = a.tiles ? a.tiles[b] : b * ((a.q.T + TILE - 1) / TILE);
-    const T* Bp = (const T*)a.Bm + g * a.Bg + (lane < N ? lane : 0);
-    const T* Cp = (const T*)a.Cm + g * a.Cg + (lane < N ? lane : 0);
-    for (long long t = 0; t < len; ++t) {
-        if (a.kept && t % TILE == 0 && live)
+        for (int n = 0; n < NP; ++n) h[n] = 0.f;
+    } else load_states<NP>(a.splits > 1 ? a.carry + carry_at(a, it.b, it.s, it.d) * N : a.state + (it.b * a.D + it.d) * N, N, h);
 #pragma unroll
-            for (int n = 0; n < NP; ++n)
-                if (n < N) a.kept[((tile0 + t / TILE) * a.D + d) * N + n] = h[n];
-        const long long r = a.q.row(t);
-        const float x = to_f32(((const T*)a.x)[at(a.xs, r, b) + d]);
-        const float raw = to_f32(((const T*)a.raw)[at(a.raws, r, b) + d]) + bias;
-        const float Bv = to_f32(Bp[at(a.Bs, r, b)]), Cv = to_f32(Cp[at(a.Cs, r, b)]);
-        const float dt = a.softplus ? softplus(raw) : raw, dx = dt * x;
-        float y[4] = {skip * x, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NP; ++n) A2[n] *= LOG2E;
+    const float skip = !PART && a.skip ? a.skip[it.d] : 0.f, bias = a.bias ? a.bias[it.d] : 0.f;
+    const long long tile0 = first_tile(a, it.b);
+    const T *xp = (const T*)a.x + it.b * a.xs.b, *rp = (const T*)a.raw + it.b * a.raws.b, *zp = (const T*)a.z + it.b * a.zs.b;
+    const T *Bp = (const T*)a.Bm + it.b * a.Bs.b + it.g * a.Bg, *Cp = (const T*)a.Cm + it.b * a.Cs.b + it.g * a.Cg;
+    T* yp = (T*)a.y + it.b * a.rows.b * a.D;
+    const unsigned d = (unsigned)it.d;
+    const bool gate = !PART && a.z;
+    T xv[AHEAD], rv[AHEAD], zv[AHEAD];
+    long long rows[AHEAD];
+    const auto fetch = [&](long long t) {
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
-            if (n < N) {
-                h[n] = fmaf(exp2_(dt * A2[n]), h[n], dx * lane_value(Bv, n));
-                y[n & 3] = fmaf(h[n], lane_value(Cv, n), y[n & 3]);
+        for (int i = 0; i < AHEAD; ++i) {
+            const long long r = uni_row(a.q, t + i < t1 ? t + i : t1 - 1);
+            rows[i] = r;
+            xv[i] = (xp + r * a.xs.t)[d];
+            rv[i] = (rp + r * a.raws.t)[d];
+            if (gate) zv[i] = (zp + r * a.zs.t)[d];
+        }
+    };
+    float sum = 0.f;
+    if (t0 < t1) fetch(t0);
+    for (long long t = t0; t < t1; t += AHEAD) {
+        if (!PART && a.kept && t % TILE == 0 && it.live) store_states<NP>(a.kept + ((tile0 + t / TILE) * a.D + it.d) * N, N, h);
+        float x[AHEAD], raw[AHEAD], z[AHEAD];
+        long long r[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) { x[i] = to_f32(xv[i]); raw[i] = to_f32(rv[i]) + bias; z[i] = gate ? to_f32(zv[i]) : 0.f; r[i] = rows[i]; }
+        if (t + AHEAD < t1) fetch(t + AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (t + i >= t1) break;
+            RowVec<T, NP, SCALAR> Bv, Cv;
+            Bv.load(Bp + r[i] * a.Bs.t, lane, N);
+            if (!PART) Cv.load(Cp + r[i] * a.Cs.t, lane, N);
+            const float dt = a.softplus ? softplus(raw[i]) : raw[i], dx = dt * x[i];
+            float y[4] = {skip * x[i], 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                h[n] = fmaf(exp2_(dt * A2[n]), h[n], dx * Bv.at(n));
+                if (!PART) y[n & 3] = fmaf(h[n], Cv.at(n), y[n & 3]);
             }
-        float out = (y[0] + y[1]) + (y[2] + y[3]);
-        if (a.z) { const float z = to_f32(((const T*)a.z)[at(a.zs, r, b) + d]); out *= z * sigmoid(z); }
-        if (live) ((T*)a.y)[at(a.rows, r, b) * a.D + d] = from_f32<T>(out);
+            if (PART) { sum += dt; continue; }
+            float out = (y[0] + y[1]) + (y[2] + y[3]);
+            if (gate) out *= z[i] * sigmoid(z[i]);
+            if (it.live) (yp + r[i] * a.rows.t * a.D)[d] = from_f32<T>(out);
+        }
     }
-    if (live)
+    if (!it.live) return;
+    if (PART) {
+        store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, h);
+        a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
+    } else if (t1 == len) store_states<NP>(a.last + (it.b * a.D + it.d) * N, N, h);
+}
+
+// What the gradient of the state at the end of a split becomes at its beginning, without what enters at the end: g = a (g + dy' C),
+// from the last step to the first, and the sum of its dt.  Laid out as the forward pass.
+template <typename T, int NP, bool SCALAR>
+__global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
+{
+    const Item it(a);
+    const int lane = threadIdx.x, N = a.N;
+    const long long t0 = it.t0, t1 = it.t1;
+    if (t0 >= it.len || it.s == 0) return;     // nothing leaves the first
+    float A2[NP], g[NP];
+    load_states<NP>(a.A + (long long)it.d * N, N, A2);
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
-            if (n < N) a.last[(b * a.D + d) * N + n] = h[n];
+    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
+    const float bias = a.bias ? a.bias[it.d] : 0.f;
+    const T *dp = (const T*)a.dy + it.b * a.dys.b, *rp = (const T*)a.raw + it.b * a.raws.b, *zp = (const T*)a.z + it.b * a.zs.b;
+    const T* Cp = (const T*)a.Cm + it.b * a.Cs.b + it.g * a.Cg;
+    const unsigned d = (unsigned)it.d;
+    T dv[AHEAD], rv[AHEAD], zv[AHEAD];
+    long long rows[AHEAD];
+    const auto fetch = [&](long long t) {      // steps t - 1, t - 2, ...
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const long long r = uni_row(a.q, t - 1 - i >= t0 ? t - 1 - i : t0);
+            rows[i] = r;
+            dv[i] = (dp + r * a.dys.t)[d];
+            rv[i] = (rp + r * a.raws.t)[d];
+            if (a.z) zv[i] = (zp + r * a.zs.t)[d];
+        }
+    };
+    float sum = 0.f;
+    fetch(t1);
+    for (long long t = t1; t > t0; t -= AHEAD) {
+        float dy[AHEAD], raw[AHEAD];
+        long long r[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float z = a.z ? to_f32(zv[i]) : 0.f;
+            dy[i] = to_f32(dv[i]) * (a.z ? z * sigmoid(z) : 1.0f);
+            raw[i] = to_f32(rv[i]) + bias;
+            r[i] = rows[i];
+        }
+        if (t - AHEAD > t0) fetch(t - AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (t - 1 - i < t0) break;
+            RowVec<T, NP, SCALAR> Cv;
+            Cv.load(Cp + r[i] * a.Cs.t, lane, N);
+            const float dt = a.softplus ? softplus(raw[i]) : raw[i];
+            sum += dt;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(dy[i], Cv.at(n), g[n]);
+        }
+    }
+    if (!it.live) return;
+    store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, g);
+    a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
+}
+
+// Joins the splits of a sequence: carry[s] holds what split s gives alone and receives what enters it.  Forward from the state before
+// the first step, backward (REV) from the gradient of the state behind the last; a thread a state.
+template <bool REV>
+__global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
+{
+    const long long dn = (long long)a.D * a.N, e = (long long)blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    if (e >= dn) return;
+    const int d = (int)(e / a.N);
+    const float A2 = a.A[e] * LOG2E;
+    const float* from = REV ? a.dlast : a.state;
+    const long long len = uni_len(a.q, b);
+    const int used = len > 0 ? (int)((len + a.span - 1) / a.span) : 1;          // no steps: the first split still hands on what enters it
+    float in = from ? from[b * dn + e] : 0.f;
+    float* c = a.carry + b * a.splits * dn + e;
+    const float* sd = a.sdt + b * a.splits * (long long)a.D + d;
+    constexpr int U = 8;
+    for (int k0 = 0; k0 < used; k0 += U) {
+        float own[U], sum[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int s = REV ? used - 1 - (k0 + i) : k0 + i;
+            const bool has = k0 + i < used && (REV ? s > 0 : s < used - 1);        // the last one's own part is not made
+            own[i] = has ? c[s * dn] : 0.f;
+            sum[i] = has ? sd[(long long)s * a.D] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (k0 + i >= used) break;
+            const int s = REV ? used - 1 - (k0 + i) : k0 + i;
+            c[s * dn] = in;
+            in = fmaf(exp2_(sum[i] * A2), in, own[i]);
+        }
+    }
 }
 
 // v + v of the lane that `ctrl` names, in one instruction
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v)
 {
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140, ROR4 = 0x124, ROR8 = 0x128;
 // sum over the low bits of the lane number, LPC lanes; every one of them holds it.  A mirror reverses lanes that hold the same
@@ -103,128 +307,164 @@ template <int LPC> __device__ __forceinline__ float sum_low(float v)
     if (LPC > 8) v = dpp_add<MIRROR>(v);
     return v;
 }
-// sum over the lanes of a row of 16 that share their low bits (LPC of them)
-template <int LPC> __device__ __forceinline__ float sum_high16(float v)
+// sum over the LPC lanes of a row of 16 that share their low bits (of which there are 16 / LPC values)
+template <int LPC> __device__ __forceinline__ float sum_slices(float v)
 {
-    if (LPC <= 1) v = dpp_add<XOR1>(v);
-    if (LPC <= 2) v = dpp_add<XOR2>(v);
-    if (LPC <= 4) v = dpp_add<ROR4>(v);
-    if (LPC <= 8) v = dpp_add<ROR8>(v);
+    if (LPC > 8) v = dpp_add<XOR1>(v);
+    if (LPC > 4) v = dpp_add<XOR2>(v);
+    v = dpp_add<ROR4>(v);
+    v = dpp_add<ROR8>(v);
     return v;
 }
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// Block: 256 / LPC channels of a group of one sequence; lane = channel * LPC + slice, a thread holds the 4 states 4 slice .. of its channel.
+// The backward pass.  A block takes 256 / LPC channels of a group of one sequence and walks a split's tiles backwards; a thread holds the
+// four states 4 slice .. of a channel.  In a wave, lane % 16 = slice * (16 / LPC) + low bits of the channel, lane / 16 = its high bits:
+//   sums over states go over the slices, within a row of 16 lanes (two to four DPP additions);
+//   sums over channels (dB, dC of a step: eight values a thread) go over lane / 16 in the matrix unit, v_mfma_f32_16x16x4f32 with the
+//   value as A and a unit column as B: 16 of them put 2 steps' values into 16 columns of one accumulator, whose rows are lane % 16, so
+//   that the four registers of a lane are the low bits of the channel (and of the slice).  The products are with 1 and 0: exact.
+// Elements of a tile are loaded while the tile behind it is worked on, and what the tile's end needs of them waits in LDS.
 template <typename T, int LPC>
-__global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs a)
+__global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 {
-    constexpr int NP = 4 * LPC, BC = 256 / LPC, PE = TILE * BC / 256;
-    __shared__ float s_dt[TILE][BC], s_dx[TILE][BC], s_dy[TILE][BC];           // dt, dt x, dy'; then the sums over n of dh B, da A, C h
-    __shared__ __align__(16) float s_B[TILE][NP], s_C[TILE][NP];
+    constexpr int NP = 4 * LPC, BC = 256 / LPC, PE = TILE * BC / 256, CL = 16 / LPC, BCE = TILE * 2 * NP / 256;
+    __shared__ float s_dt[TILE][BC], s_dx[TILE][BC], s_dy[TILE][BC];           // dt, dt x, dy'
+    __shared__ float s_x[TILE][BC], s_slope[TILE][BC], s_gz[TILE][BC];         // x, d dt / d raw, dout silu'(z)
+    __shared__ float s_q1[TILE][BC], s_q2[TILE][BC], s_q3[TILE][BC];           // sums over n of dh B, da A, C h
+    __shared__ __align__(16) float s_BC[TILE][2 * NP];
     __shared__ float s_red[TILE][4][2 * NP];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int ch = tid / LPC, ns = tid % LPC;                                  // the scan's channel and slice
-    const int pc = tid % BC, pt = tid / BC;                                    // the channel and first step of the per-element work
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int ns = (lane & 15) / CL, ch = wave * (64 / LPC) + (lane >> 4) * CL + (lane & (CL - 1));    // the scan's slice and channel
+    const int pc = tid % BC, pt = BC >= 64 ? __builtin_amdgcn_readfirstlane(tid / BC) : tid / BC;      // channel and first step of the per-element work
     const int nb = a.G * a.blocks_per_group, N = a.N;
-    const long long b = blockIdx.x / nb;
+    const long long item = blockIdx.x / nb, b = item / a.splits;               // item: sequence and split
+    const int s = (int)(item % a.splits);
     const int cb = (int)(blockIdx.x % nb), g = cb / a.blocks_per_group, cg = cb % a.blocks_per_group;
     const int base = cg * BC;                                                  // of the block's channels in the group
     const bool live = base + ch < a.per, plive = base + pc < a.per;
     const int d = g * a.per + (live ? base + ch : 0), pd = g * a.per + (plive ? base + pc : 0);
-    const long long len = a.q.length(b);
-    const long long tile0 = a.tiles ? a.tiles[b] : b * ((a.q.T + TILE - 1) / TILE);
-    float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dh[4];
+    const long long len = uni_len(a.q, b), end = (s + 1) * a.span < len ? (s + 1) * a.span : len;
+    const long long tile0 = first_tile(a, b);
+    float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dh[4], pick[16];
+    const float* into = a.splits > 1 && s * a.span < len ? a.carry + carry_at(a, b, s, d) * N : (a.dlast ? a.dlast + (b * a.D + d) * N : nullptr);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int n = ns * 4 + j;
         A2[j] = live && n < N ? a.A[(long long)d * N + n] * LOG2E : 0.f;
-        dh[j] = live && n < N && a.dlast ? a.dlast[(b * a.D + d) * N + n] : 0.f;
+        dh[j] = live && n < N && into ? into[n] : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) pick[k] = (lane & 15) == k ? 1.0f : 0.0f;
     const float skip = a.skip && plive ? a.skip[pd] : 0.f, bias = a.bias && plive ? a.bias[pd] : 0.f;
     float dskip = 0.f, dbias = 0.f;
-    for (long long tile = (len + TILE - 1) / TILE - 1; tile >= 0; --tile) {
+
+    T xv[PE], rv[PE], dv[PE], zv[PE], bv[BCE];
+    float hv[4];
+    const auto fetch = [&](long long tile) {
         const long long t0 = tile * TILE;
-        const int steps = (int)(len - t0 < TILE ? len - t0 : TILE);
-        float x[PE], dt[PE], slope[PE], dy[PE], dout[PE], z[PE], sig[PE];
+        const int steps = (int)(end - t0 < TILE ? end - t0 : TILE);
+#pragma unroll
+        for (int i = 0; i < PE; ++i) {
+            const int t = pt + i * (256 / BC);
+            const long long at_t = t0 + (t < steps ? t : 0), r = BC >= 64 ? uni_row(a.q, at_t) : a.q.row(at_t);
+            xv[i] = ((const T*)a.x + at(a.xs, r, b))[(unsigned)pd];
+            rv[i] = ((const T*)a.raw + at(a.raws, r, b))[(unsigned)pd];
+            dv[i] = ((const T*)a.dy + at(a.dys, r, b))[(unsigned)pd];
+            if (a.z) zv[i] = ((const T*)a.z + at(a.zs, r, b))[(unsigned)pd];
+        }
+#pragma unroll
+        for (int i = 0; i < BCE; ++i) {
+            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP), n = k % NP;
+            const long long r = a.q.row(t0 + (t < steps ? t : 0));
+            const int m = n < N ? n : 0;
+            bv[i] = k < NP ? ((const T*)a.Bm)[at(a.Bs, r, b) + g * a.Bg + m] : ((const T*)a.Cm)[at(a.Cs, r, b) + g * a.Cg + m];
+        }
+        const float* h0 = a.kept + ((tile0 + tile) * a.D + d) * N;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) hv[j] = h0[ns * 4 + j < N ? ns * 4 + j : 0];
+    };
+    const long long tile_end = (end + TILE - 1) / TILE, tile_begin = s * (a.span / TILE);
+    if (tile_end > tile_begin) fetch(tile_end - 1);
+    for (long long tile = tile_end - 1; tile >= tile_begin; --tile) {
+        const long long t0 = tile * TILE;
+        const int steps = (int)(end - t0 < TILE ? end - t0 : TILE);
 #pragma unroll
         for (int i = 0; i < PE; ++i) {
             const int t = pt + i * (256 / BC);
             const bool in = plive && t < steps;
-            const long long r = a.q.row(t0 + (t < steps ? t : 0));
-            x[i] = in ? to_f32(((const T*)a.x)[at(a.xs, r, b) + pd]) : 0.f;
-            const float raw = in ? to_f32(((const T*)a.raw)[at(a.raws, r, b) + pd]) + bias : 0.f;
-            dout[i] = in ? to_f32(((const T*)a.dy)[at(a.dys, r, b) + pd]) : 0.f;
-            z[i] = in && a.z ? to_f32(((const T*)a.z)[at(a.zs, r, b) + pd]) : 0.f;
-            sig[i] = sigmoid(z[i]);
-            dt[i] = in ? (a.softplus ? softplus(raw) : raw) : 0.f;
-            slope[i] = a.softplus ? sigmoid(raw) : 1.0f;
-            dy[i] = a.z ? dout[i] * z[i] * sig[i] : dout[i];
-            s_dt[t][pc] = dt[i];
-            s_dx[t][pc] = dt[i] * x[i];
-            s_dy[t][pc] = dy[i];
+            const float x = in ? to_f32(xv[i]) : 0.f, raw = in ? to_f32(rv[i]) + bias : 0.f, dout = in ? to_f32(dv[i]) : 0.f;
+            const float dt = in ? (a.softplus ? softplus(raw) : raw) : 0.f;
+            float dy = dout, gz = 0.f;
+            if (a.z) {
+                const float z = in ? to_f32(zv[i]) : 0.f, sg = sigmoid(z), zs = z * sg;
+                dy = dout * zs;
+                gz = dout * fmaf(zs, 1.0f - sg, sg);
+            }
+            s_dt[t][pc] = dt;
+            s_dx[t][pc] = dt * x;
+            s_dy[t][pc] = dy;
+            s_x[t][pc] = x;
+            s_slope[t][pc] = a.softplus ? sigmoid(raw) : 1.0f;
+            s_gz[t][pc] = gz;
         }
-        for (int e = tid; e < TILE * NP; e += 256) {
-            const int t = e / NP, n = e % NP;
-            const bool in = t < steps && n < N;
-            const long long r = a.q.row(t0 + (t < steps ? t : 0));
-            s_B[t][n] = in ? to_f32(((const T*)a.Bm)[at(a.Bs, r, b) + g * a.Bg + n]) : 0.f;
-            s_C[t][n] = in ? to_f32(((const T*)a.Cm)[at(a.Cs, r, b) + g * a.Cg + n]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < BCE; ++i) {
+            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP);
+            s_BC[t][k] = t < steps && k % NP < N ? to_f32(bv[i]) : 0.f;
         }
         float h[TILE + 1][4], av[TILE][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = ns * 4 + j;
-            h[0][j] = live && n < N ? a.kept[((tile0 + tile) * a.D + d) * N + n] : 0.f;
-        }
+        for (int j = 0; j < 4; ++j) h[0][j] = live && ns * 4 + j < N ? hv[j] : 0.f;
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < TILE; ++t) {
             const float dtv = s_dt[t][ch], dxv = s_dx[t][ch];
-            const float4 Bv = *reinterpret_cast<const float4*>(&s_B[t][ns * 4]);
-            const float Bj[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+            const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 av[t][j] = exp2_(dtv * A2[j]);
-                h[t + 1][j] = fmaf(av[t][j], h[t][j], dxv * Bj[j]);
+                h[t + 1][j] = fmaf(av[t][j], h[t][j], dxv * Bv[j]);
             }
         }
+        asm volatile("" ::: "memory");           // the steps' values are read from LDS again: kept, they would be 96 registers
+        f32x4 acc;
 #pragma unroll
         for (int t = TILE - 1; t >= 0; --t) {
+            if (t == TILE - 6 && tile > tile_begin) fetch(tile - 1);            // where the registers of five steps are free again
             const float dtv = s_dt[t][ch], dxv = s_dx[t][ch], dyv = s_dy[t][ch];
-            const float4 Bv = *reinterpret_cast<const float4*>(&s_B[t][ns * 4]), Cv = *reinterpret_cast<const float4*>(&s_C[t][ns * 4]);
-            const float Bj[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cj[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
+            const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]), Cv = *reinterpret_cast<const f32x4*>(&s_BC[t][NP + ns * 4]);
             float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                dh[j] = fmaf(dyv, Cj[j], dh[j]);
-                q1 = fmaf(dh[j], Bj[j], q1);
+                dh[j] = fmaf(dyv, Cv[j], dh[j]);
+                q1 = fmaf(dh[j], Bv[j], q1);
                 v[j] = dh[j] * dxv;
                 v[4 + j] = dyv * h[t + 1][j];
-                q3 = fmaf(Cj[j], h[t + 1][j], q3);
+                q3 = fmaf(Cv[j], h[t + 1][j], q3);
                 dh[j] *= av[t][j];
                 const float da = dh[j] * h[t][j];
                 q2 = fmaf(da, A2[j], q2);
                 dA[j] = fmaf(da, dtv, dA[j]);
             }
-            q1 = sum_low<LPC>(q1);
-            q2 = sum_low<LPC>(q2);
-            q3 = sum_low<LPC>(q3);
-            if (ns == 0) { s_dt[t][ch] = q1; s_dx[t][ch] = q2; s_dy[t][ch] = q3; }       // this wave's channels: read above by the same wave
-            // over the wave's channels: two exchanges leave a lane the sums of two of the eight, bits 5 and 4 of the lane say which
-            float u[4], w[2];
+            q1 = sum_slices<LPC>(q1);
+            q2 = sum_slices<LPC>(q2);
+            q3 = sum_slices<LPC>(q3);
+            if (ns == 0) { s_q1[t][ch] = q1; s_q2[t][ch] = q2; s_q3[t][ch] = q3; }
+            if (t & 1) acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(v[k + 4]), false, false);
-                u[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-            }
+            for (int k = 0; k < 8; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v[k], pick[(t & 1) * 8 + k], acc, 0, 0, 0);
+            if (!(t & 1)) {
+                // this lane: column lane % 16 = a step and one of its values, rows 4 (lane / 16) + r = slice * CL + low bits of the channel
+                const int step = t + ((lane >> 3) & 1), side = ((lane >> 2) & 1) * NP, j = lane & 3, q = lane >> 4;
+                if (LPC == 4) s_red[step][wave][side + q * 4 + j] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                if (LPC == 8) {
+                    s_red[step][wave][side + (q * 2) * 4 + j] = acc[0] + acc[1];
+                    s_red[step][wave][side + (q * 2 + 1) * 4 + j] = acc[2] + acc[3];
+                }
+                if (LPC == 16)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[k + 2]), false, false);
-                w[k] = sum_high16<LPC>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
-            }
-            if ((lane & 15) < LPC) {
-                const int n = (lane & (LPC - 1)) * 4 + ((lane >> 4) & 1) * 2, side = (lane >> 5) * NP;
-                s_red[t][wave][side + n] = w[0];
-                s_red[t][wave][side + n + 1] = w[1];
+                    for (int r = 0; r < 4; ++r) s_red[step][wave][side + (q * 4 + r) * 4 + j] = acc[r];
             }
         }
         __syncthreads();
@@ -232,17 +472,18 @@ __global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs a)
         for (int i = 0; i < PE; ++i) {
             const int t = pt + i * (256 / BC);
             if (!(plive && t < steps)) continue;
-            const long long o = at(a.rows, a.q.row(t0 + t), b) * a.D + pd;
-            const float q1 = s_dt[t][pc], q2 = s_dx[t][pc] * LN2, q3 = s_dy[t][pc];
-            const float dr = fmaf(x[i], q1, q2) * slope[i];
-            ((T*)a.dx)[o] = from_f32<T>(fmaf(dt[i], q1, skip * dy[i]));
-            ((T*)a.draw)[o] = from_f32<T>(dr);
-            if (a.z) ((T*)a.dz)[o] = from_f32<T>(dout[i] * fmaf(skip, x[i], q3) * sig[i] * fmaf(z[i], 1.0f - sig[i], 1.0f));
-            dskip = fmaf(dy[i], x[i], dskip);
+            const long long r = BC >= 64 ? uni_row(a.q, t0 + t) : a.q.row(t0 + t), o = at(a.rows, r, b) * a.D;
+            const float q1 = s_q1[t][pc], x = s_x[t][pc], dy = s_dy[t][pc];
+            const float dr = fmaf(x, q1, s_q2[t][pc] * LN2) * s_slope[t][pc];
+            ((T*)a.dx + o)[(unsigned)pd] = from_f32<T>(fmaf(s_dt[t][pc], q1, skip * dy));
+            ((T*)a.draw + o)[(unsigned)pd] = from_f32<T>(dr);
+            if (a.z) ((T*)a.dz + o)[(unsigned)pd] = from_f32<T>(s_gz[t][pc] * fmaf(skip, x, s_q3[t][pc]));
+            dskip = fmaf(dy, x, dskip);
             dbias += dr;
         }
-        for (int e = tid; e < TILE * 2 * NP; e += 256) {
-            const int t = e / (2 * NP), k = e % (2 * NP), n = k % NP;
+#pragma unroll
+        for (int i = 0; i < BCE; ++i) {
+            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP), n = k % NP;
             if (t >= steps || n >= N) continue;
             const long long row = at(a.rows, a.q.row(t0 + t), b);
             a.pBC[(((long long)cg * a.nrows + row) * a.G + g) * 2 * N + (k / NP) * N + n] = (s_red[t][0][k] + s_red[t][1][k]) + (s_red[t][2][k] + s_red[t][3][k]);
@@ -254,18 +495,17 @@ __global__ __launch_bounds__(256) void k_scan_bwd(ScanArgs a)
         for (int j = 0; j < 4; ++j) {
             const int n = ns * 4 + j;
             if (n >= N) continue;
-            a.pA[(b * a.D + d) * N + n] = dA[j];
-            if (a.dstate) a.dstate[(b * a.D + d) * N + n] = dh[j];
+            a.pA[(item * a.D + d) * N + n] = dA[j];
+            if (a.dstate && s == 0) a.dstate[(b * a.D + d) * N + n] = dh[j];
         }
-    __syncthreads();
     s_dt[pt][pc] = dskip;
     s_dx[pt][pc] = dbias;
     __syncthreads();
     if (pt == 0 && plive) {
         float u = s_dt[0][pc], v = s_dx[0][pc];
         for (int i = 1; i < 256 / BC; ++i) { u += s_dt[i][pc]; v += s_dx[i][pc]; }
-        a.pD[b * a.D + pd] = u;
-        a.pD[(a.q.B + b) * a.D + pd] = v;
+        a.pD[item * a.D + pd] = u;
+        a.pD[(a.q.B * a.splits + item) * a.D + pd] = v;
     }
 }
 
@@ -310,21 +550,69 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
     if (ns == 0) ((T*)a.y)[bd] = from_f32<T>(y);
 }
 
-int slices(long long N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+int slices(long long N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+int bwd_slices(long long N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+int padded(long long N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
-template <typename T> void run_fwd(const ScanArgs& a, unsigned blocks, hipStream_t st)
+// How many steps a split of the time axis takes.  `units`: what runs at once without one, `want`: what fills the card.
+long long span_of(long long T, long long units, long long want)
 {
-    if (a.N <= 8) k_scan_fwd<T, 8><<<blocks, 64, 0, st>>>(a);
-    else if (a.N <= 16) k_scan_fwd<T, 16><<<blocks, 64, 0, st>>>(a);
-    else if (a.N <= 32) k_scan_fwd<T, 32><<<blocks, 64, 0, st>>>(a);
-    else k_scan_fwd<T, 64><<<blocks, 64, 0, st>>>(a);
+    const long long all = ceil_div(T > 0 ? T : 1, TILE) * TILE;
+    if (units * 2 > want || all <= 2 * MIN_SPAN) return all;
+    const long long span = ceil_div(ceil_div(all * units, want), TILE) * TILE;
+    return span > MIN_SPAN ? span : MIN_SPAN;
+}
+struct Plan { long long blocks_per_group, span, splits; };
+Plan plan_of(long long T, long long B, long long D, long long G, long long channels, long long want)
+{
+    Plan p;
+    p.blocks_per_group = ceil_div(D / G, channels);
+    p.span = span_of(T, B * G * p.blocks_per_group, want);
+    p.splits = ceil_div(T > 0 ? T : 1, p.span);
+    return p;
+}
+Plan fwd_plan(long long T, long long B, long long D, long long G) { return plan_of(T, B, D, G, 64, FWD_WAVES); }
+Plan bwd_plan(long long T, long long B, long long D, long long N, long long G) { return plan_of(T, B, D, G, 256 / bwd_slices(N), BWD_BLOCKS); }
+size_t carry_bytes(long long B, long long D, long long N, long long splits)
+{
+    return splits > 1 ? ppk_align_up((size_t)B * splits * D * N * 4, 256) + ppk_align_up((size_t)B * splits * D * 4, 256) : 0;
+}
+
+// SCALAR of the kernels: rows of exactly NP elements that begin on 4 bytes
+template <typename T> bool scalar_rows(const void* p, const Stride& s, long long group, int N)
+{
+    const long long per = 4 / (long long)sizeof(T);
+    return N == padded(N) && ((uintptr_t)p & 3) == 0 && s.t % per == 0 && s.b % per == 0 && group % per == 0;
+}
+template <typename T, int NP, bool SCALAR> void launch_fwd(const ScanArgs& a, bool part, unsigned blocks, hipStream_t st)
+{
+    if (part) k_scan_fwd<T, NP, SCALAR, true><<<blocks, 64, 0, st>>>(a);
+    else k_scan_fwd<T, NP, SCALAR, false><<<blocks, 64, 0, st>>>(a);
+}
+template <typename T> void run_fwd(const ScanArgs& a, bool part, unsigned blocks, hipStream_t st)
+{
+    const bool sc = scalar_rows<T>(a.Bm, a.Bs, a.Bg, a.N) && scalar_rows<T>(a.Cm, a.Cs, a.Cg, a.N);
+    switch (padded(a.N)) {
+        case 8: if (sc) launch_fwd<T, 8, true>(a, part, blocks, st); else launch_fwd<T, 8, false>(a, part, blocks, st); break;
+        case 16: if (sc) launch_fwd<T, 16, true>(a, part, blocks, st); else launch_fwd<T, 16, false>(a, part, blocks, st); break;
+        case 32: launch_fwd<T, 32, false>(a, part, blocks, st); break;
+        default: launch_fwd<T, 64, false>(a, part, blocks, st);
+    }
+}
+template <typename T> void run_bwd_part(const ScanArgs& a, unsigned blocks, hipStream_t st)
+{
+    const bool sc = scalar_rows<T>(a.Cm, a.Cs, a.Cg, a.N);
+    switch (padded(a.N)) {
+        case 8: if (sc) k_scan_bwd_part<T, 8, true><<<blocks, 64, 0, st>>>(a); else k_scan_bwd_part<T, 8, false><<<blocks, 64, 0, st>>>(a); break;
+        case 16: if (sc) k_scan_bwd_part<T, 16, true><<<blocks, 64, 0, st>>>(a); else k_scan_bwd_part<T, 16, false><<<blocks, 64, 0, st>>>(a); break;
+        case 32: k_scan_bwd_part<T, 32, false><<<blocks, 64, 0, st>>>(a); break;
+        default: k_scan_bwd_part<T, 64, false><<<blocks, 64, 0, st>>>(a);
+    }
 }
 template <typename T> void run_bwd(const ScanArgs& a, unsigned blocks, hipStream_t st)
 {
-    switch (slices(a.N)) {
-        case 1: k_scan_bwd<T, 1><<<blocks, 256, 0, st>>>(a); break;
-        case 2: k_scan_bwd<T, 2><<<blocks, 256, 0, st>>>(a); break;
+    switch (bwd_slices(a.N)) {
         case 4: k_scan_bwd<T, 4><<<blocks, 256, 0, st>>>(a); break;
         case 8: k_scan_bwd<T, 8><<<blocks, 256, 0, st>>>(a); break;
         default: k_scan_bwd<T, 16><<<blocks, 256, 0, st>>>(a);
@@ -350,16 +638,18 @@ int scan_check(const char* what, int dtype, long long T, long long B, long long 
     return PPK_OK;
 }
 
-struct BwdWs { size_t a, d, bc, sum, total; long long blocks_per_group; };
-BwdWs bwd_ws(long long B, long long D, long long N, long long G, long long rows)
+struct BwdWs { size_t a, d, bc, carry, sum, total; Plan p; };
+BwdWs bwd_ws(long long T, long long B, long long D, long long N, long long G, long long rows)
 {
     BwdWs w;
-    w.blocks_per_group = ceil_div(D / G, 256 / slices(N));
-    w.a = ppk_align_up((size_t)B * D * N * 4, 256);
-    w.d = ppk_align_up((size_t)B * 2 * D * 4, 256);
-    w.bc = ppk_align_up((size_t)w.blocks_per_group * rows * G * 2 * N * 4, 256);
-    w.sum = ppk::partial_sum_ws_bytes(B, D * N);
-    w.total = w.a + w.d + w.bc + w.sum;
+    w.p = bwd_plan(T, B, D, N, G);
+    const long long items = B * w.p.splits;
+    w.a = ppk_align_up((size_t)items * D * N * 4, 256);
+    w.d = ppk_align_up((size_t)items * 2 * D * 4, 256);
+    w.bc = ppk_align_up((size_t)w.p.blocks_per_group * rows * G * 2 * N * 4, 256);
+    w.carry = carry_bytes(B, D, N, w.p.splits);
+    w.sum = ppk::partial_sum_ws_bytes(items, D * N);
+    w.total = w.a + w.d + w.bc + w.carry + w.sum;
     return w;
 }
 
@@ -379,10 +669,16 @@ extern "C" {
 
 int64_t ppk_selective_scan_tile(void) { return TILE; }
 
+size_t ppk_selective_scan_fwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G)
+{
+    if (T < 0 || B < 0 || D < 1 || N < 1 || G < 1) return 0;
+    return carry_bytes(B, D, N, fwd_plan(T, B, D, G).splits);
+}
+
 int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, const int64_t* step_off, const int64_t* lengths,
                            const int64_t* tiles, const void* x, const void* raw, const float* A, const void* Bm, const void* Cm, const float* skip,
                            const void* z, const float* bias, const float* state, int softplus, void* y, float* last_state, float* kept,
-                           const int64_t* strides_host, ppk_stream_t stream)
+                           const int64_t* strides_host, void* workspace, size_t ws_bytes, ppk_stream_t stream)
 {
     int rc = scan_check("selective_scan_fwd", dtype, T, B, D, N, G);
     if (rc) return rc;
@@ -392,14 +688,26 @@ int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
     ScanArgs a = {};
     a.q = {step_off, lengths, T, B};
     a.tiles = tiles;
-    a.D = (int)D; a.N = (int)N; a.G = (int)G; a.per = (int)(D / G); a.blocks_per_group = (int)ceil_div(a.per, 64);
+    const Plan p = fwd_plan(T, B, D, G);
+    a.D = (int)D; a.N = (int)N; a.G = (int)G; a.per = (int)(D / G); a.blocks_per_group = (int)p.blocks_per_group;
+    a.span = p.span; a.splits = (int)p.splits;
     a.x = x; a.raw = raw; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.skip = skip; a.bias = bias; a.state = state; a.softplus = softplus;
     a.y = y; a.last = last_state; a.kept = kept;
     set_strides(a, strides_host);
-    const long long blocks = B * G * a.blocks_per_group;
-    if (blocks > 0x7fffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_fwd: B=%lld D=%lld", (long long)B, (long long)D);
-    if (dtype == PPK_F32) run_fwd<float>(a, (unsigned)blocks, (hipStream_t)stream);
-    else run_fwd<bf16_t>(a, (unsigned)blocks, (hipStream_t)stream);
+    const long long blocks = B * p.splits * G * a.blocks_per_group;
+    if (blocks > 0x7fffffffLL || (p.splits > 1 && B > 65535)) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_fwd: B=%lld D=%lld", (long long)B, (long long)D);
+    hipStream_t st = (hipStream_t)stream;
+    if (p.splits > 1) {
+        if (ws_bytes < carry_bytes(B, D, N, p.splits) || !workspace) PPK_FAIL(PPK_ERR_WS, "selective_scan_fwd: workspace of %zu bytes", ws_bytes);
+        char* cur = (char*)workspace;
+        a.carry = (float*)ppk_carve(cur, (size_t)B * p.splits * D * N * 4);
+        a.sdt = (float*)cur;
+        if (dtype == PPK_F32) run_fwd<float>(a, true, (unsigned)blocks, st);
+        else run_fwd<bf16_t>(a, true, (unsigned)blocks, st);
+        k_scan_join<false><<<dim3((unsigned)ceil_div(D * N, 256), (unsigned)B), 256, 0, st>>>(a);
+    }
+    if (dtype == PPK_F32) run_fwd<float>(a, false, (unsigned)blocks, st);
+    else run_fwd<bf16_t>(a, false, (unsigned)blocks, st);
     PPK_CHECK_LAUNCH("selective_scan_fwd");
     return PPK_OK;
 }
@@ -407,7 +715,7 @@ int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
 size_t ppk_selective_scan_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows)
 {
     if (T < 0 || B < 0 || D < 1 || N < 1 || N > 64 || G < 1 || rows < 0) return 0;
-    return bwd_ws(B, D, N, G, rows).total;
+    return bwd_ws(T, B, D, N, G, rows).total;
 }
 
 int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N, int64_t G, int64_t rows, const int64_t* step_off,
@@ -422,24 +730,39 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
     if (!A || !dA || !workspace || !strides_host || (rows > 0 && (!x || !raw || !Bm || !Cm || !dy || !kept || !dx || !draw || !dB || !dC || (z && !dz))))
         PPK_FAIL(PPK_ERR_NULL, "selective_scan_bwd: null pointer");
     if (step_off && (!lengths || !tiles)) PPK_FAIL(PPK_ERR_NULL, "selective_scan_bwd: a packed batch needs its lengths and tiles");
-    const BwdWs w = bwd_ws(B, D, N, G, rows);
+    const BwdWs w = bwd_ws(T, B, D, N, G, rows);
+    const long long items = B * w.p.splits;
     if (ws_bytes < w.total) PPK_FAIL(PPK_ERR_WS, "selective_scan_bwd: workspace of %zu bytes, %zu needed", ws_bytes, w.total);
     hipStream_t st = (hipStream_t)stream;
     char* cur = (char*)workspace;
     ScanArgs a = {};
-    a.pA = (float*)ppk_carve(cur, (size_t)B * D * N * 4);
-    a.pD = (float*)ppk_carve(cur, (size_t)B * 2 * D * 4);
+    a.pA = (float*)ppk_carve(cur, w.a);
+    a.pD = (float*)ppk_carve(cur, w.d);
     a.pBC = (float*)ppk_carve(cur, w.bc);
+    if (w.p.splits > 1) {
+        a.carry = (float*)ppk_carve(cur, (size_t)items * D * N * 4);
+        a.sdt = (float*)ppk_carve(cur, (size_t)items * D * 4);
+    }
     void* sum_ws = cur;
     a.q = {step_off, lengths, T, B};
     a.tiles = tiles;
-    a.D = (int)D; a.N = (int)N; a.G = (int)G; a.per = (int)(D / G); a.blocks_per_group = (int)w.blocks_per_group;
+    a.D = (int)D; a.N = (int)N; a.G = (int)G; a.per = (int)(D / G); a.blocks_per_group = (int)w.p.blocks_per_group;
+    a.span = w.p.span; a.splits = (int)w.p.splits;
     a.x = x; a.raw = raw; a.Bm = Bm; a.Cm = Cm; a.z = z; a.dy = dy; a.A = A; a.skip = skip; a.bias = bias; a.dlast = dlast_state; a.softplus = softplus;
     a.dx = dx; a.draw = draw; a.dz = dz; a.kept = const_cast<float*>(kept); a.dstate = dstate; a.nrows = rows;
     set_strides(a, strides_host);
-    const long long blocks = B * G * a.blocks_per_group, bc = rows * G * 2 * N;
-    if (blocks > 0x7fffffffLL || ceil_div(bc, 256) > 0x7fffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_bwd: B=%lld D=%lld rows=%lld", (long long)B, (long long)D, (long long)rows);
+    const long long blocks = items * G * a.blocks_per_group, bc = rows * G * 2 * N;
+    if (blocks > 0x7fffffffLL || ceil_div(bc, 256) > 0x7fffffffLL || (w.p.splits > 1 && B > 65535))
+        PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_bwd: B=%lld D=%lld rows=%lld", (long long)B, (long long)D, (long long)rows);
     if (blocks > 0) {
+        if (w.p.splits > 1) {
+            ScanArgs part = a;
+            part.blocks_per_group = (int)ceil_div(a.per, 64);
+            const unsigned pb = (unsigned)(items * G * part.blocks_per_group);
+            if (dtype == PPK_F32) run_bwd_part<float>(part, pb, st);
+            else run_bwd_part<bf16_t>(part, pb, st);
+            k_scan_join<true><<<dim3((unsigned)ceil_div(D * N, 256), (unsigned)B), 256, 0, st>>>(a);
+        }
         if (dtype == PPK_F32) run_bwd<float>(a, (unsigned)blocks, st);
         else run_bwd<bf16_t>(a, (unsigned)blocks, st);
     }
@@ -448,9 +771,9 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
         if (dtype == PPK_F32) k_scan_bc<float><<<nb, 256, 0, st>>>(a.pBC, a.blocks_per_group, rows, (int)G, (int)N, (float*)dB, (float*)dC);
         else k_scan_bc<bf16_t><<<nb, 256, 0, st>>>(a.pBC, a.blocks_per_group, rows, (int)G, (int)N, (bf16_t*)dB, (bf16_t*)dC);
     }
-    rc = ppk::partial_sum(a.pA, B, D * N, dA, sum_ws, st);
-    if (!rc && dskip) rc = ppk::partial_sum(a.pD, B, D, dskip, sum_ws, st);
-    if (!rc && dbias) rc = ppk::partial_sum(a.pD + B * D, B, D, dbias, sum_ws, st);
+    rc = ppk::partial_sum(a.pA, items, D * N, dA, sum_ws, st);
+    if (!rc && dskip) rc = ppk::partial_sum(a.pD, items, D, dskip, sum_ws, st);
+    if (!rc && dbias) rc = ppk::partial_sum(a.pD + items * D, items, D, dbias, sum_ws, st);
     if (rc) return rc;
     PPK_CHECK_LAUNCH("selective_scan_bwd");
     return PPK_OK;

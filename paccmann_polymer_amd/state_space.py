@@ -307,9 +307,11 @@ class _SelectiveScan(torch.autograd.Function):
                 n = batch.plan.kept if batch.plan is not None else batch.B * ((batch.T + tile - 1) // tile)
                 kept = torch.empty(n, width, N, dtype=torch.float32, device=dev)
             off, lengths = batch.pointers()
+            wsb = _lib.ppk_selective_scan_fwd_workspace_bytes(batch.T, batch.B, width, N, G)
+            ws = _ws(wsb, dev) if wsb else None
             _C.check(_lib.ppk_selective_scan_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, off, lengths, _C.p(tiles), _C.p(x), _C.p(dt), _C.p(A),
                                                  _C.p(B), _C.p(C), _C.p(D), _C.p(z), _C.p(dt_bias), _C.p(state), softplus, _C.p(y), _C.p(last), _C.p(kept),
-                                                 _scan_strides(batch, x, dt, B, C, z, batch.out_rows, None), _C.stream()))
+                                                 _scan_strides(batch, x, dt, B, C, z, batch.out_rows, None), _C.p(ws), wsb, _C.stream()))
         if kept is not None:
             ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, kept)
             ctx.batch, ctx.softplus, ctx.has_state = batch, softplus, state is not None

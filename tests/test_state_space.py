@@ -153,9 +153,10 @@ def strides(n):
     (lambda L: L.ppk_causal_conv_fwd(0, 5, 0, 8, 4, None, None, None, 16, None, None, 1, None, None, strides(4), None), 0),
     (lambda L: L.ppk_causal_conv_bwd(0, 1, 1, 8, 4, None, None, 16, 16, None, None, 1, 16, None, 16, 16, None, None, strides(6), 256, 8, None), -3),
     (lambda L: L.ppk_causal_conv_step(0, 1, 8, 4, 16, 8, None, 16, None, 1, 16, None, None), -6),
-    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 65, 1, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -4),
-    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 3, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -1),
-    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 1, 16, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None), -6),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 65, 1, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None, 0, None), -4),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 3, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None, 0, None), -1),
+    (lambda L: L.ppk_selective_scan_fwd(0, 1, 1, 8, 4, 1, 16, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None, 0, None), -6),
+    (lambda L: L.ppk_selective_scan_fwd(0, 4096, 1, 8, 4, 1, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None, 0, None), -3),
     (lambda L: L.ppk_selective_scan_bwd(0, 2, 1, 8, 4, 1, 2, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 8, None), -3),
     (lambda L: L.ppk_selective_scan_bwd(0, 2, 1, 8, 4, 1, 3, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 8, None), -1),
     (lambda L: L.ppk_selective_scan_step(0, 1, 8, 4, 1, *[16] * 5, *[None] * 4, 1, 16, 16, strides(16), None), -6),
