@@ -51,7 +51,18 @@ __device__ __forceinline__ float lane_value(float v, int lane) { return __uint_a
 // memory that the kernel does not write, at an address that all lanes share: loaded into scalar registers
 #define UNIFORM __attribute__((address_space(4)))
 template <typename T> __device__ __forceinline__ const UNIFORM T* uniform(const void* p) { return (const UNIFORM T*)(uintptr_t)p; }
-__device__ __forceinline__ long long uni_row(const SeqBatch& q, long long t) { return q.off ? uniform<long long>(q.off)[t] : t; }
+__device__ __forceinline__ unsigned uni_row(const SeqBatch& q, long long t) { return q.off ? (unsigned)uniform<long long>(q.off)[t] : (unsigned)t; }
+// Addresses: a base and a step's offset that all lanes share, in scalar registers, and a lane's own 32-bit offset in bytes.  A batch has
+// fewer than 2^31 steps and rows, and a row's stride is below 2^32 bytes (the host sees to it): their product is two 32-bit ones.
+template <typename T> struct Rows {
+    const char* base;
+    unsigned stride;
+    __device__ __forceinline__ Rows(const void* p, long long offset, long long stride_)
+        : base((const char*)p + offset * (long long)sizeof(T)), stride((unsigned)(stride_ * (long long)sizeof(T))) {}
+    __device__ __forceinline__ const char* row(unsigned r) const { return base + (unsigned long long)r * stride; }
+    __device__ __forceinline__ T get(unsigned r, unsigned byte) const { return *(const T*)(row(r) + byte); }
+    __device__ __forceinline__ void put(unsigned r, unsigned byte, T v) const { *(T*)(const_cast<char*>(row(r)) + byte) = v; }
+};
 __device__ __forceinline__ long long uni_len(const SeqBatch& q, long long b) { return q.len ? uniform<long long>(q.len)[b] : q.T; }
 __device__ __forceinline__ long long first_tile(const ScanArgs& a, long long b) { return a.tiles ? uniform<long long>(a.tiles)[b] : b * ((a.q.T + TILE - 1) / TILE); }
 
@@ -105,8 +116,8 @@ template <int NP> __device__ __forceinline__ void store_states(float* p, int N, 
 // What a wave of the kernels with a lane a channel works on: 64 channels of a group of one sequence, one split of its steps
 struct Item {
     long long b, t0, t1, len;
-    int s, g, d;                               // split, group, this lane's channel (a channel of the group where it has none of its own)
-    bool live;
+    int s, g, d;                               // split, group, this lane's channel (a lane behind a group's last channel does that one again,
+                                               // and stores the same values to the same places: no lane is masked)
     __device__ __forceinline__ Item(const ScanArgs& a)
     {
         const int nb = a.G * a.blocks_per_group, cb = (int)(blockIdx.x % nb);
@@ -115,8 +126,7 @@ struct Item {
         b = rest / a.splits;
         g = cb / a.blocks_per_group;
         const int dl = (cb % a.blocks_per_group) * 64 + (int)threadIdx.x;
-        live = dl < a.per;
-        d = g * a.per + (live ? dl : 0);
+        d = g * a.per + (dl < a.per ? dl : a.per - 1);
         len = uni_len(a.q, b);
         t0 = s * a.span;
         t1 = t0 + a.span < len ? t0 + a.span : len;
@@ -124,7 +134,17 @@ struct Item {
 };
 __device__ __forceinline__ long long carry_at(const ScanArgs& a, long long b, int s, int d) { return (b * a.splits + s) * a.D + d; }
 
-constexpr int AHEAD = 8;                       // steps whose elements are loaded before those of the steps before them are used
+constexpr int AHEAD = 4;                       // steps whose elements are loaded before those of the steps before them are used
+
+// rows of AHEAD steps from t on, in direction dir, none behind `last`
+__device__ __forceinline__ void rows_of(const SeqBatch& q, long long t, long long last, int dir, unsigned (&rows)[AHEAD])
+{
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) { const long long u = t + dir * i; rows[i] = (unsigned)(dir > 0 ? (u < last ? u : last) : (u > last ? u : last)); }
+    if (q.off)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) rows[i] = (unsigned)uniform<long long>(q.off)[rows[i]];
+}
 
 // The forward pass: a lane a channel with its NP >= N states in registers, B and C of a step in scalar registers (SCALAR) or handed over
 // from lanes.  PART: only the state at the end of a split that begins with none, and the sum of its dt.
@@ -146,39 +166,37 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     for (int n = 0; n < NP; ++n) A2[n] *= LOG2E;
     const float skip = !PART && a.skip ? a.skip[it.d] : 0.f, bias = a.bias ? a.bias[it.d] : 0.f;
     const long long tile0 = first_tile(a, it.b);
-    const T *xp = (const T*)a.x + it.b * a.xs.b, *rp = (const T*)a.raw + it.b * a.raws.b, *zp = (const T*)a.z + it.b * a.zs.b;
-    const T *Bp = (const T*)a.Bm + it.b * a.Bs.b + it.g * a.Bg, *Cp = (const T*)a.Cm + it.b * a.Cs.b + it.g * a.Cg;
-    T* yp = (T*)a.y + it.b * a.rows.b * a.D;
-    const unsigned d = (unsigned)it.d;
+    const Rows<T> xs(a.x, it.b * a.xs.b, a.xs.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
+    const Rows<T> Bs(a.Bm, it.b * a.Bs.b + it.g * a.Bg, a.Bs.t), Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t), ys(a.y, it.b * a.rows.b * a.D, a.rows.t * a.D);
+    const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
     const bool gate = !PART && a.z;
     T xv[AHEAD], rv[AHEAD], zv[AHEAD];
-    long long rows[AHEAD];
-    const auto fetch = [&](long long t) {
+    unsigned rows[AHEAD];
+    const auto fetch = [&](long long t) {      // steps t, t + 1, ...; behind the last one, the last one
+        rows_of(a.q, t, t1 - 1, 1, rows);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const long long r = uni_row(a.q, t + i < t1 ? t + i : t1 - 1);
-            rows[i] = r;
-            xv[i] = (xp + r * a.xs.t)[d];
-            rv[i] = (rp + r * a.raws.t)[d];
-            if (gate) zv[i] = (zp + r * a.zs.t)[d];
-        }
+        for (int i = 0; i < AHEAD; ++i) { xv[i] = xs.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
+        if (gate)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) zv[i] = zs.get(rows[i], d);
     };
     float sum = 0.f;
     if (t0 < t1) fetch(t0);
     for (long long t = t0; t < t1; t += AHEAD) {
-        if (!PART && a.kept && t % TILE == 0 && it.live) store_states<NP>(a.kept + ((tile0 + t / TILE) * a.D + it.d) * N, N, h);
+        if (!PART && a.kept && t % TILE == 0) store_states<NP>(a.kept + ((tile0 + t / TILE) * a.D + it.d) * N, N, h);
         float x[AHEAD], raw[AHEAD], z[AHEAD];
-        long long r[AHEAD];
+        unsigned r[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) { x[i] = to_f32(xv[i]); raw[i] = to_f32(rv[i]) + bias; z[i] = gate ? to_f32(zv[i]) : 0.f; r[i] = rows[i]; }
         if (t + AHEAD < t1) fetch(t + AHEAD);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (t + i >= t1) break;
+            __builtin_amdgcn_sched_barrier(0);     // one step's scalars at a time: those of eight do not fit
             RowVec<T, NP, SCALAR> Bv, Cv;
-            Bv.load(Bp + r[i] * a.Bs.t, lane, N);
-            if (!PART) Cv.load(Cp + r[i] * a.Cs.t, lane, N);
-            const float dt = a.softplus ? softplus(raw[i]) : raw[i], dx = dt * x[i];
+            Bv.load((const T*)Bs.row(r[i]), lane, N);
+            if (!PART) Cv.load((const T*)Cs.row(r[i]), lane, N);
+            // a step behind the last is the last one again, with dt = 0: the state stays, and y is stored a second time
+            const float s = a.softplus ? softplus(raw[i]) : raw[i], dt = t + i < t1 ? s : 0.f, dx = dt * x[i];
             float y[4] = {skip * x[i], 0.f, 0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
@@ -188,10 +206,9 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
             if (PART) { sum += dt; continue; }
             float out = (y[0] + y[1]) + (y[2] + y[3]);
             if (gate) out *= z[i] * sigmoid(z[i]);
-            if (it.live) (yp + r[i] * a.rows.t * a.D)[d] = from_f32<T>(out);
+            ys.put(r[i], d, from_f32<T>(out));
         }
     }
-    if (!it.live) return;
     if (PART) {
         store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, h);
         a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
@@ -212,26 +229,24 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 #pragma unroll
     for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
     const float bias = a.bias ? a.bias[it.d] : 0.f;
-    const T *dp = (const T*)a.dy + it.b * a.dys.b, *rp = (const T*)a.raw + it.b * a.raws.b, *zp = (const T*)a.z + it.b * a.zs.b;
-    const T* Cp = (const T*)a.Cm + it.b * a.Cs.b + it.g * a.Cg;
-    const unsigned d = (unsigned)it.d;
+    const Rows<T> ds(a.dy, it.b * a.dys.b, a.dys.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
+    const Rows<T> Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t);
+    const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
     T dv[AHEAD], rv[AHEAD], zv[AHEAD];
-    long long rows[AHEAD];
-    const auto fetch = [&](long long t) {      // steps t - 1, t - 2, ...
+    unsigned rows[AHEAD];
+    const auto fetch = [&](long long t) {      // steps t - 1, t - 2, ...; before the first one, the first one
+        rows_of(a.q, t - 1, t0, -1, rows);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const long long r = uni_row(a.q, t - 1 - i >= t0 ? t - 1 - i : t0);
-            rows[i] = r;
-            dv[i] = (dp + r * a.dys.t)[d];
-            rv[i] = (rp + r * a.raws.t)[d];
-            if (a.z) zv[i] = (zp + r * a.zs.t)[d];
-        }
+        for (int i = 0; i < AHEAD; ++i) { dv[i] = ds.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
+        if (a.z)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) zv[i] = zs.get(rows[i], d);
     };
     float sum = 0.f;
     fetch(t1);
     for (long long t = t1; t > t0; t -= AHEAD) {
         float dy[AHEAD], raw[AHEAD];
-        long long r[AHEAD];
+        unsigned r[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             const float z = a.z ? to_f32(zv[i]) : 0.f;
@@ -242,16 +257,16 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
         if (t - AHEAD > t0) fetch(t - AHEAD);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (t - 1 - i < t0) break;
+            __builtin_amdgcn_sched_barrier(0);
             RowVec<T, NP, SCALAR> Cv;
-            Cv.load(Cp + r[i] * a.Cs.t, lane, N);
-            const float dt = a.softplus ? softplus(raw[i]) : raw[i];
+            Cv.load((const T*)Cs.row(r[i]), lane, N);
+            const bool in = t - 1 - i >= t0;
+            const float s = a.softplus ? softplus(raw[i]) : raw[i], dt = in ? s : 0.f, u = in ? dy[i] : 0.f;
             sum += dt;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(dy[i], Cv.at(n), g[n]);
+            for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(u, Cv.at(n), g[n]);
         }
     }
-    if (!it.live) return;
     store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, g);
     a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
 }
@@ -317,13 +332,15 @@ template <int LPC> __device__ __forceinline__ float sum_slices(float v)
     return v;
 }
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // The backward pass.  A block takes 256 / LPC channels of a group of one sequence and walks a split's tiles backwards; a thread holds the
 // four states 4 slice .. of a channel.  In a wave, lane % 16 = slice * (16 / LPC) + low bits of the channel, lane / 16 = its high bits:
 //   sums over states go over the slices, within a row of 16 lanes (two to four DPP additions);
-//   sums over channels (dB, dC of a step: eight values a thread) go over lane / 16 in the matrix unit, v_mfma_f32_16x16x4f32 with the
-//   value as A and a unit column as B: 16 of them put 2 steps' values into 16 columns of one accumulator, whose rows are lane % 16, so
-//   that the four registers of a lane are the low bits of the channel (and of the slice).  The products are with 1 and 0: exact.
+//   sums over channels (dB, dC of a step: eight values a thread) halve what a lane holds at each exchange of half waves.
+//   The matrix unit can make them too, with the value as one operand and a unit column as the other: 128 products a tile instead of
+//   256 vector instructions, and slower: 1574 against 1222 us on 2048 sequences of 20 to 100 steps, 512 channels, 16 states, fp32, where the
+//   matrix unit and the vector unit were busy for 80 % of the time together, one after the other.
 // Elements of a tile are loaded while the tile behind it is worked on, and what the tile's end needs of them waits in LDS.
 template <typename T, int LPC>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
@@ -331,9 +348,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
     constexpr int NP = 4 * LPC, BC = 256 / LPC, PE = TILE * BC / 256, CL = 16 / LPC, BCE = TILE * 2 * NP / 256;
     __shared__ float s_dt[TILE][BC], s_dx[TILE][BC], s_dy[TILE][BC];           // dt, dt x, dy'
     __shared__ float s_x[TILE][BC], s_slope[TILE][BC], s_gz[TILE][BC];         // x, d dt / d raw, dout silu'(z)
-    __shared__ float s_q1[TILE][BC], s_q2[TILE][BC], s_q3[TILE][BC];           // sums over n of dh B, da A, C h
+    __shared__ float s_q[4][TILE][BC];                                         // sums over n of dh B, da A, C h
     __shared__ __align__(16) float s_BC[TILE][2 * NP];
-    __shared__ float s_red[TILE][4][2 * NP];
+    __shared__ __align__(16) float s_red[TILE][4][2 * NP];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int ns = (lane & 15) / CL, ch = wave * (64 / LPC) + (lane >> 4) * CL + (lane & (CL - 1));    // the scan's slice and channel
     const int pc = tid % BC, pt = BC >= 64 ? __builtin_amdgcn_readfirstlane(tid / BC) : tid / BC;      // channel and first step of the per-element work
@@ -346,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
     const int d = g * a.per + (live ? base + ch : 0), pd = g * a.per + (plive ? base + pc : 0);
     const long long len = uni_len(a.q, b), end = (s + 1) * a.span < len ? (s + 1) * a.span : len;
     const long long tile0 = first_tile(a, b);
-    float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dh[4], pick[16];
+    float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dh[4];
     const float* into = a.splits > 1 && s * a.span < len ? a.carry + carry_at(a, b, s, d) * N : (a.dlast ? a.dlast + (b * a.D + d) * N : nullptr);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -354,38 +371,49 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
         A2[j] = live && n < N ? a.A[(long long)d * N + n] * LOG2E : 0.f;
         dh[j] = live && n < N && into ? into[n] : 0.f;
     }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) pick[k] = (lane & 15) == k ? 1.0f : 0.0f;
     const float skip = a.skip && plive ? a.skip[pd] : 0.f, bias = a.bias && plive ? a.bias[pd] : 0.f;
     float dskip = 0.f, dbias = 0.f;
 
+    const Rows<T> xs(a.x, b * a.xs.b, a.xs.t), rs(a.raw, b * a.raws.b, a.raws.t), ds(a.dy, b * a.dys.b, a.dys.t);
+    const Rows<T> zs(a.z ? a.z : a.x, b * (a.z ? a.zs.b : a.xs.b), a.z ? a.zs.t : a.xs.t);      // no gate: x again, unused
+    const unsigned pb = (unsigned)pd * (unsigned)sizeof(T);
+    // this thread's element of a row's B and C: column (tid % (2 NP)) of every 256 / (2 NP)-th row
+    const int bk = tid % (2 * NP), bn = bk % NP, bt = tid / (2 * NP);
+    const Rows<T> bcs(bk < NP ? a.Bm : a.Cm, (bk < NP ? b * a.Bs.b + g * a.Bg : b * a.Cs.b + g * a.Cg) + (bn < N ? bn : 0), bk < NP ? a.Bs.t : a.Cs.t);
+    const Rows<T> dxs(a.dx, b * a.rows.b * a.D, a.rows.t * a.D), drs(a.draw, b * a.rows.b * a.D, a.rows.t * a.D), dzs(a.dz, b * a.rows.b * a.D, a.rows.t * a.D);
+    const float* h0 = a.kept + (tile0 * a.D + d) * N + (ns * 4 < N ? ns * 4 : 0);
     T xv[PE], rv[PE], dv[PE], zv[PE], bv[BCE];
-    float hv[4];
+    unsigned row[PE], brow[BCE];
+    f32x4 hv;
+    const auto locate = [&](long long tile) {                                  // the rows of a tile; a step behind the last is the first one again
+        const unsigned t0 = (unsigned)(tile * TILE);
+        const int steps = (int)(end - tile * TILE < TILE ? end - tile * TILE : TILE);
+#pragma unroll
+        for (int i = 0; i < PE; ++i) { const int t = pt + i * (256 / BC); row[i] = t0 + (t < steps ? t : 0); }
+#pragma unroll
+        for (int i = 0; i < BCE; ++i) { const int t = bt + i * (256 / (2 * NP)); brow[i] = t0 + (t < steps ? t : 0); }
+        if (!a.q.off) return;
+#pragma unroll
+        for (int i = 0; i < PE; ++i) row[i] = BC >= 64 ? (unsigned)uniform<long long>(a.q.off)[row[i]] : (unsigned)a.q.off[row[i]];
+#pragma unroll
+        for (int i = 0; i < BCE; ++i) brow[i] = (unsigned)a.q.off[brow[i]];
+    };
     const auto fetch = [&](long long tile) {
-        const long long t0 = tile * TILE;
-        const int steps = (int)(end - t0 < TILE ? end - t0 : TILE);
 #pragma unroll
         for (int i = 0; i < PE; ++i) {
-            const int t = pt + i * (256 / BC);
-            const long long at_t = t0 + (t < steps ? t : 0), r = BC >= 64 ? uni_row(a.q, at_t) : a.q.row(at_t);
-            xv[i] = ((const T*)a.x + at(a.xs, r, b))[(unsigned)pd];
-            rv[i] = ((const T*)a.raw + at(a.raws, r, b))[(unsigned)pd];
-            dv[i] = ((const T*)a.dy + at(a.dys, r, b))[(unsigned)pd];
-            if (a.z) zv[i] = ((const T*)a.z + at(a.zs, r, b))[(unsigned)pd];
+            xv[i] = xs.get(row[i], pb);
+            rv[i] = rs.get(row[i], pb);
+            dv[i] = ds.get(row[i], pb);
+            zv[i] = zs.get(row[i], pb);
         }
 #pragma unroll
-        for (int i = 0; i < BCE; ++i) {
-            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP), n = k % NP;
-            const long long r = a.q.row(t0 + (t < steps ? t : 0));
-            const int m = n < N ? n : 0;
-            bv[i] = k < NP ? ((const T*)a.Bm)[at(a.Bs, r, b) + g * a.Bg + m] : ((const T*)a.Cm)[at(a.Cs, r, b) + g * a.Cg + m];
-        }
-        const float* h0 = a.kept + ((tile0 + tile) * a.D + d) * N;
+        for (int i = 0; i < BCE; ++i) bv[i] = bcs.get(brow[i], 0);
+        const float* p = h0 + tile * (long long)a.D * N;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) hv[j] = h0[ns * 4 + j < N ? ns * 4 + j : 0];
+        for (int j = 0; j < 4; ++j) hv[j] = p[ns * 4 + j < N ? j : 0];
     };
     const long long tile_end = (end + TILE - 1) / TILE, tile_begin = s * (a.span / TILE);
-    if (tile_end > tile_begin) fetch(tile_end - 1);
+    if (tile_end > tile_begin) { locate(tile_end - 1); fetch(tile_end - 1); }
     for (long long tile = tile_end - 1; tile >= tile_begin; --tile) {
         const long long t0 = tile * TILE;
         const int steps = (int)(end - t0 < TILE ? end - t0 : TILE);
@@ -410,12 +438,14 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
         }
 #pragma unroll
         for (int i = 0; i < BCE; ++i) {
-            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP);
-            s_BC[t][k] = t < steps && k % NP < N ? to_f32(bv[i]) : 0.f;
+            const int t = bt + i * (256 / (2 * NP));
+            s_BC[t][bk] = t < steps && bn < N ? to_f32(bv[i]) : 0.f;
         }
         float h[TILE + 1][4], av[TILE][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[0][j] = live && ns * 4 + j < N ? hv[j] : 0.f;
+        const long long next = tile > tile_begin ? tile - 1 : tile;
+        locate(next);
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < TILE; ++t) {
@@ -428,10 +458,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
             }
         }
         asm volatile("" ::: "memory");           // the steps' values are read from LDS again: kept, they would be 96 registers
-        f32x4 acc;
 #pragma unroll
         for (int t = TILE - 1; t >= 0; --t) {
-            if (t == TILE - 6 && tile > tile_begin) fetch(tile - 1);            // where the registers of five steps are free again
+            if (t == TILE - 6) fetch(next);                                     // where the registers of five steps are free again
             const float dtv = s_dt[t][ch], dxv = s_dx[t][ch], dyv = s_dy[t][ch];
             const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]), Cv = *reinterpret_cast<const f32x4*>(&s_BC[t][NP + ns * 4]);
             float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
@@ -450,43 +479,43 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
             q1 = sum_slices<LPC>(q1);
             q2 = sum_slices<LPC>(q2);
             q3 = sum_slices<LPC>(q3);
-            if (ns == 0) { s_q1[t][ch] = q1; s_q2[t][ch] = q2; s_q3[t][ch] = q3; }
-            if (t & 1) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+            s_q[ns & 3][t][ch] = (ns & 3) == 0 ? q1 : (ns & 3) == 1 ? q2 : q3;   // every slice holds all three: the fourth writes nobody's
+            // over the wave's channels: two exchanges of halves leave a lane the sums of two of the eight values (bit 5 of the lane: dC,
+            // bit 4: the upper two states), the low bits of the channel follow within a row of 16
+            float u[4], w[2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v[k], pick[(t & 1) * 8 + k], acc, 0, 0, 0);
-            if (!(t & 1)) {
-                // this lane: column lane % 16 = a step and one of its values, rows 4 (lane / 16) + r = slice * CL + low bits of the channel
-                const int step = t + ((lane >> 3) & 1), side = ((lane >> 2) & 1) * NP, j = lane & 3, q = lane >> 4;
-                if (LPC == 4) s_red[step][wave][side + q * 4 + j] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                if (LPC == 8) {
-                    s_red[step][wave][side + (q * 2) * 4 + j] = acc[0] + acc[1];
-                    s_red[step][wave][side + (q * 2 + 1) * 4 + j] = acc[2] + acc[3];
-                }
-                if (LPC == 16)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s_red[step][wave][side + (q * 4 + r) * 4 + j] = acc[r];
+            for (int k = 0; k < 4; ++k) {
+                const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(v[k + 4]), false, false);
+                u[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
             }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[k + 2]), false, false);
+                w[k] = sum_low<CL>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+            }
+            // CL lanes hold the same two sums and store them to the same place
+            *reinterpret_cast<f32x2*>(&s_red[t][wave][(lane >> 5) * NP + ns * 4 + ((lane >> 4) & 1) * 2]) = f32x2{w[0], w[1]};
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PE; ++i) {
             const int t = pt + i * (256 / BC);
             if (!(plive && t < steps)) continue;
-            const long long r = BC >= 64 ? uni_row(a.q, t0 + t) : a.q.row(t0 + t), o = at(a.rows, r, b) * a.D;
-            const float q1 = s_q1[t][pc], x = s_x[t][pc], dy = s_dy[t][pc];
-            const float dr = fmaf(x, q1, s_q2[t][pc] * LN2) * s_slope[t][pc];
-            ((T*)a.dx + o)[(unsigned)pd] = from_f32<T>(fmaf(s_dt[t][pc], q1, skip * dy));
-            ((T*)a.draw + o)[(unsigned)pd] = from_f32<T>(dr);
-            if (a.z) ((T*)a.dz + o)[(unsigned)pd] = from_f32<T>(s_gz[t][pc] * fmaf(skip, x, s_q3[t][pc]));
+            const unsigned r = BC >= 64 ? uni_row(a.q, t0 + t) : (unsigned)a.q.row(t0 + t);
+            const float q1 = s_q[0][t][pc], x = s_x[t][pc], dy = s_dy[t][pc];
+            const float dr = fmaf(x, q1, s_q[1][t][pc] * LN2) * s_slope[t][pc];
+            dxs.put(r, pb, from_f32<T>(fmaf(s_dt[t][pc], q1, skip * dy)));
+            drs.put(r, pb, from_f32<T>(dr));
+            if (a.z) dzs.put(r, pb, from_f32<T>(s_gz[t][pc] * fmaf(skip, x, s_q[2][t][pc])));
             dskip = fmaf(dy, x, dskip);
             dbias += dr;
         }
 #pragma unroll
         for (int i = 0; i < BCE; ++i) {
-            const int e = tid + i * 256, t = e / (2 * NP), k = e % (2 * NP), n = k % NP;
-            if (t >= steps || n >= N) continue;
+            const int t = bt + i * (256 / (2 * NP));
+            if (t >= steps || bn >= N) continue;
             const long long row = at(a.rows, a.q.row(t0 + t), b);
-            a.pBC[(((long long)cg * a.nrows + row) * a.G + g) * 2 * N + (k / NP) * N + n] = (s_red[t][0][k] + s_red[t][1][k]) + (s_red[t][2][k] + s_red[t][3][k]);
+            a.pBC[(((long long)cg * a.nrows + row) * a.G + g) * 2 * N + (bk < NP ? 0 : N) + bn] = (s_red[t][0][bk] + s_red[t][1][bk]) + (s_red[t][2][bk] + s_red[t][3][bk]);
         }
         __syncthreads();
     }
@@ -629,12 +658,20 @@ template <typename T> void run_step(const ScanArgs& a, unsigned blocks, const fl
     }
 }
 
+// rows are at most 2^32 bytes apart (a tensor of strides that reach further is copied by its caller)
+bool near_rows(const int64_t* s, long long D)
+{
+    for (int i : {0, 2, 4, 7, 10, 14})
+        if (s[i] < 0 || s[i] >= 1LL << 30) return false;
+    return s[12] >= 0 && s[12] < (1LL << 30) / D;
+}
 int scan_check(const char* what, int dtype, long long T, long long B, long long D, long long N, long long G)
 {
     if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "%s: type %d (fp32 and bf16 are supported)", what, dtype);
     if (T < 0 || B < 0 || D < 1 || N < 1 || G < 1 || D % G) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld N=%lld G=%lld", what, T, B, D, N, G);
     if (N > 64) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld states a channel (at most 64)", what, N);
     if (D > (1 << 20)) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld channels", what, D);
+    if (T >= 1LL << 31) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld steps", what, T);
     return PPK_OK;
 }
 
@@ -685,6 +722,7 @@ int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
     if (B == 0) return PPK_OK;
     if (!A || !last_state || !strides_host || (T > 0 && (!x || !raw || !Bm || !Cm || !y))) PPK_FAIL(PPK_ERR_NULL, "selective_scan_fwd: null pointer");
     if (step_off && (!lengths || !tiles)) PPK_FAIL(PPK_ERR_NULL, "selective_scan_fwd: a packed batch needs its lengths and tiles");
+    if (!near_rows(strides_host, D)) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_fwd: rows 2^30 elements or more apart");
     ScanArgs a = {};
     a.q = {step_off, lengths, T, B};
     a.tiles = tiles;
@@ -726,10 +764,11 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
 {
     int rc = scan_check("selective_scan_bwd", dtype, T, B, D, N, G);
     if (rc) return rc;
-    if (rows < 0 || (!step_off && rows != T * B)) PPK_FAIL(PPK_ERR_SHAPE, "selective_scan_bwd: %lld rows", (long long)rows);
+    if (rows < 0 || rows >= 1LL << 31 || (!step_off && rows != T * B)) PPK_FAIL(PPK_ERR_SHAPE, "selective_scan_bwd: %lld rows", (long long)rows);
     if (!A || !dA || !workspace || !strides_host || (rows > 0 && (!x || !raw || !Bm || !Cm || !dy || !kept || !dx || !draw || !dB || !dC || (z && !dz))))
         PPK_FAIL(PPK_ERR_NULL, "selective_scan_bwd: null pointer");
     if (step_off && (!lengths || !tiles)) PPK_FAIL(PPK_ERR_NULL, "selective_scan_bwd: a packed batch needs its lengths and tiles");
+    if (!near_rows(strides_host, D)) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_bwd: rows 2^30 elements or more apart");
     const BwdWs w = bwd_ws(T, B, D, N, G, rows);
     const long long items = B * w.p.splits;
     if (ws_bytes < w.total) PPK_FAIL(PPK_ERR_WS, "selective_scan_bwd: workspace of %zu bytes, %zu needed", ws_bytes, w.total);

@@ -26,6 +26,7 @@ from . import _C
 _lib = _C.lib
 MAX_TAPS = 8
 MAX_STATES = 64
+FAR_ROWS = 1 << 30                 # the kernels take rows that are fewer elements apart; others are copied
 
 
 class PackedRows(NamedTuple):
@@ -107,7 +108,8 @@ class _Batch:
             raise ValueError(f'{self.what}: {name} must be {[*self.lead, *tail]}, not {list(t.shape) if torch.is_tensor(t) else t}')
         if t.dtype != dtype:
             raise TypeError(f'{self.what}: {name} must be {dtype}, as x is')
-        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+        near = max(t.stride()[:2], default=0) < FAR_ROWS
+        return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
 
     def strides(self, t):
         """Of a step and of a sequence, in elements."""
