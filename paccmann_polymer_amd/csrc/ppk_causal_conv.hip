@@ -1,8 +1,8 @@
 // Short causal convolution of each channel over packed or rectangular batches of sequences, with the K - 1 inputs before the first
 // step as its state:  pre_t = bias + sum_k w_k x_{t-K+1+k},  y = pre or pre sigmoid(pre).
 //   backward: dpre = dy act'(pre);  dx_t = sum_k w_k dpre_{t+K-1-k};  dw_k = sum_t dpre_t x_{t-K+1+k};  db = sum_t dpre_t
-// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx.  A wave takes RUN steps of a sequence with the
-// window in registers, VEC channels a lane in 16-byte accesses; its neighbours' K - 1 rows come from the L2.
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx.  A wave takes a run of steps of a sequence with the
+// window in registers, VEC channels a lane; its neighbours' K - 1 rows come from the L2.
 #include "ppk_seq_rows.h"
 
 namespace ppk {
@@ -54,13 +54,17 @@ namespace {
 using ppk::SeqBatch;
 using ppk::Stride;
 using ppk::at;
+using ppk::Rows;
+using ppk::uni_len;
+using ppk::uniform;
 
-constexpr int RUN = 16;                       // steps a wave takes at a time
-constexpr int MAX_SUM_BLOCKS = 512;           // blocks of a backward launch in the sequence direction: rows of its partial sums
+constexpr int AHEAD = 4;                      // steps whose elements are loaded before those of the steps before them are used
+constexpr int SUM_BLOCKS = 1024;              // blocks of a backward launch in all: each leaves a row of partial sums for its channels
+constexpr long long WANTED_WAVES = 8192;
 
 struct ConvArgs {
     SeqBatch q;
-    int D, K, runs;                           // runs: of the longest sequence
+    int D, K, run, runs;                      // steps of a run, and runs of the longest sequence
     const void *x, *state, *dy, *dlast;
     const float *weight, *bias;
     void *y, *last, *dx, *dstate;
@@ -69,23 +73,48 @@ struct ConvArgs {
     int silu;
 };
 
-template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC])
+// VEC elements as one access of VEC * sizeof(T) bytes
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) Vec { T v[VEC]; };
+template <typename T, int VEC> __device__ __forceinline__ void widen(const Vec<T, VEC>& p, float (&v)[VEC])
 {
-    if (VEC == 1) v[0] = to_f32(*p);
-    else unpack<T>(*reinterpret_cast<const uint4*>(p), v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = to_f32(p.v[e]);
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC])
+template <typename T, int VEC> __device__ __forceinline__ Vec<T, VEC> narrow(const float (&v)[VEC])
 {
-    if (VEC == 1) *p = from_f32<T>(v[0]);
-    else *reinterpret_cast<uint4*>(p) = pack<T>(v);
+    Vec<T, VEC> p;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) p.v[e] = from_f32<T>(v[e]);
+    return p;
 }
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) { widen<T, VEC>(*reinterpret_cast<const Vec<T, VEC>*>(p), v); }
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) { *reinterpret_cast<Vec<T, VEC>*>(p) = narrow<T, VEC>(v); }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
-// the input of step t, which is of the state before the first step; r = row of step t where t >= 0
-template <typename T, int VEC>
-__device__ __forceinline__ void input_at(const ConvArgs& a, long long t, long long b, int c, float (&v)[VEC])
+// A wave's (CL == 64) or a row of 16 lanes' run of a sequence.  Runs at the same steps of sequences next to each other are worked on
+// together: their rows are next to each other in a packed batch.
+template <int CL> struct Run {
+    long long b, t0, t1, len;
+    bool any;
+    __device__ __forceinline__ Run(const ConvArgs& a, long long item)
+    {
+        if (CL == 64) item = ((long long)__builtin_amdgcn_readfirstlane((int)(item >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)item);
+        const long long k = item / a.q.B;
+        b = item - k * a.q.B;
+        any = k < a.runs;
+        t0 = k * a.run;
+        len = !any ? 0 : CL == 64 ? uni_len(a.q, b) : a.q.length(b);
+        if (t0 >= len && t0 > 0) any = false;
+        t1 = t0 + a.run < len ? t0 + a.run : len;
+    }
+};
+template <int CL> __device__ __forceinline__ unsigned row_of(const SeqBatch& q, long long t) { return CL == 64 ? ppk::uni_row(q, t) : (unsigned)q.row(t); }
+
+// the input of step t, which is of the state before the first step
+template <typename T, int VEC, int CL>
+__device__ __forceinline__ void input_at(const ConvArgs& a, const Rows<T>& xs, long long t, long long b, int c, float (&v)[VEC])
 {
-    if (t >= 0) { load_vec<T, VEC>((const T*)a.x + at(a.xs, a.q.row(t), b) + c, v); return; }
+    if (t >= 0) { widen<T, VEC>(xs.template get_as<Vec<T, VEC>>(row_of<CL>(a.q, t), c * (unsigned)sizeof(T)), v); return; }
     const long long i = t + a.K - 1;
     if (i >= 0 && a.state) { load_vec<T, VEC>((const T*)a.state + (b * (a.K - 1) + i) * a.D + c, v); return; }
 #pragma unroll
@@ -102,113 +131,144 @@ template <int VEC, int KP> __device__ __forceinline__ void load_taps(const ConvA
     }
 }
 
-// block 256 = 256 / CL items (a run of a sequence) x CL lanes of VEC channels
+// block 256 = 256 / CL runs x CL lanes of VEC channels
 template <typename T, int VEC, int KP, int CL>
-__global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a)
+__global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a, int channel_blocks)
 {
-    const int c = (blockIdx.y * CL + threadIdx.x % CL) * VEC;
-    const long long item = (long long)blockIdx.x * (256 / CL) + threadIdx.x / CL;
-    const long long b = item / a.runs, t0 = (item % a.runs) * RUN;
-    if (c >= a.D || b >= a.q.B) return;
-    const long long len = a.q.length(b);
-    if (t0 >= len && t0 > 0) return;
-    const long long t1 = t0 + RUN < len ? t0 + RUN : len;
+    const int c = ((int)(blockIdx.x % channel_blocks) * CL + threadIdx.x % CL) * VEC;
+    const Run<CL> run(a, (long long)(blockIdx.x / channel_blocks) * (256 / CL) + threadIdx.x / CL);
+    if (c >= a.D || !run.any) return;
+    const long long b = run.b, t0 = run.t0, t1 = run.t1;
+    const Rows<T> xs(a.x, b * a.xs.b, a.xs.t), ys(a.y, b * a.ys.b, a.ys.t);
+    const unsigned cb = c * (unsigned)sizeof(T);
+    Vec<T, VEC> next[AHEAD];
+    unsigned rows[AHEAD], r[AHEAD];
+    const auto fetch = [&](long long t) {                    // behind the last step, that one again
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) rows[i] = row_of<CL>(a.q, t + i < t1 ? t + i : t1 - 1);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) next[i] = xs.template get_as<Vec<T, VEC>>(rows[i], cb);
+    };
+    if (t0 < t1) fetch(t0);
     float w[KP][VEC], bias[VEC], win[KP][VEC];
     load_taps<VEC, KP>(a, c, w, bias);
 #pragma unroll
-    for (int j = 0; j < KP - 1; ++j) input_at<T, VEC>(a, t0 - (KP - 1) + j, b, c, win[j]);
-#pragma unroll 4
-    for (long long t = t0; t < t1; ++t) {
-        const long long r = a.q.row(t);
-        load_vec<T, VEC>((const T*)a.x + at(a.xs, r, b) + c, win[KP - 1]);
-        float out[VEC];
+    for (int j = 0; j < KP - 1; ++j) input_at<T, VEC, CL>(a, xs, t0 - (KP - 1) + j, b, c, win[j]);
+    for (long long t = t0; t < t1; t += AHEAD) {
+        float x[AHEAD][VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            float s = bias[e];
+        for (int i = 0; i < AHEAD; ++i) { widen<T, VEC>(next[i], x[i]); r[i] = rows[i]; }
+        if (t + AHEAD < t1) fetch(t + AHEAD);
 #pragma unroll
-            for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
-            out[e] = a.silu ? s * sigmoid(s) : s;
+        for (int i = 0; i < AHEAD; ++i) {
+            if (t + i >= t1) break;
+            float out[VEC];
 #pragma unroll
-            for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+            for (int e = 0; e < VEC; ++e) {
+                win[KP - 1][e] = x[i][e];
+                float s = bias[e];
+#pragma unroll
+                for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+                out[e] = a.silu ? s * sigmoid(s) : s;
+#pragma unroll
+                for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+            }
+            ys.template put_as<Vec<T, VEC>>(r[i], cb, narrow<T, VEC>(out));
         }
-        store_vec<T, VEC>((T*)a.y + at(a.ys, r, b) + c, out);
     }
-    if (t1 == len && a.last)
+    if (t1 == run.len && a.last)
 #pragma unroll
         for (int j = 0; j < KP - 1; ++j)
             if (j >= KP - a.K) store_vec<T, VEC>((T*)a.last + (b * (a.K - 1) + j - (KP - a.K)) * a.D + c, win[j]);
 }
 
 template <typename T, int VEC, int KP, int CL>
-__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a)
+__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks)
 {
     constexpr int IL = 256 / CL;
     __shared__ float red[IL][CL][VEC];
-    const int cl = threadIdx.x % CL, il = threadIdx.x / CL, c = (blockIdx.y * CL + cl) * VEC;
+    const int cl = threadIdx.x % CL, il = threadIdx.x / CL, c = ((int)(blockIdx.x % channel_blocks) * CL + cl) * VEC;
+    const long long first_block = blockIdx.x / channel_blocks, blocks = gridDim.x / channel_blocks;
+    const unsigned cb = c * (unsigned)sizeof(T);
     float dw[KP][VEC] = {}, db[VEC] = {};
     if (c < a.D) {
         float w[KP][VEC], bias[VEC];
         load_taps<VEC, KP>(a, c, w, bias);
         const long long items = a.q.B * a.runs;
-        for (long long item = (long long)blockIdx.x * IL + il; item < items; item += (long long)gridDim.x * IL) {
-            const long long b = item / a.runs, t0 = (item % a.runs) * RUN, len = a.q.length(b);
-            if (t0 >= len && t0 > 0) continue;
-            const long long t1 = t0 + RUN < len ? t0 + RUN : len, first = t0 == 0 ? -(long long)(a.K - 1) : t0;
+        for (long long item = first_block * IL + il; item < items; item += blocks * IL) {
+            const Run<CL> run(a, item);
+            if (!run.any) continue;
+            const long long b = run.b, t0 = run.t0, t1 = run.t1, len = run.len, first = t0 == 0 ? -(long long)(a.K - 1) : t0;
+            const Rows<T> xs(a.x, b * a.xs.b, a.xs.t), dys(a.dy, b * a.dys.b, a.dys.t), dxs(a.dx, b * a.ys.b, a.ys.t);
+            Vec<T, VEC> nx[AHEAD], nd[AHEAD];
+            const auto fetch = [&](long long t) {            // behind the sequence's last step, that one again
+                unsigned rows[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) rows[i] = row_of<CL>(a.q, t + i < len ? t + i : len - 1);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) { nx[i] = xs.template get_as<Vec<T, VEC>>(rows[i], cb); nd[i] = dys.template get_as<Vec<T, VEC>>(rows[i], cb); }
+            };
+            if (len > 0) fetch(t0);
             float win[KP][VEC], dp[KP][VEC];                 // inputs t - KP + 1 .. t; dp[j] = dpre of step t - j
 #pragma unroll
-            for (int j = 0; j < KP - 1; ++j) input_at<T, VEC>(a, t0 - (KP - 1) + j, b, c, win[j]);
+            for (int j = 0; j < KP - 1; ++j) input_at<T, VEC, CL>(a, xs, t0 - (KP - 1) + j, b, c, win[j]);
 #pragma unroll
             for (int j = 0; j < KP; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) dp[j][e] = 0.f;
-#pragma unroll 4
-            for (long long t = t0; t < t1 + KP - 1; ++t) {
+            const long long te = t1 + KP - 1;
+            for (long long tg = t0; tg < te; tg += AHEAD) {
+                float x[AHEAD][VEC], dy[AHEAD][VEC];
 #pragma unroll
-                for (int j = KP - 1; j > 0; --j)
+                for (int i = 0; i < AHEAD; ++i) { widen<T, VEC>(nx[i], x[i]); widen<T, VEC>(nd[i], dy[i]); }
+                if (tg + AHEAD < te && len > 0) fetch(tg + AHEAD);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
-                if (t < len) {
-                    const long long r = a.q.row(t);
-                    float dy[VEC];
-                    load_vec<T, VEC>((const T*)a.x + at(a.xs, r, b) + c, win[KP - 1]);
-                    load_vec<T, VEC>((const T*)a.dy + at(a.dys, r, b) + c, dy);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const long long t = tg + i;
+                    if (t >= te) break;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        float s = bias[e];
+                    for (int j = KP - 1; j > 0; --j)
 #pragma unroll
-                        for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
-                        if (a.silu) { const float g = sigmoid(s); dy[e] *= g * fmaf(s, 1.0f - g, 1.0f); }
-                        dp[0][e] = dy[e];
-                        if (t < t1) {
-                            db[e] += dy[e];
-#pragma unroll
-                            for (int j = 0; j < KP; ++j) dw[j][e] = fmaf(dy[e], win[j][e], dw[j][e]);
-                        }
-#pragma unroll
-                        for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
-                    }
-                } else {
+                        for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) dp[0][e] = 0.f;
-                }
-                const long long tt = t - (KP - 1);           // the step whose input's gradient is complete
-                if (tt < first || tt >= t1) continue;
-                float dx[VEC];
+                    if (t < len) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    dx[e] = 0.f;
+                        for (int e = 0; e < VEC; ++e) {
+                            win[KP - 1][e] = x[i][e];
+                            float s = bias[e], d = dy[i][e];
 #pragma unroll
-                    for (int j = 0; j < KP; ++j) dx[e] = fmaf(w[j][e], dp[j][e], dx[e]);
-                }
-                const long long i = tt - (len - (a.K - 1));
-                if (i >= 0 && a.dlast) {                     // the last K - 1 inputs are the new state too
-                    float g[VEC];
-                    load_vec<T, VEC>((const T*)a.dlast + (b * (a.K - 1) + i) * a.D + c, g);
+                            for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+                            if (a.silu) { const float g = sigmoid(s); d *= g * fmaf(s, 1.0f - g, 1.0f); }
+                            dp[0][e] = d;
+                            if (t < t1) {
+                                db[e] += d;
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) dx[e] += g[e];
+                                for (int j = 0; j < KP; ++j) dw[j][e] = fmaf(d, win[j][e], dw[j][e]);
+                            }
+#pragma unroll
+                            for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+                        }
+                    }
+                    const long long tt = t - (KP - 1);       // the step whose input's gradient is complete
+                    if (tt < first || tt >= t1) continue;
+                    float dx[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        dx[e] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < KP; ++j) dx[e] = fmaf(w[j][e], dp[j][e], dx[e]);
+                    }
+                    const long long k = tt - (len - (a.K - 1));
+                    if (k >= 0 && a.dlast) {                 // the last K - 1 inputs are the new state too
+                        float g[VEC];
+                        load_vec<T, VEC>((const T*)a.dlast + (b * (a.K - 1) + k) * a.D + c, g);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) dx[e] += g[e];
+                    }
+                    if (tt >= 0) dxs.template put_as<Vec<T, VEC>>(row_of<CL>(a.q, tt), cb, narrow<T, VEC>(dx));
+                    else if (a.dstate) store_vec<T, VEC>((T*)a.dstate + (b * (a.K - 1) + tt + a.K - 1) * a.D + c, dx);
                 }
-                if (tt >= 0) store_vec<T, VEC>((T*)a.dx + at(a.ys, a.q.row(tt), b) + c, dx);
-                else if (a.dstate) store_vec<T, VEC>((T*)a.dstate + (b * (a.K - 1) + tt + a.K - 1) * a.D + c, dx);
             }
         }
     }
@@ -226,7 +286,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a)
             for (int e = 0; e < VEC; ++e) {
                 float s = red[0][cl][e];
                 for (int i = 1; i < IL; ++i) s += red[i][cl][e];
-                a.part[((long long)blockIdx.x * (a.K + 1) + col) * a.D + c + e] = s;
+                a.part[(first_block * (a.K + 1) + col) * a.D + c + e] = s;
             }
         }
     }
@@ -269,9 +329,9 @@ int taps(long long K) { return K <= 2 ? 2 : K <= 4 ? 4 : 8; }
 
 template <typename T, int VEC, int KP, int CL> void launch_conv(const ConvArgs& a, bool bwd, unsigned blocks, hipStream_t st)
 {
-    const dim3 grid(blocks, (unsigned)((a.D + CL * VEC - 1) / (CL * VEC)));
-    if (bwd) k_conv_bwd<T, VEC, KP, CL><<<grid, 256, 0, st>>>(a);
-    else k_conv_fwd<T, VEC, KP, CL><<<grid, 256, 0, st>>>(a);
+    const int cb = (a.D + CL * VEC - 1) / (CL * VEC);
+    if (bwd) k_conv_bwd<T, VEC, KP, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
+    else k_conv_fwd<T, VEC, KP, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
 }
 template <typename T, int VEC, int KP> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
 {
@@ -286,40 +346,57 @@ template <typename T, int VEC> void launch_conv(const ConvArgs& a, bool bwd, int
         default: launch_conv<T, VEC, 8>(a, bwd, cl, blocks, st);
     }
 }
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int WIDE = 4;                       // channels of a lane where they can be loaded together: 16 bytes in fp32, 8 in bf16
 
-// 16-byte accesses where every row that a lane touches begins on one; single elements otherwise
+// accesses of WIDE elements where every row that a lane touches begins on one; single elements otherwise
 bool conv_vec(const ConvArgs& a, int elem)
 {
-    const int E = 16 / elem;
     const long long s = a.xs.t | a.xs.b | a.ys.t | a.ys.b | a.dys.t | a.dys.b | a.D;
-    return s % E == 0 && aligned16(a.x) && aligned16(a.state) && aligned16(a.dy) && aligned16(a.dlast) && aligned16(a.y) && aligned16(a.last) &&
-           aligned16(a.dx) && aligned16(a.dstate);
+    uintptr_t p = 0;
+    for (const void* q : {a.x, a.state, a.dy, a.dlast, (const void*)a.y, (const void*)a.last, (const void*)a.dx, (const void*)a.dstate}) p |= (uintptr_t)q;
+    return s % WIDE == 0 && p % (uintptr_t)(WIDE * elem) == 0;
 }
-long long conv_items(long long T, long long B) { const long long r = (T + RUN - 1) / RUN; return B * (r > 0 ? r : 1); }
-int conv_lanes(long long D, int vec) { return D <= 16 * vec ? 16 : 64; }
-long long conv_blocks(long long items, int cl) { return (items + 256 / cl - 1) / (256 / cl); }
-unsigned conv_sum_blocks(long long items, int cl) { const long long b = conv_blocks(items, cl); return (unsigned)(b < MAX_SUM_BLOCKS ? b : MAX_SUM_BLOCKS); }
+// How a launch is cut.  A run's K - 1 rows on either side are read again, so runs are as long as leaves enough waves to fill the card.
+struct ConvCut { int lanes, run, channel_blocks; long long runs, blocks; };
+ConvCut conv_cut(long long T, long long B, long long D, bool vec, bool bwd)
+{
+    ConvCut k;
+    const int w = vec ? WIDE : 1;
+    k.lanes = D <= 16 * w ? 16 : 64;
+    k.channel_blocks = (int)((D + k.lanes * w - 1) / (k.lanes * w));
+    for (k.run = 64; k.run > 8; k.run /= 2)
+        if (B * ((T + k.run - 1) / k.run) * k.channel_blocks * k.lanes / 64 >= WANTED_WAVES) break;
+    k.runs = T > 0 ? (T + k.run - 1) / k.run : 1;
+    k.blocks = (B * k.runs + 256 / k.lanes - 1) / (256 / k.lanes);
+    if (bwd) {
+        const long long most = k.channel_blocks >= SUM_BLOCKS / 64 ? 64 : SUM_BLOCKS / k.channel_blocks;
+        if (k.blocks > most) k.blocks = most;
+    }
+    return k;
+}
 
-int conv_check(const char* what, int dtype, long long T, long long B, long long D, long long K, const void* x, const float* w, const int64_t* strides)
+int conv_check(const char* what, int dtype, long long T, long long B, long long D, long long K, const void* x, const float* w, const int64_t* strides, int nstrides)
 {
     if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "%s: type %d (fp32 and bf16 are supported)", what, dtype);
     if (T < 0 || B < 0 || D < 1 || D > (1 << 20) || K < 1) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld K=%lld", what, T, B, D, K);
     if (K > 8) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld taps (at most 8)", what, K);
     if (!strides || !w || (B > 0 && T > 0 && !x)) PPK_FAIL(PPK_ERR_NULL, "%s: null pointer", what);
-    if (conv_blocks(conv_items(T, B), 64) > 0x7fffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "%s: T=%lld B=%lld", what, T, B);
+    if (T >= 1LL << 31 || B >= 1LL << 31 || conv_cut(T, B, D, false, false).blocks * conv_cut(T, B, D, false, false).channel_blocks > 0x7fffffffLL)
+        PPK_FAIL(PPK_ERR_UNSUP, "%s: T=%lld B=%lld D=%lld", what, T, B, D);
+    for (int i = 0; i < nstrides; i += 2)
+        if (strides[i] < 0 || strides[i] >= 1LL << 30) PPK_FAIL(PPK_ERR_UNSUP, "%s: rows 2^30 elements or more apart", what);
     return PPK_OK;
 }
 
-template <typename T> int conv_run(const ConvArgs& a, bool bwd, long long items, hipStream_t st)
+template <typename T> int conv_run(ConvArgs a, bool bwd, hipStream_t st)
 {
-    constexpr int E = 16 / (int)sizeof(T);
     const bool vec = conv_vec(a, (int)sizeof(T));
-    const int cl = conv_lanes(a.D, vec ? E : 1);
-    const unsigned blocks = bwd ? conv_sum_blocks(items, cl) : (unsigned)conv_blocks(items, cl);
-    if (vec) launch_conv<T, E>(a, bwd, cl, blocks, st);
-    else launch_conv<T, 1>(a, bwd, cl, blocks, st);
-    return (int)blocks;
+    const ConvCut k = conv_cut(a.q.T, a.q.B, a.D, vec, bwd);
+    a.run = k.run;
+    a.runs = (int)k.runs;
+    if (vec) launch_conv<T, WIDE>(a, bwd, k.lanes, (unsigned)k.blocks, st);
+    else launch_conv<T, 1>(a, bwd, k.lanes, (unsigned)k.blocks, st);
+    return (int)k.blocks;
 }
 
 }  // namespace
@@ -330,17 +407,17 @@ int ppk_causal_conv_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
                         const void* x, const float* weight, const float* bias, const void* state, int silu, void* y, void* new_state,
                         const int64_t* strides_host, ppk_stream_t stream)
 {
-    int rc = conv_check("causal_conv_fwd", dtype, T, B, D, K, x, weight, strides_host);
+    int rc = conv_check("causal_conv_fwd", dtype, T, B, D, K, x, weight, strides_host, 4);
     if (rc) return rc;
     if (B == 0) return PPK_OK;
     if (T > 0 && !y) PPK_FAIL(PPK_ERR_NULL, "causal_conv_fwd: null pointer");
     ConvArgs a = {};
     a.q = {step_off, lengths, T, B};
-    a.D = (int)D; a.K = (int)K; a.runs = (int)(conv_items(T, 1));
+    a.D = (int)D; a.K = (int)K;
     a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.y = y; a.last = K > 1 ? new_state : nullptr; a.silu = silu;
     a.xs = {strides_host[0], strides_host[1]}; a.ys = {strides_host[2], strides_host[3]};
-    if (dtype == PPK_F32) conv_run<float>(a, false, conv_items(T, B), (hipStream_t)stream);
-    else conv_run<bf16_t>(a, false, conv_items(T, B), (hipStream_t)stream);
+    if (dtype == PPK_F32) conv_run<float>(a, false, (hipStream_t)stream);
+    else conv_run<bf16_t>(a, false, (hipStream_t)stream);
     PPK_CHECK_LAUNCH("causal_conv_fwd");
     return PPK_OK;
 }
@@ -349,7 +426,7 @@ size_t ppk_causal_conv_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int6
 {
     if (T < 0 || B < 0 || D < 1 || K < 1) return 0;
     const size_t cols = (size_t)(K + 1) * (size_t)D;
-    return ppk_align_up((size_t)MAX_SUM_BLOCKS * cols * 4, 256) + ppk::partial_sum_ws_bytes(MAX_SUM_BLOCKS, (long long)cols) + ppk_align_up(cols * 4, 256);
+    return ppk_align_up((size_t)SUM_BLOCKS * cols * 4, 256) + ppk::partial_sum_ws_bytes(SUM_BLOCKS, (long long)cols) + ppk_align_up(cols * 4, 256);
 }
 
 int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
@@ -357,7 +434,7 @@ int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
                         void* dx, float* dweight, float* dbias, void* dstate, const int64_t* strides_host,
                         void* workspace, size_t ws_bytes, ppk_stream_t stream)
 {
-    int rc = conv_check("causal_conv_bwd", dtype, T, B, D, K, x, weight, strides_host);
+    int rc = conv_check("causal_conv_bwd", dtype, T, B, D, K, x, weight, strides_host, 6);
     if (rc) return rc;
     if (!dweight || !workspace || (B > 0 && T > 0 && (!dy || !dx))) PPK_FAIL(PPK_ERR_NULL, "causal_conv_bwd: null pointer");
     if (ws_bytes < ppk_causal_conv_bwd_workspace_bytes(T, B, D, K)) PPK_FAIL(PPK_ERR_WS, "causal_conv_bwd: workspace of %zu bytes", ws_bytes);
@@ -365,16 +442,16 @@ int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
     const long long cols = (K + 1) * D;
     char* cur = (char*)workspace;
     ConvArgs a = {};
-    a.part = (float*)ppk_carve(cur, (size_t)MAX_SUM_BLOCKS * (size_t)cols * 4);
-    void* sum_ws = ppk_carve(cur, ppk::partial_sum_ws_bytes(MAX_SUM_BLOCKS, cols));
+    a.part = (float*)ppk_carve(cur, (size_t)SUM_BLOCKS * (size_t)cols * 4);
+    void* sum_ws = ppk_carve(cur, ppk::partial_sum_ws_bytes(SUM_BLOCKS, cols));
     float* sums = (float*)cur;
     a.q = {step_off, lengths, T, B};
-    a.D = (int)D; a.K = (int)K; a.runs = (int)(conv_items(T, 1));
+    a.D = (int)D; a.K = (int)K;
     a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.dy = dy; a.silu = silu; a.dx = dx;
     a.dlast = K > 1 ? dnew_state : nullptr; a.dstate = K > 1 ? dstate : nullptr;
     a.xs = {strides_host[0], strides_host[1]}; a.dys = {strides_host[2], strides_host[3]}; a.ys = {strides_host[4], strides_host[5]};
     int blocks = 0;
-    if (B > 0) blocks = dtype == PPK_F32 ? conv_run<float>(a, true, conv_items(T, B), st) : conv_run<bf16_t>(a, true, conv_items(T, B), st);
+    if (B > 0) blocks = dtype == PPK_F32 ? conv_run<float>(a, true, st) : conv_run<bf16_t>(a, true, st);
     rc = ppk::partial_sum(a.part, blocks, cols, sums, sum_ws, st);
     if (rc) return rc;
     k_conv_unpack<<<(unsigned)((cols + 255) / 256), 256, 0, st>>>(sums, (int)D, (int)K, dweight, dbias);

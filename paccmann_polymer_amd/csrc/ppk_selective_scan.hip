@@ -12,6 +12,9 @@ namespace {
 using ppk::SeqBatch;
 using ppk::Stride;
 using ppk::at;
+using ppk::Rows;
+using ppk::uni_len;
+using ppk::uniform;
 
 constexpr int TILE = 16;                     // steps between two kept states
 constexpr long long MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 1024;
@@ -48,22 +51,6 @@ __device__ __forceinline__ float softplus(float x)
 }
 __device__ __forceinline__ float lane_value(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 
-// memory that the kernel does not write, at an address that all lanes share: loaded into scalar registers
-#define UNIFORM __attribute__((address_space(4)))
-template <typename T> __device__ __forceinline__ const UNIFORM T* uniform(const void* p) { return (const UNIFORM T*)(uintptr_t)p; }
-__device__ __forceinline__ unsigned uni_row(const SeqBatch& q, long long t) { return q.off ? (unsigned)uniform<long long>(q.off)[t] : (unsigned)t; }
-// Addresses: a base and a step's offset that all lanes share, in scalar registers, and a lane's own 32-bit offset in bytes.  A batch has
-// fewer than 2^31 steps and rows, and a row's stride is below 2^32 bytes (the host sees to it): their product is two 32-bit ones.
-template <typename T> struct Rows {
-    const char* base;
-    unsigned stride;
-    __device__ __forceinline__ Rows(const void* p, long long offset, long long stride_)
-        : base((const char*)p + offset * (long long)sizeof(T)), stride((unsigned)(stride_ * (long long)sizeof(T))) {}
-    __device__ __forceinline__ const char* row(unsigned r) const { return base + (unsigned long long)r * stride; }
-    __device__ __forceinline__ T get(unsigned r, unsigned byte) const { return *(const T*)(row(r) + byte); }
-    __device__ __forceinline__ void put(unsigned r, unsigned byte, T v) const { *(T*)(const_cast<char*>(row(r)) + byte) = v; }
-};
-__device__ __forceinline__ long long uni_len(const SeqBatch& q, long long b) { return q.len ? uniform<long long>(q.len)[b] : q.T; }
 __device__ __forceinline__ long long first_tile(const ScanArgs& a, long long b) { return a.tiles ? uniform<long long>(a.tiles)[b] : b * ((a.q.T + TILE - 1) / TILE); }
 
 // N consecutive elements at a uniform address, 4-byte aligned, as scalars
