@@ -34,16 +34,55 @@ __global__ __launch_bounds__(256) void k_ps_final(const double* __restrict__ par
     for (int p = 0; p < n; ++p) s += part[p * C + c];
     out[c] = (float)s;
 }
+struct SumJobs { SumJob job[3]; int n; };
+// up to ONE_PASS_ROWS rows: 64 columns a block, 16 interleaved slices of the rows, joined in order.  One launch for all of a call's sums.
+__global__ __launch_bounds__(1024) void k_ps_one(SumJobs jobs)
+{
+    __shared__ double red[16][64];
+    const SumJob j = jobs.job[blockIdx.y];
+    const long long c0 = (long long)blockIdx.x * 64;
+    if (c0 >= j.C) return;
+    const int col = threadIdx.x & 63, slice = threadIdx.x >> 6;
+    const long long c = c0 + col;
+    double s = 0;
+    if (c < j.C) {
+        long long p = slice;
+        for (; p + 7 * 16 < j.P; p += 8 * 16) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = j.part[(p + k * 16) * j.C + c];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += (double)v[k];
+        }
+        for (; p < j.P; p += 16) s += (double)j.part[p * j.C + c];
+    }
+    red[slice][col] = s;
+    __syncthreads();
+    if (slice || c >= j.C) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += red[k][col];
+    if (!j.taps) { j.out[c] = (float)s; return; }
+    const long long d = j.C / (j.taps + 1), k = c / d;        // rows of [taps + 1, D]: a weight's gradient [D, taps], then the bias'
+    if (k < j.taps) j.out[(c - k * d) * j.taps + k] = (float)s;
+    else if (j.out2) j.out2[c - k * d] = (float)s;
+}
 }  // namespace
 
-size_t partial_sum_ws_bytes(long long P, long long C) { return ppk_align_up((size_t)((P + PS_ROWS - 1) / PS_ROWS) * (size_t)C * 8, 256); }
-int partial_sum(const float* part, long long P, long long C, float* out, void* ws, hipStream_t stream)
+size_t partial_sum_ws_bytes(long long P, long long C) { return P > ONE_PASS_ROWS ? ppk_align_up((size_t)((P + PS_ROWS - 1) / PS_ROWS) * (size_t)C * 8, 256) : 0; }
+int partial_sums(const SumJob* jobs, int count, void* ws, hipStream_t stream)
 {
-    if (C <= 0) return PPK_OK;
-    const unsigned cb = (unsigned)((C + 255) / 256), chunks = (unsigned)((P + PS_ROWS - 1) / PS_ROWS);
-    if (chunks) k_ps_part<<<dim3(cb, chunks), 256, 0, stream>>>(part, P, C, (double*)ws);
-    k_ps_final<<<cb, 256, 0, stream>>>((const double*)ws, (int)chunks, C, out);
-    PPK_CHECK_LAUNCH("partial_sum");
+    SumJobs small = {};
+    long long widest = 0;
+    for (int k = 0; k < count; ++k) {
+        const SumJob& j = jobs[k];
+        if (j.C <= 0 || !j.out) continue;
+        if (j.P <= ONE_PASS_ROWS) { small.job[small.n++] = j; widest = j.C > widest ? j.C : widest; continue; }
+        const unsigned cb = (unsigned)((j.C + 255) / 256), chunks = (unsigned)((j.P + PS_ROWS - 1) / PS_ROWS);
+        k_ps_part<<<dim3(cb, chunks), 256, 0, stream>>>(j.part, j.P, j.C, (double*)ws);
+        k_ps_final<<<cb, 256, 0, stream>>>((const double*)ws, (int)chunks, j.C, j.out);
+    }
+    if (small.n) k_ps_one<<<dim3((unsigned)((widest + 63) / 64), (unsigned)small.n), 1024, 0, stream>>>(small);
+    PPK_CHECK_LAUNCH("partial_sums");
     return PPK_OK;
 }
 
@@ -59,6 +98,7 @@ using ppk::uni_len;
 using ppk::uniform;
 
 constexpr int AHEAD = 4;                      // steps whose elements are loaded before those of the steps before them are used
+static_assert(1024 <= ppk::ONE_PASS_ROWS, "one launch adds them");
 constexpr int SUM_BLOCKS = 1024;              // blocks of a backward launch in all: each leaves a row of partial sums for its channels
 constexpr long long WANTED_WAVES = 8192;
 
@@ -292,16 +332,6 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks
     }
 }
 
-// [K + 1, D] -> dweight [D, K], dbias [D]
-__global__ __launch_bounds__(256) void k_conv_unpack(const float* __restrict__ sums, int D, int K, float* __restrict__ dw, float* __restrict__ db)
-{
-    const int e = blockIdx.x * 256 + threadIdx.x;
-    if (e >= D * (K + 1)) return;
-    const int k = e / D, d = e % D;
-    if (k < K) dw[(long long)d * K + k] = sums[e];
-    else if (db) db[d] = sums[e];
-}
-
 template <typename T, int KP>
 __global__ __launch_bounds__(256) void k_conv_step(long long B, int D, int K, const T* __restrict__ x, long long ldx, const T* state,
                                                    const float* __restrict__ weight, const float* __restrict__ bias, int silu, T* __restrict__ y, T* next)
@@ -426,7 +456,7 @@ size_t ppk_causal_conv_bwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int6
 {
     if (T < 0 || B < 0 || D < 1 || K < 1) return 0;
     const size_t cols = (size_t)(K + 1) * (size_t)D;
-    return ppk_align_up((size_t)SUM_BLOCKS * cols * 4, 256) + ppk::partial_sum_ws_bytes(SUM_BLOCKS, (long long)cols) + ppk_align_up(cols * 4, 256);
+    return ppk_align_up((size_t)SUM_BLOCKS * cols * 4, 256);
 }
 
 int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, const int64_t* step_off, const int64_t* lengths,
@@ -440,11 +470,8 @@ int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
     if (ws_bytes < ppk_causal_conv_bwd_workspace_bytes(T, B, D, K)) PPK_FAIL(PPK_ERR_WS, "causal_conv_bwd: workspace of %zu bytes", ws_bytes);
     hipStream_t st = (hipStream_t)stream;
     const long long cols = (K + 1) * D;
-    char* cur = (char*)workspace;
     ConvArgs a = {};
-    a.part = (float*)ppk_carve(cur, (size_t)SUM_BLOCKS * (size_t)cols * 4);
-    void* sum_ws = ppk_carve(cur, ppk::partial_sum_ws_bytes(SUM_BLOCKS, cols));
-    float* sums = (float*)cur;
+    a.part = (float*)workspace;
     a.q = {step_off, lengths, T, B};
     a.D = (int)D; a.K = (int)K;
     a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.dy = dy; a.silu = silu; a.dx = dx;
@@ -452,9 +479,9 @@ int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
     a.xs = {strides_host[0], strides_host[1]}; a.dys = {strides_host[2], strides_host[3]}; a.ys = {strides_host[4], strides_host[5]};
     int blocks = 0;
     if (B > 0) blocks = dtype == PPK_F32 ? conv_run<float>(a, true, st) : conv_run<bf16_t>(a, true, st);
-    rc = ppk::partial_sum(a.part, blocks, cols, sums, sum_ws, st);
+    const ppk::SumJob job = {a.part, blocks, cols, dweight, (int)K, dbias};
+    rc = ppk::partial_sums(&job, 1, nullptr, st);
     if (rc) return rc;
-    k_conv_unpack<<<(unsigned)((cols + 255) / 256), 256, 0, st>>>(sums, (int)D, (int)K, dweight, dbias);
     PPK_CHECK_LAUNCH("causal_conv_bwd");
     return PPK_OK;
 }

@@ -538,8 +538,10 @@ __global__ __launch_bounds__(256) void k_scan_bc(const float* __restrict__ p, in
     (k < N ? dB : dC)[rg * N + (k < N ? k : k - N)] = from_f32<T>(s);
 }
 
-// One token of each sequence: lane = channel * LPC + slice as in the backward pass, four states a thread
-template <typename T, int LPC>
+// One token of each sequence: lane = channel * LPC + slice, four states a thread.  WIDE: they begin on 16 bytes, and those of B and C
+// on four elements, everywhere: a wave then reads and writes a kilobyte of states at a time.
+template <typename T> struct alignas(4 * sizeof(T)) Quad { T v[4]; };
+template <typename T, int LPC, bool WIDE>
 __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* state, float* next)
 {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -547,22 +549,43 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
     const long long bd = e / LPC;
     if (bd >= a.q.B * a.D) return;                                             // whole groups of LPC lanes
     const long long b = bd / a.D;
-    const int d = (int)(bd % a.D), g = d / a.per;
+    const int d = (int)(bd - b * a.D), g = d / a.per;
+    float A[4], h[4], Bv[4], Cv[4];
+    const T *Bp = (const T*)a.Bm + b * a.Bs.b + g * a.Bg + ns * 4, *Cp = (const T*)a.Cm + b * a.Cs.b + g * a.Cg + ns * 4;
+    const long long at_A = (long long)d * N + ns * 4, at_h = bd * N + ns * 4;
+    if (WIDE) {
+        const float4 u = *reinterpret_cast<const float4*>(state + at_h), v = *reinterpret_cast<const float4*>(a.A + at_A);
+        const Quad<T> p = *reinterpret_cast<const Quad<T>*>(Bp), q = *reinterpret_cast<const Quad<T>*>(Cp);
+        h[0] = u.x; h[1] = u.y; h[2] = u.z; h[3] = u.w;
+        A[0] = v.x; A[1] = v.y; A[2] = v.z; A[3] = v.w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { Bv[j] = to_f32(p.v[j]); Cv[j] = to_f32(q.v[j]); }
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = ns * 4 + j < N;
+            h[j] = in ? state[at_h + j] : 0.f;
+            A[j] = in ? a.A[at_A + j] : 0.f;
+            Bv[j] = in ? to_f32(Bp[j]) : 0.f;
+            Cv[j] = in ? to_f32(Cp[j]) : 0.f;
+        }
     const float x = to_f32(((const T*)a.x)[b * a.xs.b + d]);
     const float raw = to_f32(((const T*)a.raw)[b * a.raws.b + d]) + (a.bias ? a.bias[d] : 0.f);
+    const float z = a.z ? to_f32(((const T*)a.z)[b * a.zs.b + d]) : 0.f, skip = a.skip ? a.skip[d] : 0.f;
     const float dt = a.softplus ? softplus(raw) : raw, dx = dt * x;
     float y = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int n = ns * 4 + j;
-        if (n >= N) continue;
-        const float Bv = to_f32(((const T*)a.Bm)[b * a.Bs.b + g * a.Bg + n]), Cv = to_f32(((const T*)a.Cm)[b * a.Cs.b + g * a.Cg + n]);
-        const float h = fmaf(exp2_(dt * (a.A[(long long)d * N + n] * LOG2E)), state[bd * N + n], dx * Bv);
-        next[bd * N + n] = h;
-        y = fmaf(h, Cv, y);
+        h[j] = fmaf(exp2_(dt * (A[j] * LOG2E)), h[j], dx * Bv[j]);
+        y = fmaf(h[j], Cv[j], y);
     }
-    y = sum_low<LPC>(y) + (a.skip ? a.skip[d] * x : 0.f);
-    if (a.z) { const float z = to_f32(((const T*)a.z)[b * a.zs.b + d]); y *= z * sigmoid(z); }
+    if (WIDE) *reinterpret_cast<float4*>(next + at_h) = make_float4(h[0], h[1], h[2], h[3]);
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ns * 4 + j < N) next[at_h + j] = h[j];
+    y = sum_low<LPC>(y) + skip * x;
+    if (a.z) y *= z * sigmoid(z);
     if (ns == 0) ((T*)a.y)[bd] = from_f32<T>(y);
 }
 
@@ -634,14 +657,21 @@ template <typename T> void run_bwd(const ScanArgs& a, unsigned blocks, hipStream
         default: k_scan_bwd<T, 16><<<blocks, 256, 0, st>>>(a);
     }
 }
+template <typename T, int LPC> void launch_step(const ScanArgs& a, unsigned blocks, const float* state, float* next, hipStream_t st)
+{
+    const uintptr_t p = (uintptr_t)state | (uintptr_t)next | (uintptr_t)a.A, q = (uintptr_t)a.Bm | (uintptr_t)a.Cm;
+    const long long s = a.Bs.b | a.Bg | a.Cs.b | a.Cg;
+    if (a.N == 4 * LPC && p % 16 == 0 && q % (4 * sizeof(T)) == 0 && s % 4 == 0) k_scan_step<T, LPC, true><<<blocks, 256, 0, st>>>(a, state, next);
+    else k_scan_step<T, LPC, false><<<blocks, 256, 0, st>>>(a, state, next);
+}
 template <typename T> void run_step(const ScanArgs& a, unsigned blocks, const float* state, float* next, hipStream_t st)
 {
     switch (slices(a.N)) {
-        case 1: k_scan_step<T, 1><<<blocks, 256, 0, st>>>(a, state, next); break;
-        case 2: k_scan_step<T, 2><<<blocks, 256, 0, st>>>(a, state, next); break;
-        case 4: k_scan_step<T, 4><<<blocks, 256, 0, st>>>(a, state, next); break;
-        case 8: k_scan_step<T, 8><<<blocks, 256, 0, st>>>(a, state, next); break;
-        default: k_scan_step<T, 16><<<blocks, 256, 0, st>>>(a, state, next);
+        case 1: launch_step<T, 1>(a, blocks, state, next, st); break;
+        case 2: launch_step<T, 2>(a, blocks, state, next, st); break;
+        case 4: launch_step<T, 4>(a, blocks, state, next, st); break;
+        case 8: launch_step<T, 8>(a, blocks, state, next, st); break;
+        default: launch_step<T, 16>(a, blocks, state, next, st);
     }
 }
 
@@ -797,9 +827,8 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
         if (dtype == PPK_F32) k_scan_bc<float><<<nb, 256, 0, st>>>(a.pBC, a.blocks_per_group, rows, (int)G, (int)N, (float*)dB, (float*)dC);
         else k_scan_bc<bf16_t><<<nb, 256, 0, st>>>(a.pBC, a.blocks_per_group, rows, (int)G, (int)N, (bf16_t*)dB, (bf16_t*)dC);
     }
-    rc = ppk::partial_sum(a.pA, items, D * N, dA, sum_ws, st);
-    if (!rc && dskip) rc = ppk::partial_sum(a.pD, items, D, dskip, sum_ws, st);
-    if (!rc && dbias) rc = ppk::partial_sum(a.pD + items * D, items, D, dbias, sum_ws, st);
+    const ppk::SumJob jobs[3] = {{a.pA, items, D * N, dA, 0, nullptr}, {a.pD, items, D, dskip, 0, nullptr}, {a.pD + items * D, items, D, dbias, 0, nullptr}};
+    rc = ppk::partial_sums(jobs, 3, sum_ws, st);
     if (rc) return rc;
     PPK_CHECK_LAUNCH("selective_scan_bwd");
     return PPK_OK;

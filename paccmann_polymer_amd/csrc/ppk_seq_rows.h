@@ -36,9 +36,12 @@ template <typename T> struct Rows {
 };
 __device__ __forceinline__ long long uni_len(const SeqBatch& q, long long b) { return q.len ? uniform<long long>(q.len)[b] : q.T; }
 
-// out[c] = sum over p of part[p * C + c], p ascending, in fp64: the partial sums of blocks that ran in any order, added in one
-constexpr int PS_ROWS = 64;                   // rows of a first-pass sum
+// out[c] = sum over p of part[p * C + c], in an order that the sizes alone set and in fp64: the partial sums of blocks that ran in any order.
+// taps != 0: the columns are [taps + 1, D], out a weight's gradient [D, taps] and out2 (or null) a bias' [D].
+struct SumJob { const float* part; long long P, C; float* out; int taps; float* out2; };
+constexpr int PS_ROWS = 64;                   // rows of a first-pass sum ...
+constexpr long long ONE_PASS_ROWS = 4096;     // ... where there are more than this; jobs with taps have at most so many
 size_t partial_sum_ws_bytes(long long P, long long C);
-int partial_sum(const float* part, long long P, long long C, float* out, void* ws, hipStream_t stream);
+int partial_sums(const SumJob* jobs, int count, void* ws, hipStream_t stream);      // at most three jobs
 
 }  // namespace ppk
