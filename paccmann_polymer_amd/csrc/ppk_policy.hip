@@ -12,7 +12,8 @@
 namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int COUNT_BLOCK = 4096;                // targets per partial count
+constexpr int COUNT_BLOCK = 1024;                // targets per partial count
+constexpr long long COUNT_INLINE = 2048;         // up to so many rows, every block counts them itself: cheaper than a launch of their own
 constexpr int MAX_BLOCKS = 4096;                 // row blocks of a launch, and rows of its partial sums
 
 // What a row of logits meets.  `old` etc. are read only in the policy modes.
@@ -47,10 +48,13 @@ __global__ __launch_bounds__(256) void k_count_rows(const int64_t* __restrict__ 
 }
 
 // the number of rows that count, the same in every thread of a block; `red` is LDS of one int per wave
-__device__ __forceinline__ int total_count(const int* counts, int n, int* red)
+__device__ __forceinline__ int total_count(const RowArgs& a, int* red)
 {
     int c = 0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) c += counts[i];
+    if (a.counts)
+        for (int i = threadIdx.x; i < a.ncounts; i += blockDim.x) c += a.counts[i];
+    else
+        for (int i = threadIdx.x; i < (int)a.rows; i += blockDim.x) c += a.targets[i] != a.ignore;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
@@ -62,8 +66,7 @@ __device__ __forceinline__ int total_count(const int* counts, int n, int* red)
 
 template <int TG> __device__ __forceinline__ float group_max(float v, float* red)
 {
-#pragma unroll
-    for (int o = (TG < 64 ? TG : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    v = lanes_max<(TG < 64 ? TG : 64)>(v);
     if (TG > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -76,8 +79,7 @@ template <int TG> __device__ __forceinline__ float group_max(float v, float* red
 }
 template <int TG> __device__ __forceinline__ float group_sum(float v, float* red)
 {
-#pragma unroll
-    for (int o = (TG < 64 ? TG : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    v = lanes_sum<(TG < 64 ? TG : 64)>(v);
     if (TG > 64) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
@@ -89,27 +91,61 @@ template <int TG> __device__ __forceinline__ float group_sum(float v, float* red
     return v;
 }
 
-// The terms of one row in fp64: e^d - d - 1 of a small d and the border of the clip both need more than 24 bits, and a row
-// costs one lane a few hundred cycles beside V exponentials.  Returns dloss / dlp of the row (before the division by n).
-__device__ __forceinline__ double policy_terms(const RowArgs& a, long long row, double lp, double& pg, double& kl, double& clipped)
+// log s of a sum s >= 1 in fp64: s = 2^k f with f in [1/sqrt 2, sqrt 2), log f = 2 atanh r = 2 (r + r^3/3 + ...), r = (f - 1) / (f + 1), where
+// |r| < 0.172 and seven terms leave 2e-12.  An fp32 logarithm would round at the size of log s, and d = ref - lp has to be exact
+// at its own: the KL term of a row is about d^2 / 2.
+__device__ __forceinline__ double log_sum(float s)
 {
-    double em[2];                                  // expm1 of lp - old and of ref - lp: exp(u) = expm1(u) + 1 to an absolute 2^-53
-    const double u[2] = {lp - (double)a.old[row], a.ref ? (double)a.ref[row] - lp : 0.0};
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) em[k] = expm1(u[k]);
-    const double adv = a.adv[row], ratio = em[0] + 1.0;
-    const double held_r = ratio < (double)a.low ? (double)a.low : (ratio > (double)a.high ? (double)a.high : ratio);
-    const double free_ = ratio * adv, held = held_r * adv;
+    int k = __builtin_amdgcn_frexp_expf(s);
+    float f = __builtin_amdgcn_frexp_mantf(s);                    // [0.5, 1)
+    if (f < 0.70710678f) { f += f; --k; }
+    const double n = (double)f - 1.0, q = (double)f + 1.0;
+    double r = (double)__builtin_amdgcn_rcpf((float)q);
+    r = fma(r, fma(-q, r, 1.0), r);                               // Newton: 2^-46 from the reciprocal's 2^-23
+    r *= n;
+    const double r2 = r * r;
+    double p = fma(r2, 1.0 / 13, 1.0 / 11);
+    p = fma(r2, p, 1.0 / 9);
+    p = fma(r2, p, 1.0 / 7);
+    p = fma(r2, p, 1.0 / 5);
+    p = fma(r2, p, 1.0 / 3);
+    p = fma(r2, p, 1.0);
+    return s != s || s == INFINITY ? (double)s : fma((double)k, 0.69314718055994530942, 2.0 * r * p);
+}
+
+// e^d - d - 1: its series where the sum would cancel (|d| < 1/4: nine terms, the first left out 1e-10 of the whole), itself elsewhere
+__device__ __forceinline__ float kl_of(float d)
+{
+    float p = fmaf(d, 1.0f / 362880, 1.0f / 40320);
+    p = fmaf(d, p, 1.0f / 5040);
+    p = fmaf(d, p, 1.0f / 720);
+    p = fmaf(d, p, 1.0f / 120);
+    p = fmaf(d, p, 1.0f / 24);
+    p = fmaf(d, p, 1.0f / 6);
+    p = fmaf(d, p, 0.5f);
+    return fabsf(d) < 0.25f ? d * d * p : expf(d) - d - 1.0f;
+}
+
+// The terms of one row.  lp is fp64 (above); the differences that it enters are rounded once.  Returns dloss / dlp (before the division by n).
+__device__ __forceinline__ float policy_terms(const RowArgs& a, float old, float adv, float ref, double lp, float& pg, float& kl, float& clipped)
+{
+    const float ratio = expf((float)(lp - (double)old));
+    const float held_r = ratio < a.low ? a.low : (ratio > a.high ? a.high : ratio);
+    const float free_ = ratio * adv, held = held_r * adv;
     pg = -(free_ <= held ? free_ : (free_ != free_ ? free_ : held));
-    clipped = held < free_ ? 1.0 : 0.0;
-    double g = free_ <= held ? -free_ : 0.0;
-    kl = 0.0;
+    clipped = held < free_ ? 1.0f : 0.0f;
+    float g = free_ <= held ? -free_ : 0.0f;
+    kl = 0.0f;
     if (a.ref) {
-        kl = em[1] - u[1];
-        g -= (double)a.beta * em[1];
+        const float d = (float)((double)ref - lp);
+        kl = kl_of(d);
+        g = fmaf(-a.beta, kl + d, g);                             // 1 - e^d = -(kl + d)
     }
     return g;
 }
+
+// Keeps what a chunk holds as it is: without it the compiler keeps the bf16 elements that one pass unpacked for the next, twice the registers
+__device__ __forceinline__ void hold(uint4& c) { asm volatile("" : "+v"(c.x), "+v"(c.y), "+v"(c.z), "+v"(c.w)); }
 
 // One group of TG threads a row (TG <= 64: 256 / TG rows a workgroup at once; above, one), NV chunks of 16 bytes a thread.
 // NV = 0: the row does not fit in registers and is read again for its gradient.
@@ -121,23 +157,34 @@ __global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
     __shared__ int redc[THREADS / 64];
     __shared__ double acc_s[GROUPS][3];
     const int g = threadIdx.x / TG, l = threadIdx.x % TG;
-    double inv_n = 1.0;
+    float scale = 1.0f;                                                   // 1 / (n temperature)
     if (MODE == MODE_POLICY_GRAD) {
-        const int n = total_count(a.counts, a.ncounts, redc);
-        inv_n = 1.0 / (double)(n > 0 ? n : 1);
+        const int n = total_count(a, redc);
+        scale = (float)((double)a.inv_t / (double)(n > 0 ? n : 1));
     }
     const float k2 = a.inv_t * LOG2E;
     double s_pg = 0, s_kl = 0, s_cl = 0;
-    for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < a.rows; row0 += (long long)gridDim.x * GROUPS) {
+    uint4 raw[NV > 0 ? NV : 1];
+    const auto fetch = [&](long long row) {                               // a row behind the last: nothing
+        const RowChunks<T> rc((const T*)a.logits + (row < a.rows ? row : 0) * a.ld, row < a.rows ? a.V : 0);
+        if (NV > 0)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) raw[i] = rc.load(l + i * TG, -INFINITY);
+    };
+    const long long step = (long long)gridDim.x * GROUPS;
+    for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < a.rows; row0 += step) {
         const long long row = row0 + g;
         const bool live = row < a.rows;                                   // TG <= 64: whole groups idle, no barrier inside
         const T* x = (const T*)a.logits + (live ? row : 0) * a.ld;
         const RowChunks<T> rc(x, live ? a.V : 0);
-        uint4 raw[NV > 0 ? NV : 1];
+        fetch(row);
+        const long long t = live ? a.targets[row] : a.ignore;
+        const bool counts = t != a.ignore, good = t >= 0 && t < a.V;
+        const float taken = counts && good ? to_f32(x[t]) : 0.f;
+        float old = 0.f, adv = 0.f, ref = 0.f;
+        if (MODE != MODE_LOGP && counts) { old = a.old[row]; adv = a.adv[row]; ref = a.ref ? a.ref[row] : 0.f; }
         float m = -INFINITY;
         if (NV > 0) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) raw[i] = rc.load(l + i * TG, -INFINITY);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 float v[E];
@@ -154,6 +201,9 @@ __global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
             }
         }
         m = group_max<TG>(m, red);
+        if (NV > 0 && sizeof(T) == 2)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) hold(raw[i]);
         float s = 0.f;
         if (NV > 0) {
 #pragma unroll
@@ -172,11 +222,12 @@ __global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
             }
         }
         s = group_sum<TG>(s, red);
+        if (NV > 0 && sizeof(T) == 2)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) hold(raw[i]);
         if (!live) continue;                                              // no barrier below; the whole group leaves together
-        const long long t = a.targets[row];
-        const bool counts = t != a.ignore, good = t >= 0 && t < a.V;
         double lp = 0.0;
-        if (counts) lp = good ? ((double)to_f32(x[t]) - (double)m) * (double)a.inv_t - log((double)s) : (double)NAN;   // an id outside the vocabulary: NaN, never a guess
+        if (counts) lp = good ? ((double)taken - (double)m) * (double)a.inv_t - log_sum(s) : (double)NAN;   // an id outside the vocabulary: NaN, never a guess
         if (MODE == MODE_LOGP) {
             if (l == 0) {
                 a.logp[row] = (float)lp;
@@ -184,14 +235,14 @@ __global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
             }
             continue;
         }
-        double gr = 0.0;
+        float gr = 0.f;
         if (counts) {
-            double pg, kl, cl;
-            gr = policy_terms(a, row, lp, pg, kl, cl);
+            float pg, kl, cl;
+            gr = policy_terms(a, old, adv, ref, lp, pg, kl, cl);
             s_pg += pg; s_kl += kl; s_cl += cl;
         }
         if (MODE == MODE_POLICY_GRAD) {
-            const float gt = (float)(gr * inv_n * (double)a.inv_t);
+            const float gt = gr * scale;
             const float gp = -gt / s;
             T* out = (T*)a.grad + row * a.ldg;
             const RowChunks<T> oc(out, a.V);
@@ -230,25 +281,28 @@ __global__ __launch_bounds__(TG > 256 ? TG : 256) void k_rows_lp(RowArgs a)
     }
 }
 
-__global__ __launch_bounds__(256) void k_policy_final(const double* __restrict__ part, int nparts, const int* __restrict__ counts, int ncounts,
-                                                      float beta, float* __restrict__ loss, float* __restrict__ stats)
+__global__ __launch_bounds__(1024) void k_policy_final(RowArgs a, int nparts, float* __restrict__ loss, float* __restrict__ stats)
 {
-    __shared__ int redc[4];
-    __shared__ double red[4][3];
-    const int n = total_count(counts, ncounts, redc);
-    double a[3] = {0, 0, 0};
-    for (int p = threadIdx.x; p < nparts; p += 256)
-        for (int k = 0; k < 3; ++k) a[k] += part[(long long)p * 3 + k];
+    __shared__ int redc[16];
+    __shared__ double red[16][3];
+    const int n = total_count(a, redc);
+    double s[3] = {0, 0, 0};
+    for (int p = threadIdx.x; p < nparts; p += 1024)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) s[k] += a.part[(long long)p * 3 + k];
+#pragma unroll
     for (int k = 0; k < 3; ++k) {
-        a[k] = ppk_wave_sum_d(a[k]);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][k] = a[k];
+        s[k] = ppk_wave_sum_d(s[k]);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][k] = s[k];
     }
     __syncthreads();
     if (threadIdx.x == 0) {
         const double inv = 1.0 / (double)(n > 0 ? n : 1);
-        double t[3];
-        for (int k = 0; k < 3; ++k) t[k] = ((red[0][k] + red[1][k]) + (red[2][k] + red[3][k])) * inv;
-        loss[0] = (float)(t[0] + (double)beta * t[1]);
+        double t[3] = {0, 0, 0};
+        for (int w = 0; w < 16; ++w)
+            for (int k = 0; k < 3; ++k) t[k] += red[w][k];
+        for (int k = 0; k < 3; ++k) t[k] *= inv;
+        loss[0] = (float)(t[0] + (double)a.beta * t[1]);
         for (int k = 0; k < 3; ++k) stats[k] = (float)t[k];
     }
 }
@@ -305,8 +359,8 @@ void launch_rows(const RowArgs& a, int mode, int blocks, hipStream_t st)
     else k_rows_lp<T, TG, NV, MODE_POLICY_GRAD><<<blocks, block, 0, st>>>(a);
 }
 
-// group width of a row of `chunks` 16-byte chunks, and the blocks of a launch over `rows`
-int group_width(long long chunks) { return chunks <= 64 ? 16 : chunks <= 512 ? 64 : chunks <= 2048 ? 256 : 1024; }
+// The threads of a row of `chunks` 16-byte chunks: as few as hold it in 64 registers each (more rows at once hide each other's waits)
+int group_width(long long chunks) { return chunks <= 64 ? 16 : chunks <= 512 ? 64 : chunks <= 4096 ? 256 : chunks <= 8192 ? 512 : 1024; }      // 1024: read again instead
 int row_blocks(long long rows, int tg)
 {
     const int groups = tg >= 256 ? 1 : 256 / tg;
@@ -317,17 +371,15 @@ int row_blocks(long long rows, int tg)
 template <typename T>
 void dispatch_rows(const RowArgs& a, int mode, int blocks, long long chunks, hipStream_t st)
 {
-    if (chunks <= 16) launch_rows<T, 16, 1>(a, mode, blocks, st);
-    else if (chunks <= 64) launch_rows<T, 16, 4>(a, mode, blocks, st);
-    else if (chunks <= 128) launch_rows<T, 64, 2>(a, mode, blocks, st);
-    else if (chunks <= 256) launch_rows<T, 64, 4>(a, mode, blocks, st);
-    else if (chunks <= 512) launch_rows<T, 64, 8>(a, mode, blocks, st);
-    else if (chunks <= 1024) launch_rows<T, 256, 4>(a, mode, blocks, st);
-    else if (chunks <= 2048) launch_rows<T, 256, 8>(a, mode, blocks, st);
-    else if (chunks <= 4096) launch_rows<T, 1024, 4>(a, mode, blocks, st);
-    else if (chunks <= 8192) launch_rows<T, 1024, 8>(a, mode, blocks, st);
-    else if (chunks <= 16384) launch_rows<T, 1024, 16>(a, mode, blocks, st);
-    else launch_rows<T, 1024, 0>(a, mode, blocks, st);
+    const int tg = group_width(chunks);
+    const long long nv = (chunks + tg - 1) / tg;
+#define ROWS(TG, NV) if (tg == TG && nv <= NV) return launch_rows<T, TG, NV>(a, mode, blocks, st)
+    ROWS(16, 1); ROWS(16, 2); ROWS(16, 4);
+    ROWS(64, 2); ROWS(64, 3); ROWS(64, 4); ROWS(64, 6); ROWS(64, 8);
+    ROWS(256, 3); ROWS(256, 4); ROWS(256, 6); ROWS(256, 8); ROWS(256, 12); ROWS(256, 16);
+    ROWS(512, 12); ROWS(512, 16);
+#undef ROWS
+    launch_rows<T, 1024, 0>(a, mode, blocks, st);
 }
 
 int elem_bytes(int dtype) { return dtype == PPK_F32 ? 4 : 2; }
@@ -345,7 +397,7 @@ int check_rows(const char* what, int dtype, long long rows, long long V, const v
 }
 
 struct PolicyWs { int* counts; double* part; };
-int count_blocks(long long rows) { return (int)((rows + COUNT_BLOCK - 1) / COUNT_BLOCK); }
+int count_blocks(long long rows) { return rows <= COUNT_INLINE ? 0 : (int)((rows + COUNT_BLOCK - 1) / COUNT_BLOCK); }
 size_t policy_ws_bytes(long long rows) { return ppk_align_up((size_t)count_blocks(rows) * 4, 256) + ppk_align_up((size_t)MAX_BLOCKS * 24, 256); }
 
 }  // namespace
@@ -413,7 +465,7 @@ int ppk_policy_loss(int dtype, const void* logits, int64_t ldl, const int64_t* t
     a.logits = logits; a.ld = ldl; a.targets = targets; a.rows = rows; a.V = (int)V; a.ignore = ignore_index; a.inv_t = 1.0f / temperature;
     a.old = old_logp; a.adv = advantages; a.ref = ref_logp;
     a.low = 1.0f - clip_low; a.high = 1.0f + clip_high; a.beta = kl_coef;
-    a.counts = counts; a.ncounts = nc; a.grad = dlogits; a.ldg = ldd;
+    a.counts = nc ? counts : nullptr; a.ncounts = nc; a.grad = dlogits; a.ldg = ldd;
     a.part = (double*)cur;
     const long long ch = row_chunks(V, dtype);
     const int blocks = row_blocks(rows, group_width(ch));
@@ -423,7 +475,7 @@ int ppk_policy_loss(int dtype, const void* logits, int64_t ldl, const int64_t* t
         if (dtype == PPK_F32) dispatch_rows<float>(a, mode, blocks, ch, st);
         else dispatch_rows<bf16_t>(a, mode, blocks, ch, st);
     }
-    k_policy_final<<<1, 256, 0, st>>>(a.part, rows > 0 ? blocks : 0, counts, nc, kl_coef, loss, stats);
+    k_policy_final<<<1, 1024, 0, st>>>(a, rows > 0 ? blocks : 0, loss, stats);
     PPK_CHECK_LAUNCH("policy_loss");
     return PPK_OK;
 }

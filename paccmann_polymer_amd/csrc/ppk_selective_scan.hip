@@ -293,29 +293,13 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
     }
 }
 
-// v + v of the lane that `ctrl` names, in one instruction
-template <int CTRL> __device__ __forceinline__ float dpp_add(float v)
-{
-    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140, ROR4 = 0x124, ROR8 = 0x128;
-// sum over the low bits of the lane number, LPC lanes; every one of them holds it.  A mirror reverses lanes that hold the same
-// sum already within each half, which is what an xor of that half's width would reach.
-template <int LPC> __device__ __forceinline__ float sum_low(float v)
-{
-    if (LPC > 1) v = dpp_add<XOR1>(v);
-    if (LPC > 2) v = dpp_add<XOR2>(v);
-    if (LPC > 4) v = dpp_add<HALF_MIRROR>(v);
-    if (LPC > 8) v = dpp_add<MIRROR>(v);
-    return v;
-}
 // sum over the LPC lanes of a row of 16 that share their low bits (of which there are 16 / LPC values)
 template <int LPC> __device__ __forceinline__ float sum_slices(float v)
 {
-    if (LPC > 8) v = dpp_add<XOR1>(v);
-    if (LPC > 4) v = dpp_add<XOR2>(v);
-    v = dpp_add<ROR4>(v);
-    v = dpp_add<ROR8>(v);
+    if (LPC > 8) v += dpp_of<DPP_XOR1>(v);
+    if (LPC > 4) v += dpp_of<DPP_XOR2>(v);
+    v += dpp_of<DPP_ROR4>(v);
+    v += dpp_of<DPP_ROR8>(v);
     return v;
 }
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -478,7 +462,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[k + 2]), false, false);
-                w[k] = sum_low<CL>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+                w[k] = lanes_sum<CL>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
             }
             // CL lanes hold the same two sums and store them to the same place
             *reinterpret_cast<f32x2*>(&s_red[t][wave][(lane >> 5) * NP + ns * 4 + ((lane >> 4) & 1) * 2]) = f32x2{w[0], w[1]};
@@ -584,7 +568,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (ns * 4 + j < N) next[at_h + j] = h[j];
-    y = sum_low<LPC>(y) + skip * x;
+    y = lanes_sum<LPC>(y) + skip * x;
     if (a.z) y *= z * sigmoid(z);
     if (ns == 0) ((T*)a.y)[bd] = from_f32<T>(y);
 }

@@ -2,6 +2,25 @@
 #pragma once
 #include "ppk_common.h"
 
+// v combined with v of the lane that `ctrl` names, in one instruction
+template <int CTRL> __device__ __forceinline__ float dpp_of(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_HALF_MIRROR = 0x141, DPP_MIRROR = 0x140, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
+// Sum and maximum over groups of W neighbouring lanes (W a power of two up to 64), in every one of them, without LDS.  A mirror reverses
+// lanes that agree already within each half, which is what an xor of that half's width would reach; between rows of 16 and between halves
+// of a wave the exchange instructions hand over whole rows.
+template <int W, typename F> __device__ __forceinline__ float lanes_all(float v, F f)
+{
+    if (W > 1) v = f(v, dpp_of<DPP_XOR1>(v));
+    if (W > 2) v = f(v, dpp_of<DPP_XOR2>(v));
+    if (W > 4) v = f(v, dpp_of<DPP_HALF_MIRROR>(v));
+    if (W > 8) v = f(v, dpp_of<DPP_MIRROR>(v));
+    if (W > 16) { const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false); v = f(__uint_as_float(p[0]), __uint_as_float(p[1])); }
+    if (W > 32) { const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false); v = f(__uint_as_float(p[0]), __uint_as_float(p[1])); }
+    return v;
+}
+template <int W> __device__ __forceinline__ float lanes_sum(float v) { return lanes_all<W>(v, [](float a, float b) { return a + b; }); }
+template <int W> __device__ __forceinline__ float lanes_max(float v) { return lanes_all<W>(v, [](float a, float b) { return fmaxf(a, b); }); }
+
 struct bf16_t { unsigned short v; };
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
