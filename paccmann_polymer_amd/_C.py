@@ -5,6 +5,7 @@ import fails loudly when the library has not been built
 (`python -c "import __graft_entry__ as g; g.build()"` or
 `make -C paccmann_polymer_amd/csrc`).
 """
+import contextlib
 import ctypes
 import os
 
@@ -162,6 +163,24 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def addr(t):
+    """device address of a tensor (or None), as the integer that ctypes takes for a pointer."""
+    return None if t is None else t.data_ptr()
+
+
+def stream_on(device):
+    """the current stream of a device, as `stream()` of the current one; a call costs a tenth of making a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Makes a tensor's device the current one, where it is not."""
+    return _HERE_ALREADY if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def dtype_code(t, what):
     """The library's code of a tensor's element type; a type that the kernels do not take is refused."""
     if t.dtype not in DTYPES:
@@ -172,10 +191,15 @@ def dtype_code(t, what):
 def one_device(*tensors):
     """The GPU that all of these tensors (None: left out) are on; anything else is refused."""
     require_gpu(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise PPKError(f'tensors on different devices: {sorted(map(str, devices))}')
-    return devices.pop()
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise PPKError(f'tensors on different devices: {device} and {t.device}')
+    return device
 
 
 def require_gpu(*tensors):

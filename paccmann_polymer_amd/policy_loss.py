@@ -57,10 +57,10 @@ class _TokenLogProbs(torch.autograd.Function):
         dev = _C.one_device(logits, targets)
         x, t = _rows_of(logits), targets.contiguous()
         rows, V = x.shape
-        with torch.cuda.device(dev):
+        with _C.on_device(dev):
             logp = torch.empty(rows, dtype=torch.float32, device=dev)
             saved = torch.empty(rows, 2, dtype=torch.float32, device=dev) if want_grad else None
-            _C.check(_lib.ppk_token_logp_fwd(code, _C.p(x), _ld(x), _C.p(t), rows, V, ignore_index, temperature, _C.p(logp), _C.p(saved), _C.stream()))
+            _C.check(_lib.ppk_token_logp_fwd(code, _C.addr(x), _ld(x), _C.addr(t), rows, V, ignore_index, temperature, _C.addr(logp), _C.addr(saved), _C.stream_on(x.device)))
         if saved is not None:
             ctx.save_for_backward(x, t, saved)
             ctx.args = (code, ignore_index, temperature)
@@ -72,10 +72,10 @@ class _TokenLogProbs(torch.autograd.Function):
         x, t, saved = ctx.saved_tensors
         code, ignore_index, temperature = ctx.args
         rows, V = x.shape
-        with torch.cuda.device(x.device):
+        with _C.on_device(x.device):
             d = torch.empty(rows, V, dtype=x.dtype, device=x.device)
             g = dlogp.to(torch.float32).contiguous()
-            _C.check(_lib.ppk_token_logp_bwd(code, _C.p(x), _ld(x), _C.p(t), rows, V, ignore_index, temperature, _C.p(saved), _C.p(g), _C.p(d), V, _C.stream()))
+            _C.check(_lib.ppk_token_logp_bwd(code, _C.addr(x), _ld(x), _C.addr(t), rows, V, ignore_index, temperature, _C.addr(saved), _C.addr(g), _C.addr(d), V, _C.stream_on(x.device)))
         return d, None, None, None, None
 
 
@@ -91,14 +91,14 @@ def _policy_call(code, x, t, old, adv, ref, args, want_grad):
     rows, V = x.shape
     clip_low, clip_high, kl_coef, ignore_index, temperature = args
     dev = x.device
-    with torch.cuda.device(dev):
+    with _C.on_device(dev):
         out = torch.empty(4, dtype=torch.float32, device=dev)
         loss, stats = out[:1], out[1:]
         d = torch.empty(rows, V, dtype=x.dtype, device=dev) if want_grad else None
         wsb = _lib.ppk_policy_loss_workspace_bytes(rows)
         ws = torch.empty(max(int(wsb), 256), dtype=torch.uint8, device=dev)
-        _C.check(_lib.ppk_policy_loss(code, _C.p(x), _ld(x), _C.p(t), rows, V, ignore_index, temperature, _C.p(old), _C.p(adv), _C.p(ref),
-                                      clip_low, clip_high, kl_coef, _C.p(loss), _C.p(stats), _C.p(d), V, _C.p(ws), wsb, _C.stream()))
+        _C.check(_lib.ppk_policy_loss(code, _C.addr(x), _ld(x), _C.addr(t), rows, V, ignore_index, temperature, _C.addr(old), _C.addr(adv), _C.addr(ref),
+                                      clip_low, clip_high, kl_coef, _C.addr(loss), _C.addr(stats), _C.addr(d), V, _C.addr(ws), wsb, _C.stream_on(x.device)))
     return loss.reshape(()), stats, d
 
 
@@ -120,13 +120,14 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _dstats):
-        x, targets, old, adv, ref = ctx.saved_tensors
         d, ctx.grad = ctx.grad, None                        # it is handed on and may be changed: a second backward pass makes its own
         if d is None:
+            x, targets, old, adv, ref = ctx.saved_tensors
             d = _policy_call(ctx.code, x, targets, old, adv, ref, ctx.args, True)[2]
-        with torch.cuda.device(x.device):
-            s = dloss.to(torch.float32).reshape(1).contiguous()
-            _C.check(_lib.ppk_scale_unless_one(ctx.code, _C.p(d), d.numel(), _C.p(s), _C.stream()))
+        dev = d.device
+        with _C.on_device(dev):
+            s = dloss if dloss.dtype == torch.float32 else dloss.to(torch.float32)
+            _C.check(_lib.ppk_scale_unless_one(ctx.code, _C.addr(d), d.numel(), _C.addr(s), _C.stream_on(dev)))
         return d, None, None, None, None, None, None
 
 

@@ -124,7 +124,7 @@ class _Batch:
 
     def pointers(self):
         p = self.plan
-        return (None, None) if p is None else (_C.p(p.offsets), _C.p(p.lengths))
+        return (None, None) if p is None else (_C.addr(p.offsets), _C.addr(p.lengths))
 
     def tensors(self):
         return () if self.plan is None else (self.plan.offsets, self.plan.lengths, self.plan.tiles)
@@ -162,12 +162,12 @@ class _CausalConv(torch.autograd.Function):
         dev = x.device
         weight, bias, state = weight.contiguous(), _contiguous(bias), _contiguous(state)
         D, K = weight.shape
-        with torch.cuda.device(dev):
+        with _C.on_device(dev):
             y = batch.new((D,), x.dtype, dev)
             last = torch.empty(batch.B, K - 1, D, dtype=x.dtype, device=dev)
             off, lengths = batch.pointers()
-            _C.check(_lib.ppk_causal_conv_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.p(x), _C.p(weight), _C.p(bias), _C.p(state),
-                                              silu, _C.p(y), _C.p(last), _ints(*batch.strides(x), *batch.strides(y)), _C.stream()))
+            _C.check(_lib.ppk_causal_conv_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.addr(x), _C.addr(weight), _C.addr(bias), _C.addr(state),
+                                              silu, _C.addr(y), _C.addr(last), _ints(*batch.strides(x), *batch.strides(y)), _C.stream_on(dev)))
         ctx.save_for_backward(x, weight, bias, state)
         ctx.batch, ctx.silu = batch, silu
         ctx.set_materialize_grads(False)
@@ -179,7 +179,7 @@ class _CausalConv(torch.autograd.Function):
         x, weight, bias, state = ctx.saved_tensors
         batch, dev = ctx.batch, x.device
         D, K = weight.shape
-        with torch.cuda.device(dev):
+        with _C.on_device(dev):
             dy = torch.zeros(*batch.lead, D, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (D,), x.dtype)
             dlast = _contiguous(dlast)
             dx = batch.new((D,), x.dtype, dev)
@@ -189,9 +189,9 @@ class _CausalConv(torch.autograd.Function):
             off, lengths = batch.pointers()
             wsb = _lib.ppk_causal_conv_bwd_workspace_bytes(batch.T, batch.B, D, K)
             ws = _ws(wsb, dev)
-            _C.check(_lib.ppk_causal_conv_bwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.p(x), _C.p(weight), _C.p(bias), _C.p(state), ctx.silu,
-                                              _C.p(dy), _C.p(dlast), _C.p(dx), _C.p(dw), _C.p(db), _C.p(ds),
-                                              _ints(*batch.strides(x), *batch.strides(dy), *batch.strides(dx)), _C.p(ws), wsb, _C.stream()))
+            _C.check(_lib.ppk_causal_conv_bwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.addr(x), _C.addr(weight), _C.addr(bias), _C.addr(state), ctx.silu,
+                                              _C.addr(dy), _C.addr(dlast), _C.addr(dx), _C.addr(dw), _C.addr(db), _C.addr(ds),
+                                              _ints(*batch.strides(x), *batch.strides(dy), *batch.strides(dx)), _C.addr(ws), wsb, _C.stream_on(dev)))
         return None, None, dx, dw, db, ds
 
 
@@ -274,14 +274,14 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
     if state.dtype != x.dtype:
         raise TypeError(f'{what}: state must be {x.dtype}, as x is')
     dev = _C.one_device(x, state, weight, bias)
-    with torch.no_grad(), torch.cuda.device(dev):
+    with _C.on_device(dev):
         x = x.detach()
         x = x if x.stride(1) == 1 or D == 1 else x.contiguous()
         weight, bias = weight.contiguous(), _contiguous(bias)
         new = _step_out(what, state, out, (x, weight, bias))
         state = state.contiguous()
         y = torch.empty(B, D, dtype=x.dtype, device=dev)
-        _C.check(_lib.ppk_causal_conv_step(code, B, D, K, _C.p(x), x.stride(0), _C.p(state), _C.p(weight), _C.p(bias), silu, _C.p(y), _C.p(new), _C.stream()))
+        _C.check(_lib.ppk_causal_conv_step(code, B, D, K, _C.addr(x), x.stride(0), _C.addr(state), _C.addr(weight), _C.addr(bias), silu, _C.addr(y), _C.addr(new), _C.stream_on(dev)))
     return y, new
 
 
@@ -300,7 +300,7 @@ class _SelectiveScan(torch.autograd.Function):
         A, D, dt_bias, state = A.contiguous(), _contiguous(D), _contiguous(dt_bias), _contiguous(state)
         N, G, width = A.shape[1], B.shape[-2], batch.D
         tiles = None if batch.plan is None else batch.plan.tiles
-        with torch.cuda.device(dev):
+        with _C.on_device(dev):
             y = batch.new((width,), x.dtype, dev)
             last = torch.empty(batch.B, width, N, dtype=torch.float32, device=dev)
             kept = None
@@ -311,9 +311,9 @@ class _SelectiveScan(torch.autograd.Function):
             off, lengths = batch.pointers()
             wsb = _lib.ppk_selective_scan_fwd_workspace_bytes(batch.T, batch.B, width, N, G)
             ws = _ws(wsb, dev) if wsb else None
-            _C.check(_lib.ppk_selective_scan_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, off, lengths, _C.p(tiles), _C.p(x), _C.p(dt), _C.p(A),
-                                                 _C.p(B), _C.p(C), _C.p(D), _C.p(z), _C.p(dt_bias), _C.p(state), softplus, _C.p(y), _C.p(last), _C.p(kept),
-                                                 _scan_strides(batch, x, dt, B, C, z, batch.out_rows, None), _C.p(ws), wsb, _C.stream()))
+            _C.check(_lib.ppk_selective_scan_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, off, lengths, _C.addr(tiles), _C.addr(x), _C.addr(dt), _C.addr(A),
+                                                 _C.addr(B), _C.addr(C), _C.addr(D), _C.addr(z), _C.addr(dt_bias), _C.addr(state), softplus, _C.addr(y), _C.addr(last), _C.addr(kept),
+                                                 _scan_strides(batch, x, dt, B, C, z, batch.out_rows, None), _C.addr(ws), wsb, _C.stream_on(dev)))
         if kept is not None:
             ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, kept)
             ctx.batch, ctx.softplus, ctx.has_state = batch, softplus, state is not None
@@ -327,7 +327,7 @@ class _SelectiveScan(torch.autograd.Function):
         batch, dev = ctx.batch, x.device
         N, G, width = A.shape[1], B.shape[-2], batch.D
         tiles = None if batch.plan is None else batch.plan.tiles
-        with torch.cuda.device(dev):
+        with _C.on_device(dev):
             dy = torch.zeros(*batch.lead, width, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (width,), x.dtype)
             dlast = _contiguous(dlast)
             dx, draw = batch.new((width,), x.dtype, dev), batch.new((width,), x.dtype, dev)
@@ -341,9 +341,9 @@ class _SelectiveScan(torch.autograd.Function):
             wsb = _lib.ppk_selective_scan_bwd_workspace_bytes(batch.T, batch.B, width, N, G, batch.rows)
             ws = _ws(wsb, dev)
             _C.check(_lib.ppk_selective_scan_bwd(
-                _C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, batch.rows, off, lengths, _C.p(tiles), _C.p(x), _C.p(dt), _C.p(A), _C.p(B), _C.p(C),
-                _C.p(D), _C.p(z), _C.p(dt_bias), ctx.softplus, _C.p(kept), _C.p(dy), _C.p(dlast), _C.p(dx), _C.p(draw), _C.p(dA), _C.p(dB), _C.p(dC),
-                _C.p(dD), _C.p(dz), _C.p(dbias), _C.p(dstate), _scan_strides(batch, x, dt, B, C, z, batch.out_rows, dy), _C.p(ws), wsb, _C.stream()))
+                _C.DTYPES[x.dtype], batch.T, batch.B, width, N, G, batch.rows, off, lengths, _C.addr(tiles), _C.addr(x), _C.addr(dt), _C.addr(A), _C.addr(B), _C.addr(C),
+                _C.addr(D), _C.addr(z), _C.addr(dt_bias), ctx.softplus, _C.addr(kept), _C.addr(dy), _C.addr(dlast), _C.addr(dx), _C.addr(draw), _C.addr(dA), _C.addr(dB), _C.addr(dC),
+                _C.addr(dD), _C.addr(dz), _C.addr(dbias), _C.addr(dstate), _scan_strides(batch, x, dt, B, C, z, batch.out_rows, dy), _C.addr(ws), wsb, _C.stream_on(dev)))
         return None, None, None, dx, draw, dA, dB, dC, dD, dz, dbias, dstate
 
 
@@ -427,13 +427,13 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
     Bg, Cg = row('B', Bg, Bg.shape[1:]), row('C', Cg, Cg.shape[1:])
     _param(what, 'state', state, (n, width, N))
     dev = _C.one_device(data, raw, A, Bg, Cg, D, gate, dt_bias, state)
-    with torch.no_grad(), torch.cuda.device(dev):
+    with _C.on_device(dev):
         A, D, dt_bias = A.contiguous(), _contiguous(D), _contiguous(dt_bias)
         new = _step_out(what, state, out, (data, raw, A, Bg, Cg, D, gate, dt_bias))
         state = state.contiguous()
         y = torch.empty(n, width, dtype=x.dtype, device=dev)
         pair = lambda t: (0, 0) if t is None else (0, t.stride(0))      # noqa: E731
         strides = _ints(*pair(data), *pair(raw), 0, Bg.stride(0), Bg.stride(1), 0, Cg.stride(0), Cg.stride(1), *pair(gate), 0, 1, 0, 0)
-        _C.check(_lib.ppk_selective_scan_step(code, n, width, N, Bg.shape[1], _C.p(data), _C.p(raw), _C.p(A), _C.p(Bg), _C.p(Cg), _C.p(D), _C.p(gate),
-                                              _C.p(dt_bias), _C.p(state), int(bool(dt_softplus)), _C.p(y), _C.p(new), strides, _C.stream()))
+        _C.check(_lib.ppk_selective_scan_step(code, n, width, N, Bg.shape[1], _C.addr(data), _C.addr(raw), _C.addr(A), _C.addr(Bg), _C.addr(Cg), _C.addr(D), _C.addr(gate),
+                                              _C.addr(dt_bias), _C.addr(state), int(bool(dt_softplus)), _C.addr(y), _C.addr(new), strides, _C.stream_on(dev)))
     return y, new
