@@ -31,6 +31,7 @@ from torch.nn.utils.rnn import PackedSequence
 
 from . import _C
 from .data_prep import known_token_range, note_token_range
+from .policy_loss import policy_loss, token_log_probs
 
 _lib = _C.lib
 
@@ -592,6 +593,16 @@ def _final_row_index(packed: PackedSequence, device):
     return fin.to(device)
 
 
+def _packed_samples(packed: PackedSequence, device):
+    """ORIGINAL sample of each packed row."""
+    bs = packed.batch_sizes.to(torch.int64)
+    off = torch.cumsum(bs, 0) - bs
+    b = torch.arange(int(bs.sum()), dtype=torch.int64) - torch.repeat_interleave(off, bs)
+    if packed.sorted_indices is not None:
+        b = packed.sorted_indices.cpu()[b]
+    return b.to(device)
+
+
 class StackGRUEncoder(StackGRU):
 
     def __init__(self, params):
@@ -622,8 +633,8 @@ class StackGRUDecoder(StackGRU):
         self.latent_to_hidden = HIPLinear(self.latent_dim, self.rnn_cell_size)
         self.output_layer = HIPLinear(self.rnn_cell_size, self.vocab_size)
 
-    def decoder_train_step(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence):
-        """latent_z [1 or L, B, Z] in ORIGINAL sample order -> mean CE over non-pad targets."""
+    def _teacher_forced_logits(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence):
+        """(logits [NT, V], targets [NT]) in packed order: every step sees the true tokens before it."""
         _require_packed(packed_in)
         _require_packed(packed_tgt)
         dev = self.embedding.weight.device
@@ -645,9 +656,35 @@ class StackGRUDecoder(StackGRU):
         h0 = torch.stack(hs * (L // len(hs)), dim=0)
         htop = self._run_sequence(packed_in, h0)
         logits = linear(htop, self.output_layer.weight, self.output_layer.bias)
-        tgt = packed_tgt.data.reshape(-1).to(device=dev, dtype=torch.int64).contiguous()
+        return logits, packed_tgt.data.reshape(-1).to(device=dev, dtype=torch.int64).contiguous()
+
+    def decoder_train_step(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence):
+        """latent_z [1 or L, B, Z] in ORIGINAL sample order -> mean CE over non-pad targets."""
+        logits, tgt = self._teacher_forced_logits(latent_z, packed_in, packed_tgt)
         return _CrossEntropy.apply(logits, tgt, 0)
 
+    def decoder_log_probs(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence, temperature: float = 1.0):
+        """log softmax(logits / temperature) at every target, [NT] in packed order; 0 at padding targets.  Under `torch.no_grad()`:
+        the old or reference scores that `decoder_policy_step` takes."""
+        logits, tgt = self._teacher_forced_logits(latent_z, packed_in, packed_tgt)
+        return token_log_probs(logits, tgt, ignore_index=0, temperature=temperature)
+
+    def decoder_policy_step(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence, advantages, old_log_probs,
+                            ref_log_probs=None, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0):
+        """Clipped policy loss of generated sequences (`policy_loss.policy_loss`) -> (loss, stats [3]).  advantages: one per
+        sample [B] in ORIGINAL order, or one per token [NT] in packed order; old / ref log-probabilities [NT] as `decoder_log_probs`
+        gives them."""
+        logits, tgt = self._teacher_forced_logits(latent_z, packed_in, packed_tgt)
+        NT, B = int(tgt.numel()), int(packed_in.batch_sizes[0])
+        adv = torch.as_tensor(advantages, dtype=torch.float32, device=logits.device).detach()
+        if adv.dim() != 1 or adv.numel() not in (B, NT):
+            raise ValueError('advantages must be [B] or [NT]')
+        if adv.numel() == B and B != NT:                      # (B == NT: one token a sample, packed in sorted order)
+            adv = adv[_packed_samples(packed_in, logits.device)]
+        elif B == NT and packed_in.sorted_indices is not None:
+            adv = adv[packed_in.sorted_indices.to(logits.device)]
+        return policy_loss(logits, tgt, old_log_probs, adv, ref_log_probs, clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef,
+                           ignore_index=0, temperature=temperature)
 
 
 class GreedySearch:
@@ -696,6 +733,14 @@ class TeacherVAE(nn.Module):
 
     def decode(self, latent_z, input_seq, target_seq):
         return self.decoder.decoder_train_step(latent_z, input_seq, target_seq)
+
+    def log_probs(self, latent_z, input_seq, target_seq, temperature: float = 1.0):
+        """Scores of the target tokens given the latents: `StackGRUDecoder.decoder_log_probs`."""
+        return self.decoder.decoder_log_probs(latent_z, input_seq, target_seq, temperature)
+
+    def policy_loss(self, latent_z, input_seq, target_seq, advantages, old_log_probs, ref_log_probs=None, **options):
+        """`StackGRUDecoder.decoder_policy_step`."""
+        return self.decoder.decoder_policy_step(latent_z, input_seq, target_seq, advantages, old_log_probs, ref_log_probs, **options)
 
     def forward(self, input_seq, decoder_seq, target_seq, eps=None):
         mu, logvar = self.encode(input_seq)

@@ -48,6 +48,20 @@ def train_step_bundles(model, optimizer, enc_seq, dec_seq, tgt_seq, g_dists, seg
     return loss.detach(), decoder_loss.detach(), gr_loss.detach()
 
 
+def train_step_policy(model, optimizer, latent_z, dec_seq, tgt_seq, advantages, old_log_probs, ref_log_probs=None, grad_sync=None, **options):
+    """One optimizer step of fine-tuning the decoder from rewards, on sequences that it generated from `latent_z` [B, Z] (no counterpart
+    in the reference, which trains by likelihood only).  advantages [B] in the samples' order; old_log_probs / ref_log_probs:
+    `model.gru_vae.log_probs(latent_z, dec_seq, tgt_seq)` under the parameters that sampled, and under frozen ones.  options: clip_low,
+    clip_high, kl_coef, temperature.  Returns (loss, stats [3]) on the device (no host sync)."""
+    optimizer.zero_grad()
+    loss, stats = model.gru_vae.policy_loss(latent_z, dec_seq, tgt_seq, advantages, old_log_probs, ref_log_probs, **options)
+    loss.backward()
+    if grad_sync is not None:
+        grad_sync()
+    optimizer.step()
+    return loss.detach(), stats
+
+
 def train(epoch, model, train_loader, optimizer, scheduler, graph_gamma, growth_rate=0.0015, writer=None,
           verbose=False, distance_order='networkx'):
     """Reference reactions_vae.py:28-116: one bundle per step."""
