@@ -17,7 +17,10 @@ using ppk::uni_len;
 using ppk::uniform;
 
 constexpr int TILE = 16;                     // steps between two kept states
-constexpr long long MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 1024;
+// Splits of the time axis: where the sequences and channels alone leave less than half of FWD_WAVES waves (BWD_BLOCKS blocks), a split takes
+// as many steps as make that many, and MIN_SPAN at least.  Measured: 1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with
+// 32, 50 with 16 (joining them eats the rest); 1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096.
+constexpr long long MIN_SPAN = 32, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScanArgs {
@@ -102,7 +105,8 @@ template <int NP> __device__ __forceinline__ void store_states(float* p, int N, 
 
 // What a wave of the kernels with a lane a channel works on: 64 channels of a group of one sequence, one split of its steps
 struct Item {
-    long long b, t0, t1, len;
+    long long b;
+    int t0, t1, len;                           // steps
     int s, g, d;                               // split, group, this lane's channel (a lane behind a group's last channel does that one again,
                                                // and stores the same values to the same places: no lane is masked)
     __device__ __forceinline__ Item(const ScanArgs& a)
@@ -114,9 +118,10 @@ struct Item {
         g = cb / a.blocks_per_group;
         const int dl = (cb % a.blocks_per_group) * 64 + (int)threadIdx.x;
         d = g * a.per + (dl < a.per ? dl : a.per - 1);
-        len = uni_len(a.q, b);
-        t0 = s * a.span;
-        t1 = t0 + a.span < len ? t0 + a.span : len;
+        len = (int)uni_len(a.q, b);
+        const long long first = s * a.span, last = first + a.span;
+        t0 = first < len ? (int)first : len;
+        t1 = last < len ? (int)last : len;
     }
 };
 __device__ __forceinline__ long long carry_at(const ScanArgs& a, long long b, int s, int d) { return (b * a.splits + s) * a.D + d; }
@@ -124,10 +129,10 @@ __device__ __forceinline__ long long carry_at(const ScanArgs& a, long long b, in
 constexpr int AHEAD = 4;                       // steps whose elements are loaded before those of the steps before them are used
 
 // rows of AHEAD steps from t on, in direction dir, none behind `last`
-__device__ __forceinline__ void rows_of(const SeqBatch& q, long long t, long long last, int dir, unsigned (&rows)[AHEAD])
+__device__ __forceinline__ void rows_of(const SeqBatch& q, int t, int last, int dir, unsigned (&rows)[AHEAD])
 {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) { const long long u = t + dir * i; rows[i] = (unsigned)(dir > 0 ? (u < last ? u : last) : (u > last ? u : last)); }
+    for (int i = 0; i < AHEAD; ++i) { const int u = t + dir * i; rows[i] = (unsigned)(dir > 0 ? (u < last ? u : last) : (u > last ? u : last)); }
     if (q.off)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) rows[i] = (unsigned)uniform<long long>(q.off)[rows[i]];
@@ -140,7 +145,7 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 {
     const Item it(a);
     const int lane = threadIdx.x, N = a.N;
-    const long long len = it.len, t0 = it.t0, t1 = it.t1;
+    const int len = it.len, t0 = it.t0, t1 = it.t1;
     if (t0 >= len && it.s > 0) return;
     if (PART && t1 >= len) return;             // nothing enters a split behind the last
     float A2[NP], h[NP];
@@ -152,14 +157,15 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 #pragma unroll
     for (int n = 0; n < NP; ++n) A2[n] *= LOG2E;
     const float skip = !PART && a.skip ? a.skip[it.d] : 0.f, bias = a.bias ? a.bias[it.d] : 0.f;
-    const long long tile0 = first_tile(a, it.b);
+    const long long tile_size = (long long)a.D * N;
+    float* kept = a.kept ? a.kept + ((first_tile(a, it.b) + t0 / TILE) * a.D + it.d) * N : nullptr;
     const Rows<T> xs(a.x, it.b * a.xs.b, a.xs.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
     const Rows<T> Bs(a.Bm, it.b * a.Bs.b + it.g * a.Bg, a.Bs.t), Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t), ys(a.y, it.b * a.rows.b * a.D, a.rows.t * a.D);
     const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
     const bool gate = !PART && a.z;
     T xv[AHEAD], rv[AHEAD], zv[AHEAD];
     unsigned rows[AHEAD];
-    const auto fetch = [&](long long t) {      // steps t, t + 1, ...; behind the last one, the last one
+    const auto fetch = [&](int t) {            // steps t, t + 1, ...; behind the last one, the last one
         rows_of(a.q, t, t1 - 1, 1, rows);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) { xv[i] = xs.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
@@ -169,8 +175,8 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     };
     float sum = 0.f;
     if (t0 < t1) fetch(t0);
-    for (long long t = t0; t < t1; t += AHEAD) {
-        if (!PART && a.kept && t % TILE == 0) store_states<NP>(a.kept + ((tile0 + t / TILE) * a.D + it.d) * N, N, h);
+    for (int t = t0; t < t1; t += AHEAD) {
+        if (!PART && kept && t % TILE == 0) { store_states<NP>(kept, N, h); kept += tile_size; }
         float x[AHEAD], raw[AHEAD], z[AHEAD];
         unsigned r[AHEAD];
 #pragma unroll
@@ -209,7 +215,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 {
     const Item it(a);
     const int lane = threadIdx.x, N = a.N;
-    const long long t0 = it.t0, t1 = it.t1;
+    const int t0 = it.t0, t1 = it.t1;
     if (t0 >= it.len || it.s == 0) return;     // nothing leaves the first
     float A2[NP], g[NP];
     load_states<NP>(a.A + (long long)it.d * N, N, A2);
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
     T dv[AHEAD], rv[AHEAD], zv[AHEAD];
     unsigned rows[AHEAD];
-    const auto fetch = [&](long long t) {      // steps t - 1, t - 2, ...; before the first one, the first one
+    const auto fetch = [&](int t) {            // steps t - 1, t - 2, ...; before the first one, the first one
         rows_of(a.q, t - 1, t0, -1, rows);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) { dv[i] = ds.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     };
     float sum = 0.f;
     fetch(t1);
-    for (long long t = t1; t > t0; t -= AHEAD) {
+    for (int t = t1; t > t0; t -= AHEAD) {
         float dy[AHEAD], raw[AHEAD];
         unsigned r[AHEAD];
 #pragma unroll
