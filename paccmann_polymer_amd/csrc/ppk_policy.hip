@@ -139,7 +139,7 @@ __device__ __forceinline__ float policy_terms(const RowArgs& a, float old, float
     if (a.ref) {
         const float d = (float)((double)ref - lp);
         kl = kl_of(d);
-        g = fmaf(-a.beta, kl + d, g);                             // 1 - e^d = -(kl + d)
+        if (a.beta != 0.0f) g = fmaf(-a.beta, kl + d, g);         // 1 - e^d = -(kl + d); no KL term: nor what it could overflow to
     }
     return g;
 }
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(1024) void k_policy_final(RowArgs a, int nparts, fl
         for (int w = 0; w < 16; ++w)
             for (int k = 0; k < 3; ++k) t[k] += red[w][k];
         for (int k = 0; k < 3; ++k) t[k] *= inv;
-        loss[0] = (float)(t[0] + (double)a.beta * t[1]);
+        loss[0] = (float)(a.beta != 0.0f ? t[0] + (double)a.beta * t[1] : t[0]);
         for (int k = 0; k < 3; ++k) stats[k] = (float)t[k];
     }
 }
@@ -390,7 +390,7 @@ int check_rows(const char* what, int dtype, long long rows, long long V, const v
 {
     if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "%s: logits of type %d (fp32 and bf16 are supported)", what, dtype);
     if (rows < 0 || V < 1 || ld < V || V > (1LL << 30)) PPK_FAIL(PPK_ERR_SHAPE, "%s: rows=%lld V=%lld row stride=%lld", what, rows, V, ld);
-    if (!(temperature > 0.f) || temperature > 3.0e38f) PPK_FAIL(PPK_ERR_SHAPE, "%s: temperature %g", what, (double)temperature);
+    if (!(temperature >= 1.0e-30f) || temperature > 1.0e30f) PPK_FAIL(PPK_ERR_SHAPE, "%s: temperature %g", what, (double)temperature);
     if (rows > 0 && (!logits || !targets)) PPK_FAIL(PPK_ERR_NULL, "%s: null pointer", what);
     if ((uintptr_t)logits % (unsigned)elem_bytes(dtype)) PPK_FAIL(PPK_ERR_ALIGN, "%s: logits not aligned to their elements", what);
     return PPK_OK;

@@ -43,6 +43,8 @@ struct ScanArgs {
 };
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// A in the exponent of 2.  A state that forgets at once (A = -inf) keeps a finite exponent, which forgets all the same and leaves a dt of 0 one
+__device__ __forceinline__ float base2(float A) { return A == -INFINITY ? -3.4e38f : A * LOG2E; }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp2_(-LOG2E * x)); }
 // log(1 + e^x) = max(x, 0) + log1p(u), u = e^-|x|.  w = 1 + u is rounded; log1p(u) = log(w) + (u - (w - 1)) / w to first order in what
 // the rounding lost, which keeps a small dt (softplus of -7 is 1e-3) as exact as a large one.
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
         for (int n = 0; n < NP; ++n) h[n] = 0.f;
     } else load_states<NP>(a.splits > 1 ? a.carry + carry_at(a, it.b, it.s, it.d) * N : a.state + (it.b * a.D + it.d) * N, N, h);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) A2[n] *= LOG2E;
+    for (int n = 0; n < NP; ++n) A2[n] = base2(A2[n]);
     const float skip = !PART && a.skip ? a.skip[it.d] : 0.f, bias = a.bias ? a.bias[it.d] : 0.f;
     const long long tile_size = (long long)a.D * N;
     float* kept = a.kept ? a.kept + ((first_tile(a, it.b) + t0 / TILE) * a.D + it.d) * N : nullptr;
@@ -184,12 +186,12 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
         if (t + AHEAD < t1) fetch(t + AHEAD);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            __builtin_amdgcn_sched_barrier(0);     // one step's scalars at a time: those of eight do not fit
+            if (t + i >= t1) break;
+            __builtin_amdgcn_sched_barrier(0);     // one step's scalars at a time: those of all do not fit
             RowVec<T, NP, SCALAR> Bv, Cv;
             Bv.load((const T*)Bs.row(r[i]), lane, N);
             if (!PART) Cv.load((const T*)Cs.row(r[i]), lane, N);
-            // a step behind the last is the last one again, with dt = 0: the state stays, and y is stored a second time
-            const float s = a.softplus ? softplus(raw[i]) : raw[i], dt = t + i < t1 ? s : 0.f, dx = dt * x[i];
+            const float dt = a.softplus ? softplus(raw[i]) : raw[i], dx = dt * x[i];
             float y[4] = {skip * x[i], 0.f, 0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
@@ -220,7 +222,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     float A2[NP], g[NP];
     load_states<NP>(a.A + (long long)it.d * N, N, A2);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
+    for (int n = 0; n < NP; ++n) { A2[n] = base2(A2[n]); g[n] = 0.f; }
     const float bias = a.bias ? a.bias[it.d] : 0.f;
     const Rows<T> ds(a.dy, it.b * a.dys.b, a.dys.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
     const Rows<T> Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t);
@@ -250,14 +252,14 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
         if (t - AHEAD > t0) fetch(t - AHEAD);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
+            if (t - 1 - i < t0) break;
             __builtin_amdgcn_sched_barrier(0);
             RowVec<T, NP, SCALAR> Cv;
             Cv.load((const T*)Cs.row(r[i]), lane, N);
-            const bool in = t - 1 - i >= t0;
-            const float s = a.softplus ? softplus(raw[i]) : raw[i], dt = in ? s : 0.f, u = in ? dy[i] : 0.f;
+            const float dt = a.softplus ? softplus(raw[i]) : raw[i];
             sum += dt;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(u, Cv.at(n), g[n]);
+            for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(dy[i], Cv.at(n), g[n]);
         }
     }
     store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, g);
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
     const long long dn = (long long)a.D * a.N, e = (long long)blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
     if (e >= dn) return;
     const int d = (int)(e / a.N);
-    const float A2 = a.A[e] * LOG2E;
+    const float A2 = base2(a.A[e]);
     const float* from = REV ? a.dlast : a.state;
     const long long len = uni_len(a.q, b);
     const int used = len > 0 ? (int)((len + a.span - 1) / a.span) : 1;          // no steps: the first split still hands on what enters it
@@ -345,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int n = ns * 4 + j;
-        A2[j] = live && n < N ? a.A[(long long)d * N + n] * LOG2E : 0.f;
+        A2[j] = live && n < N ? base2(a.A[(long long)d * N + n]) : 0.f;
         dh[j] = live && n < N && into ? into[n] : 0.f;
     }
     const float skip = a.skip && plive ? a.skip[pd] : 0.f, bias = a.bias && plive ? a.bias[pd] : 0.f;
@@ -566,7 +568,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
     float y = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        h[j] = fmaf(exp2_(dt * (A[j] * LOG2E)), h[j], dx * Bv[j]);
+        h[j] = fmaf(exp2_(dt * base2(A[j])), h[j], dx * Bv[j]);
         y = fmaf(h[j], Cv[j], y);
     }
     if (WIDE) *reinterpret_cast<float4*>(next + at_h) = make_float4(h[0], h[1], h[2], h[3]);
@@ -678,7 +680,7 @@ int scan_check(const char* what, int dtype, long long T, long long B, long long 
     if (T < 0 || B < 0 || D < 1 || N < 1 || G < 1 || D % G) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld N=%lld G=%lld", what, T, B, D, N, G);
     if (N > 64) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld states a channel (at most 64)", what, N);
     if (D > (1 << 20)) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld channels", what, D);
-    if (T >= 1LL << 31) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld steps", what, T);
+    if (T >= 1LL << 30) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld steps", what, T);
     return PPK_OK;
 }
 

@@ -21,8 +21,8 @@ def _check_logits(what, logits, targets, temperature):
         raise ValueError(f'{what}: targets must be [rows]')
     if targets.dtype != torch.int64:
         raise TypeError(f'{what}: targets must be int64')
-    if not 0.0 < float(temperature) < float('inf'):
-        raise ValueError(f'{what}: the temperature must be positive and finite')
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError(f'{what}: the temperature must be positive and finite (1e-30 to 1e30)')
     return _C.dtype_code(logits, what)
 
 

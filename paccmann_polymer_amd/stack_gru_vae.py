@@ -665,14 +665,15 @@ class StackGRUDecoder(StackGRU):
 
     def decoder_log_probs(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence, temperature: float = 1.0):
         """log softmax(logits / temperature) at every target, [NT] in packed order; 0 at padding targets.  Under `torch.no_grad()`:
-        the old or reference scores that `decoder_policy_step` takes."""
+        the old or reference scores that `decoder_policy_step` takes (in eval mode, where the model has dropout: its factors are drawn anew
+        at every call)."""
         logits, tgt = self._teacher_forced_logits(latent_z, packed_in, packed_tgt)
         return token_log_probs(logits, tgt, ignore_index=0, temperature=temperature)
 
     def decoder_policy_step(self, latent_z, packed_in: PackedSequence, packed_tgt: PackedSequence, advantages, old_log_probs,
                             ref_log_probs=None, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0):
         """Clipped policy loss of generated sequences (`policy_loss.policy_loss`) -> (loss, stats [3]).  advantages: one per
-        sample [B] in ORIGINAL order, or one per token [NT] in packed order; old / ref log-probabilities [NT] as `decoder_log_probs`
+        sample [B] in ORIGINAL order, or one per token [NT] in packed order (as many tokens as samples: per sample); old / ref log-probabilities [NT] as `decoder_log_probs`
         gives them."""
         logits, tgt = self._teacher_forced_logits(latent_z, packed_in, packed_tgt)
         NT, B = int(tgt.numel()), int(packed_in.batch_sizes[0])

@@ -38,6 +38,7 @@ class PackedRows(NamedTuple):
     sequences: int
     rows: int
     kept: int                        # kept states in all
+    batch_sizes: torch.Tensor        # [T] int64, host: what it was made of
 
 
 def packed_rows(batch_sizes, device, sequences: Optional[int] = None) -> PackedRows:
@@ -64,7 +65,7 @@ def packed_rows(batch_sizes, device, sequences: Optional[int] = None) -> PackedR
     tiles = torch.zeros(B + 1, dtype=torch.int64)
     tiles[1:] = torch.cumsum((lengths + tile - 1) // tile, 0)
     sent = torch.cat([off, lengths, tiles]).to(device)
-    return PackedRows(sent[:T + 1], sent[T + 1:T + 1 + B], sent[T + 1 + B:], T, B, int(off[-1]), int(tiles[-1]))
+    return PackedRows(sent[:T + 1], sent[T + 1:T + 1 + B], sent[T + 1 + B:], T, B, int(off[-1]), int(tiles[-1]), bs)
 
 
 def _data(t):
@@ -84,6 +85,8 @@ class _Batch:
         if plan is not None:
             if not isinstance(plan, PackedRows):
                 raise TypeError(f'{what}: plan must be what packed_rows gives')
+            if isinstance(x, PackedSequence) and not torch.equal(x.batch_sizes, plan.batch_sizes):
+                raise ValueError(f'{what}: the plan is of another packing than x')
             if data.dim() != 2 or data.shape[0] != plan.rows:
                 raise ValueError(f'{what}: x must be [{plan.rows}, D] for this plan')
             self.T, self.B, self.rows = plan.steps, plan.sequences, plan.rows

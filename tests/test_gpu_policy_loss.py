@@ -240,3 +240,31 @@ def test_other_stream_and_graph_replays():
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b), k
+
+
+def test_reference_without_a_kl_term_cannot_spoil_it():
+    """kl_coef 0: a reference score so far off that e^d overflows is in the statistics, not in the loss or its gradient."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(9, 21, torch.float32, 3, ignored=0.0)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    ref[4] = 200.0
+    x = logits.detach().requires_grad_()
+    loss, stats = policy_loss(x, tgt, old, adv, ref)
+    bare, _ = policy_loss(x, tgt, old, adv)
+    assert torch.equal(loss, bare) and float(stats[1]) == float('inf')
+    (d,) = torch.autograd.grad(loss, x)
+    assert bool(torch.isfinite(d).all())
+
+
+@pytest.mark.parametrize('seed', range(3))
+def test_small_kl_terms_keep_their_digits(seed):
+    """d of 1e-2 to 1e-5: d^2 / 2 is far below what e^d rounds to in 32 bits."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(64, 50, torch.float32, 20 + seed, ignored=0.0)
+    lp, _ = definition(logits, tgt, 1.0)
+    ref = (lp + 10.0 ** (-2 - seed)).float()
+    d = ref.double() - lp
+    want = (torch.expm1(d) - d).mean()
+    _, stats = policy_loss(logits, tgt, lp.float(), torch.zeros(64, device='cuda'), ref, kl_coef=1.0)
+    # d is off by what lp is, 130 H; the term by d times that, and eight roundings of its series
+    assert abs(float(stats[1]) - float(want)) <= float(d.abs().max()) * 130 * H + 8 * H * float(want)

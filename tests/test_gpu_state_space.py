@@ -423,3 +423,45 @@ def test_other_stream_and_graph_replays():
         for out in outs:
             for a, b in zip(out, want):
                 assert torch.equal(a, b), k
+
+
+def test_no_sequences():
+    from paccmann_polymer_amd.state_space import causal_conv, selective_scan
+    x = torch.zeros(5, 0, 8, device=DEV, requires_grad=True)
+    bc = torch.zeros(5, 0, 4, device=DEV)
+    A, w = torch.full((8, 4), -1.0, device=DEV, requires_grad=True), torch.ones(8, 4, device=DEV, requires_grad=True)
+    y, last = selective_scan(x, x, A, bc, bc)
+    c, cl = causal_conv(x, w)
+    assert y.shape == x.shape and last.shape == (0, 8, 4) and c.shape == x.shape and cl.shape == (0, 3, 8)
+    dA, dw = torch.autograd.grad(y.sum() + c.sum(), (A, w))
+    assert not bool(dA.any()) and not bool(dw.any())
+
+
+@pytest.mark.parametrize('T', [3, 5, 200])
+def test_infinities_stay_where_the_formula_has_them(T):
+    """States that forget at once (A = -inf), an infinite input in a last step and beside it other sequences and channels that are not
+    touched by it; lengths that end inside a tile and inside a split."""
+    from paccmann_polymer_amd.state_space import causal_conv, selective_scan
+    lay, t, dy, dlast = scan_case([T, T, T - 1], 'packed', 20, 16, 1, torch.float32, True, True, True, True, True)
+    a = {k: v.clone() for k, v in t.items()}
+    a['A'][:, 3] = float('-inf')
+    leaves = {k: v.detach().requires_grad_() for k, v in a.items()}
+    y, last = selective_scan(**leaves, plan=lay.plan)
+    g = dict(zip(a, torch.autograd.grad((y, last), list(leaves.values()), (dy, dlast))))
+    assert all(bool(torch.isfinite(v).all()) for v in (y, last, *g.values()))
+    b = {k: v.clone() for k, v in t.items()}
+    b['A'][:, 3] = -1e30                                                # forgets as completely
+    y2, last2 = selective_scan(**b, plan=lay.plan)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+    row = int(lay.off[T - 1] + 1)                                       # the last step of sequence 1
+    c = {k: v.clone() for k, v in t.items()}
+    c['x'][row, 7] = float('inf')
+    clean, clean_last = selective_scan(**t, plan=lay.plan)
+    y3, last3 = selective_scan(**c, plan=lay.plan)
+    assert bool(torch.isinf(last3[1, 7]).all())
+    keep = torch.ones_like(y3, dtype=torch.bool)
+    keep[row, 7] = False
+    assert torch.equal(y3[keep], clean[keep]) and torch.equal(last3[[0, 2]], clean_last[[0, 2]])
+    w = torch.randn(20, 4, device=DEV)
+    y4, y5 = causal_conv(c['x'], w, plan=lay.plan)[0], causal_conv(t['x'], w, plan=lay.plan)[0]
+    assert torch.equal(y4[keep], y5[keep])

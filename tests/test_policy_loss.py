@@ -33,6 +33,8 @@ def good(**change):
     (dict(clip_high=float('inf')), ValueError),
     (dict(temperature=0.0), ValueError),
     (dict(temperature=float('nan')), ValueError),
+    (dict(temperature=1e-39), ValueError),
+    (dict(temperature=float('inf')), ValueError),
     (dict(), _C.PPKError),                                 # all in order, but on the CPU: there is no fallback
 ])
 def test_policy_loss_refuses(change, error):

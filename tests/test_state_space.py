@@ -163,3 +163,11 @@ def strides(n):
 ])
 def test_c_entries_return_codes(call, code):
     assert call(_C.lib) == code
+
+
+def test_plan_of_another_packing_is_refused():
+    packed = pack_sequence([torch.zeros(3, D), torch.zeros(2, D)])
+    other = S.packed_rows(pack_sequence([torch.zeros(4, D), torch.zeros(1, D)]), 'cpu')
+    assert other.rows == 5
+    with pytest.raises(ValueError, match='another packing'):
+        S.causal_conv(packed, torch.zeros(D, K), plan=other)
