@@ -190,14 +190,15 @@ def dtype_code(t, what):
 
 def one_device(*tensors):
     """The GPU that all of these tensors (None: left out) are on; anything else is refused."""
-    require_gpu(*tensors)
     device = None
     for t in tensors:
         if t is None:
             continue
         if device is None:
+            require_gpu(t)
             device = t.device
         elif t.device != device:
+            require_gpu(t)
             raise PPKError(f'tensors on different devices: {device} and {t.device}')
     return device
 

@@ -184,9 +184,7 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) { x[i] = to_f32(xv[i]); raw[i] = to_f32(rv[i]) + bias; z[i] = gate ? to_f32(zv[i]) : 0.f; r[i] = rows[i]; }
         if (t + AHEAD < t1) fetch(t + AHEAD);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (t + i >= t1) break;
+        const auto step = [&](int i) {
             __builtin_amdgcn_sched_barrier(0);     // one step's scalars at a time: those of all do not fit
             RowVec<T, NP, SCALAR> Bv, Cv;
             Bv.load((const T*)Bs.row(r[i]), lane, N);
@@ -198,10 +196,18 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
                 h[n] = fmaf(exp2_(dt * A2[n]), h[n], dx * Bv.at(n));
                 if (!PART) y[n & 3] = fmaf(h[n], Cv.at(n), y[n & 3]);
             }
-            if (PART) { sum += dt; continue; }
+            if (PART) { sum += dt; return; }
             float out = (y[0] + y[1]) + (y[2] + y[3]);
             if (gate) out *= z[i] * sigmoid(z[i]);
             ys.put(r[i], d, from_f32<T>(out));
+        };
+        if (PART || t + AHEAD <= t1) {             // a split that is not a sequence's last has whole groups only
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) step(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (t + i < t1) step(i);
         }
     }
     if (PART) {
@@ -250,9 +256,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
             r[i] = rows[i];
         }
         if (t - AHEAD > t0) fetch(t - AHEAD);
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (t - 1 - i < t0) break;
+        const auto step = [&](int i) {
             __builtin_amdgcn_sched_barrier(0);
             RowVec<T, NP, SCALAR> Cv;
             Cv.load((const T*)Cs.row(r[i]), lane, N);
@@ -260,6 +264,14 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
             sum += dt;
 #pragma unroll
             for (int n = 0; n < NP; ++n) g[n] = exp2_(dt * A2[n]) * fmaf(dy[i], Cv.at(n), g[n]);
+        };
+        if (t - AHEAD >= t0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) step(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (t - 1 - i >= t0) step(i);
         }
     }
     store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, g);

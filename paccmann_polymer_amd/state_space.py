@@ -134,14 +134,17 @@ class _Batch:
 
 
 def _param(what, name, t, shape):
-    if not torch.is_tensor(t) or tuple(t.shape) != tuple(shape):
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f'{what}: {name} must be {list(shape)}')
     if t.dtype != torch.float32:
         raise TypeError(f'{what}: {name} must be float32')
 
 
+_I64 = {n: ctypes.c_int64 * n for n in (4, 6, 16)}
+
+
 def _ints(*values):
-    return (ctypes.c_int64 * len(values))(*values)
+    return _I64[len(values)](*values)
 
 
 def _contiguous(t):
@@ -251,7 +254,7 @@ def _overlap(a, b):
 def _step_out(what, state, out, others):
     """Where a step writes its new state: `out`, or fresh memory.  `out` may be the state itself, but share memory with nothing else."""
     if out is None:
-        return torch.empty(state.shape, dtype=state.dtype, device=state.device)
+        return state.new_empty(state.shape)
     if not torch.is_tensor(out) or out.shape != state.shape or out.dtype != state.dtype or out.device != state.device or not out.is_contiguous():
         raise ValueError(f'{what}: out must be a contiguous tensor like state')
     if out.data_ptr() != state.data_ptr() and _overlap(out, state):
@@ -266,25 +269,28 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
     """One token of each of B sequences: x [B, D], state [B, K - 1, D] -> (y [B, D], new state).  `out`: where the new state goes
     (it may be `state`: updated in place).  Inference only: training goes through `causal_conv`."""
     what = 'causal_conv_step'
-    if not torch.is_tensor(x) or x.dim() != 2 or x.shape[1] < 1:
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f'{what}: x must be [B, D]')
     code = _C.dtype_code(x, what)
     B, D = x.shape
     silu = _conv_params(what, weight, bias, D, activation)
     K = weight.shape[1]
-    if not torch.is_tensor(state) or tuple(state.shape) != (B, K - 1, D):
+    if not isinstance(state, torch.Tensor) or state.shape != (B, K - 1, D):
         raise ValueError(f'{what}: state must be {[B, K - 1, D]}')
     if state.dtype != x.dtype:
         raise TypeError(f'{what}: state must be {x.dtype}, as x is')
     dev = _C.one_device(x, state, weight, bias)
     with _C.on_device(dev):
-        x = x.detach()
-        x = x if x.stride(1) == 1 or D == 1 else x.contiguous()
+        ld, unit = x.stride()
+        if unit != 1 and D != 1:
+            x = x.contiguous()
+            ld = D
         weight, bias = weight.contiguous(), _contiguous(bias)
         new = _step_out(what, state, out, (x, weight, bias))
         state = state.contiguous()
-        y = torch.empty(B, D, dtype=x.dtype, device=dev)
-        _C.check(_lib.ppk_causal_conv_step(code, B, D, K, _C.addr(x), x.stride(0), _C.addr(state), _C.addr(weight), _C.addr(bias), silu, _C.addr(y), _C.addr(new), _C.stream_on(dev)))
+        y = x.new_empty((B, D))
+        _C.check(_lib.ppk_causal_conv_step(code, B, D, K, x.data_ptr(), ld, state.data_ptr(), weight.data_ptr(), _C.addr(bias), silu, y.data_ptr(),
+                                           new.data_ptr(), _C.stream_on(dev)))
     return y, new
 
 
@@ -408,35 +414,34 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
     new state).  `out`: where the new state goes (it may be `state`: updated in place).  Inference only: training goes through
     `selective_scan`."""
     what = 'selective_scan_step'
-    if not torch.is_tensor(x) or x.dim() != 2 or x.shape[1] < 1:
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f'{what}: x must be [B, channels]')
-    code = _C.dtype_code(x, what)
+    dtype, code = x.dtype, _C.dtype_code(x, what)
     n, width = x.shape
     N = _scan_params(what, A, D, dt_bias, width)
-
-    def row(name, t, tail):
-        if not torch.is_tensor(t) or tuple(t.shape) != (n, *tail):
-            raise ValueError(f'{what}: {name} must be {[n, *tail]}')
-        if t.dtype != x.dtype:
-            raise TypeError(f'{what}: {name} must be {x.dtype}, as x is')
-        t = t.detach()
-        return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-    Bg, Cg = _grouped(what, 'B', B, (n,), width, N), _grouped(what, 'C', C, (n,), width, N)
-    if Bg.shape != Cg.shape:
-        raise ValueError(f'{what}: B has {Bg.shape[-2]} groups, C has {Cg.shape[-2]}')
-    data, raw = row('x', x, (width,)), row('dt', dt, (width,))
-    gate = None if z is None else row('z', z, (width,))
-    Bg, Cg = row('B', Bg, Bg.shape[1:]), row('C', Cg, Cg.shape[1:])
+    B, C = _grouped(what, 'B', B, (n,), width, N), _grouped(what, 'C', C, (n,), width, N)
+    if B.shape != C.shape:
+        raise ValueError(f'{what}: B has shape {list(B.shape)}, C {list(C.shape)}')
+    rows = []
+    for name, v, shape in (('x', x, (n, width)), ('dt', dt, (n, width)), ('z', z, (n, width)), ('B', B, (n, *B.shape[1:])), ('C', C, (n, *B.shape[1:]))):
+        if v is None and name == 'z':
+            rows.append(None)
+            continue
+        if not isinstance(v, torch.Tensor) or v.shape != shape:
+            raise ValueError(f'{what}: {name} must be {list(shape)}')
+        if v.dtype != dtype:
+            raise TypeError(f'{what}: {name} must be {dtype}, as x is')
+        rows.append(v if v.stride(-1) == 1 or shape[-1] == 1 else v.contiguous())
+    x, dt, z, B, C = rows
     _param(what, 'state', state, (n, width, N))
-    dev = _C.one_device(data, raw, A, Bg, Cg, D, gate, dt_bias, state)
+    dev = _C.one_device(x, dt, A, B, C, D, z, dt_bias, state)
     with _C.on_device(dev):
         A, D, dt_bias = A.contiguous(), _contiguous(D), _contiguous(dt_bias)
-        new = _step_out(what, state, out, (data, raw, A, Bg, Cg, D, gate, dt_bias))
+        new = _step_out(what, state, out, (x, dt, A, B, C, D, z, dt_bias))
         state = state.contiguous()
-        y = torch.empty(n, width, dtype=x.dtype, device=dev)
-        pair = lambda t: (0, 0) if t is None else (0, t.stride(0))      # noqa: E731
-        strides = _ints(*pair(data), *pair(raw), 0, Bg.stride(0), Bg.stride(1), 0, Cg.stride(0), Cg.stride(1), *pair(gate), 0, 1, 0, 0)
-        _C.check(_lib.ppk_selective_scan_step(code, n, width, N, Bg.shape[1], _C.addr(data), _C.addr(raw), _C.addr(A), _C.addr(Bg), _C.addr(Cg), _C.addr(D), _C.addr(gate),
-                                              _C.addr(dt_bias), _C.addr(state), int(bool(dt_softplus)), _C.addr(y), _C.addr(new), strides, _C.stream_on(dev)))
+        y = x.new_empty((n, width))
+        strides = _ints(0, x.stride(0), 0, dt.stride(0), 0, B.stride(0), B.stride(1), 0, C.stride(0), C.stride(1), 0, 0 if z is None else z.stride(0), 0, 1, 0, 0)
+        _C.check(_lib.ppk_selective_scan_step(code, n, width, N, B.shape[1], x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _C.addr(D),
+                                              _C.addr(z), _C.addr(dt_bias), state.data_ptr(), int(bool(dt_softplus)), y.data_ptr(), new.data_ptr(), strides,
+                                              _C.stream_on(dev)))
     return y, new
