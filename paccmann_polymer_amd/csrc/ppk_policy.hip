@@ -355,7 +355,8 @@ __global__ __launch_bounds__(256) void k_logp_bwd(RowArgs a, const float* __rest
     }
 }
 
-// grad *= scale[0], and nothing at all where that is 1 (the upstream gradient of a loss that is the root of the backward pass)
+// grad *= scale[0], and nothing at all where that is 1 (the upstream gradient of a loss that is the root of the backward pass).  A bf16 gradient
+// is rounded a second time here: two half-steps in all, where a factor is not a power of two.
 template <typename T>
 __global__ __launch_bounds__(256) void k_scale_unless_one(T* __restrict__ g, long long n, const float* __restrict__ scale)
 {

@@ -18,9 +18,10 @@ using ppk::uniform;
 
 constexpr int TILE = 16;                     // steps between two kept states
 // Splits of the time axis: where the sequences and channels alone leave less than half of FWD_WAVES waves (BWD_BLOCKS blocks), a split takes
-// as many steps as make that many, and MIN_SPAN at least.  Measured: 1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with
-// 32, 50 with 16 (joining them eats the rest); 1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096.
-constexpr long long MIN_SPAN = 32, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
+// as many steps as make that many, and MIN_SPAN (BWD_MIN_SPAN) at least.  Measured: 1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with
+// 32, 50 with 16 (joining them eats the rest); 1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096;
+// 21 x 100 x 333 fp32 backward 45 us in one launch, 42 us in the three of a split.
+constexpr long long MIN_SPAN = 32, BWD_MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScanArgs {
@@ -599,24 +600,24 @@ int bwd_slices(long long N) { return N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 int padded(long long N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 
 // How many steps a split of the time axis takes.  `units`: what runs at once without one, `want`: what fills the card.
-long long span_of(long long T, long long units, long long want)
+long long span_of(long long T, long long units, long long want, long long least)
 {
     const long long all = ceil_div(T > 0 ? T : 1, TILE) * TILE;
-    if (units * 2 > want || all <= 2 * MIN_SPAN) return all;
+    if (units * 2 > want || all <= 2 * least) return all;
     const long long span = ceil_div(ceil_div(all * units, want), TILE) * TILE;
-    return span > MIN_SPAN ? span : MIN_SPAN;
+    return span > least ? span : least;
 }
 struct Plan { long long blocks_per_group, span, splits; };
-Plan plan_of(long long T, long long B, long long D, long long G, long long channels, long long want)
+Plan plan_of(long long T, long long B, long long D, long long G, long long channels, long long want, long long least)
 {
     Plan p;
     p.blocks_per_group = ceil_div(D / G, channels);
-    p.span = span_of(T, B * G * p.blocks_per_group, want);
+    p.span = span_of(T, B * G * p.blocks_per_group, want, least);
     p.splits = ceil_div(T > 0 ? T : 1, p.span);
     return p;
 }
-Plan fwd_plan(long long T, long long B, long long D, long long G) { return plan_of(T, B, D, G, 64, FWD_WAVES); }
-Plan bwd_plan(long long T, long long B, long long D, long long N, long long G) { return plan_of(T, B, D, G, 256 / bwd_slices(N), BWD_BLOCKS); }
+Plan fwd_plan(long long T, long long B, long long D, long long G) { return plan_of(T, B, D, G, 64, FWD_WAVES, MIN_SPAN); }
+Plan bwd_plan(long long T, long long B, long long D, long long N, long long G) { return plan_of(T, B, D, G, 256 / bwd_slices(N), BWD_BLOCKS, BWD_MIN_SPAN); }
 size_t carry_bytes(long long B, long long D, long long N, long long splits)
 {
     return splits > 1 ? ppk_align_up((size_t)B * splits * D * N * 4, 256) + ppk_align_up((size_t)B * splits * D * 4, 256) : 0;

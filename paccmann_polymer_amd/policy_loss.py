@@ -141,7 +141,9 @@ def policy_loss(logits, targets, old_log_probs, advantages, ref_log_probs=None, 
     in the logits.  stats: [3] fp32 on the device, not differentiable: the means of the policy term, of the KL term (0 without a
     reference) and of the rows that the clip holds.
     logits [rows, V] fp32 or bf16; targets [rows] int64; old_log_probs, advantages, ref_log_probs [rows] fp32 (constants: what
-    `token_log_probs` gave under the sampling and under the reference parameters, at the same temperature)."""
+    `token_log_probs` gave under the sampling and under the reference parameters, at the same temperature).
+    A call whose logits want a gradient writes it in the same pass and holds it, a tensor of the logits' size and type, until the
+    backward pass."""
     what = 'policy_loss'
     _check_logits(what, logits, targets, temperature)
     rows = logits.shape[0]

@@ -79,7 +79,7 @@ class _Batch:
         if isinstance(x, PackedSequence) and plan is None:
             plan = packed_rows(x.batch_sizes, x.data.device)
         data = _data(x)
-        if not torch.is_tensor(data):
+        if not isinstance(data, torch.Tensor):
             raise TypeError(f'{what}: x must be a tensor or a PackedSequence')
         self.what, self.plan = what, plan
         if plan is not None:
@@ -94,7 +94,7 @@ class _Batch:
         else:
             if data.dim() != 3:
                 raise ValueError(f'{what}: x must be [T, B, D], or the rows of a packed batch with its plan')
-            self.T, self.B = data.shape[:2]
+            self.T, self.B, _ = data.shape
             self.rows = self.T * self.B
             self.lead = (self.T, self.B)
             # outputs lie as x does: batch-first where a sequence's steps are next to each other
@@ -106,24 +106,27 @@ class _Batch:
 
     def take(self, name, t, tail, dtype):
         """A per-step tensor [lead, tail], the elements of its last dimension next to each other."""
-        t = _data(t)
-        if not torch.is_tensor(t) or tuple(t.shape) != (*self.lead, *tail):
-            raise ValueError(f'{self.what}: {name} must be {[*self.lead, *tail]}, not {list(t.shape) if torch.is_tensor(t) else t}')
+        if isinstance(t, PackedSequence):
+            t = t.data
+        if not isinstance(t, torch.Tensor) or t.shape != self.lead + tail:
+            raise ValueError(f'{self.what}: {name} must be {[*self.lead, *tail]}, not {list(t.shape) if isinstance(t, torch.Tensor) else t}')
         if t.dtype != dtype:
             raise TypeError(f'{self.what}: {name} must be {dtype}, as x is')
-        near = max(t.stride()[:2], default=0) < FAR_ROWS
-        return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
+        s = t.stride()
+        return t if s[0] < FAR_ROWS and s[1] < FAR_ROWS and (s[-1] == 1 or t.shape[-1] == 1) else t.contiguous()
 
     def strides(self, t):
         """Of a step and of a sequence, in elements."""
         if t is None:
-            return (0, 0)
-        return (t.stride(0), t.stride(0)) if self.plan is not None else (t.stride(0), t.stride(1))
+            return 0, 0
+        s = t.stride()
+        return (s[0], s[0]) if self.plan is not None else s[:2]
 
-    def new(self, tail, dtype, device):
+    def new(self, tail, like):
+        """An uninitialised per-step tensor of the type and device of `like`, laid out as x is."""
         if self.plan is None and self.batch_first:
-            return torch.empty(self.B, self.T, *tail, dtype=dtype, device=device).transpose(0, 1)
-        return torch.empty(*self.lead, *tail, dtype=dtype, device=device)
+            return like.new_empty((self.B, self.T, *tail)).transpose(0, 1)
+        return like.new_empty(self.lead + tail)
 
     def pointers(self):
         p = self.plan
@@ -169,8 +172,8 @@ class _CausalConv(torch.autograd.Function):
         weight, bias, state = weight.contiguous(), _contiguous(bias), _contiguous(state)
         D, K = weight.shape
         with _C.on_device(dev):
-            y = batch.new((D,), x.dtype, dev)
-            last = torch.empty(batch.B, K - 1, D, dtype=x.dtype, device=dev)
+            y = batch.new((D,), x)
+            last = x.new_empty((batch.B, K - 1, D))
             off, lengths = batch.pointers()
             _C.check(_lib.ppk_causal_conv_fwd(_C.DTYPES[x.dtype], batch.T, batch.B, D, K, off, lengths, _C.addr(x), _C.addr(weight), _C.addr(bias), _C.addr(state),
                                               silu, _C.addr(y), _C.addr(last), _ints(*batch.strides(x), *batch.strides(y)), _C.stream_on(dev)))
@@ -188,7 +191,7 @@ class _CausalConv(torch.autograd.Function):
         with _C.on_device(dev):
             dy = torch.zeros(*batch.lead, D, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (D,), x.dtype)
             dlast = _contiguous(dlast)
-            dx = batch.new((D,), x.dtype, dev)
+            dx = batch.new((D,), x)
             dw = torch.empty_like(weight)
             db = None if bias is None else torch.empty_like(bias)
             ds = None if state is None else torch.empty_like(state)
@@ -296,9 +299,8 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
 
 # ------------------------------------------------------------------------------------------------------------ selective scan
 def _scan_strides(batch, x, raw, B, C, z, rows, dy):
-    bt, bb = batch.strides(B)
-    ct, cb = batch.strides(C)
-    return _ints(*batch.strides(x), *batch.strides(raw), bt, bb, B.stride(-2), ct, cb, C.stride(-2), *batch.strides(z), *rows, *batch.strides(dy))
+    f = batch.strides
+    return _ints(*f(x), *f(raw), *f(B), B.stride(-2), *f(C), C.stride(-2), *f(z), *rows, *f(dy))
 
 
 class _SelectiveScan(torch.autograd.Function):
@@ -310,13 +312,12 @@ class _SelectiveScan(torch.autograd.Function):
         N, G, width = A.shape[1], B.shape[-2], batch.D
         tiles = None if batch.plan is None else batch.plan.tiles
         with _C.on_device(dev):
-            y = batch.new((width,), x.dtype, dev)
-            last = torch.empty(batch.B, width, N, dtype=torch.float32, device=dev)
+            y = batch.new((width,), x)
+            last = A.new_empty((batch.B, width, N))
             kept = None
             if want_grad:
-                tile = int(_lib.ppk_selective_scan_tile())
-                n = batch.plan.kept if batch.plan is not None else batch.B * ((batch.T + tile - 1) // tile)
-                kept = torch.empty(n, width, N, dtype=torch.float32, device=dev)
+                n = batch.plan.kept if batch.plan is not None else batch.B * -(-batch.T // int(_lib.ppk_selective_scan_tile()))
+                kept = A.new_empty((n, width, N))
             off, lengths = batch.pointers()
             wsb = _lib.ppk_selective_scan_fwd_workspace_bytes(batch.T, batch.B, width, N, G)
             ws = _ws(wsb, dev) if wsb else None
@@ -339,13 +340,13 @@ class _SelectiveScan(torch.autograd.Function):
         with _C.on_device(dev):
             dy = torch.zeros(*batch.lead, width, dtype=x.dtype, device=dev) if dy is None else batch.take('dy', dy, (width,), x.dtype)
             dlast = _contiguous(dlast)
-            dx, draw = batch.new((width,), x.dtype, dev), batch.new((width,), x.dtype, dev)
-            dz = None if z is None else batch.new((width,), x.dtype, dev)
-            dB, dC = batch.new((G, N), x.dtype, dev), batch.new((G, N), x.dtype, dev)
+            dx, draw = batch.new((width,), x), batch.new((width,), x)
+            dz = None if z is None else batch.new((width,), x)
+            dB, dC = batch.new((G, N), x), batch.new((G, N), x)
             dA = torch.empty_like(A)
             dD = None if D is None else torch.empty_like(D)
             dbias = None if dt_bias is None else torch.empty_like(dt_bias)
-            dstate = torch.empty(batch.B, width, N, dtype=torch.float32, device=dev) if ctx.has_state else None
+            dstate = A.new_empty((batch.B, width, N)) if ctx.has_state else None
             off, lengths = batch.pointers()
             wsb = _lib.ppk_selective_scan_bwd_workspace_bytes(batch.T, batch.B, width, N, G, batch.rows)
             ws = _ws(wsb, dev)
@@ -371,8 +372,9 @@ def _scan_params(what, A, D, dt_bias, width):
 
 def _grouped(what, name, t, lead, width, N):
     """B or C as [..., groups, N]."""
-    t = _data(t)
-    if not torch.is_tensor(t) or t.dim() not in (len(lead) + 1, len(lead) + 2) or t.shape[-1] != N:
+    if isinstance(t, PackedSequence):
+        t = t.data
+    if not isinstance(t, torch.Tensor) or t.dim() not in (len(lead) + 1, len(lead) + 2) or t.shape[-1] != N:
         raise ValueError(f'{what}: {name} must be [..., groups, {N}] or [..., {N}]')
     t = t.unsqueeze(-2) if t.dim() == len(lead) + 1 else t
     if t.shape[-2] < 1 or width % t.shape[-2]:
@@ -399,13 +401,15 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, plan: Optional[
     Bg, Cg = _grouped(what, 'B', B, batch.lead, width, N), _grouped(what, 'C', C, batch.lead, width, N)
     if Bg.shape != Cg.shape:
         raise ValueError(f'{what}: B has {Bg.shape[-2]} groups, C has {Cg.shape[-2]}')
-    Bg, Cg = batch.take('B', Bg, Bg.shape[-2:], data.dtype), batch.take('C', Cg, Cg.shape[-2:], data.dtype)
+    tail = tuple(Bg.shape[-2:])
+    Bg, Cg = batch.take('B', Bg, tail, data.dtype), batch.take('C', Cg, tail, data.dtype)
     if state is not None:
         _param(what, 'state', state, (batch.B, width, N))
     _C.one_device(data, raw, A, Bg, Cg, D, gate, dt_bias, state, *batch.tensors())
-    inputs = (data, raw, A, Bg, Cg, D, gate, dt_bias, state)
-    want_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
-    y, last = _SelectiveScan.apply(batch, int(bool(dt_softplus)), want_grad, *inputs)
+    want_grad = torch.is_grad_enabled() and (
+        data.requires_grad or raw.requires_grad or A.requires_grad or Bg.requires_grad or Cg.requires_grad or (D is not None and D.requires_grad)
+        or (gate is not None and gate.requires_grad) or (dt_bias is not None and dt_bias.requires_grad) or (state is not None and state.requires_grad))
+    y, last = _SelectiveScan.apply(batch, int(bool(dt_softplus)), want_grad, data, raw, A, Bg, Cg, D, gate, dt_bias, state)
     return _like(x, y), last
 
 
