@@ -98,9 +98,11 @@ using ppk::uni_len;
 using ppk::uniform;
 
 constexpr int AHEAD = 4;                      // steps whose elements are loaded before those of the steps before them are used
-static_assert(1024 <= ppk::ONE_PASS_ROWS, "one launch adds them");
-constexpr int SUM_BLOCKS = 1024;              // blocks of a backward launch in all: each leaves a row of partial sums for its channels
-constexpr long long WANTED_WAVES = 8192;
+// Blocks of a backward launch in all, three a CU, what is resident together: each leaves a row of partial sums for its channels.  2048 x 20-100 x 512
+// fp32: 195 us, 199 with 1024, 258 with 2048 and shorter runs.
+constexpr int SUM_BLOCKS = 768;
+static_assert(SUM_BLOCKS <= ppk::ONE_PASS_ROWS, "one launch adds them");
+constexpr long long WANTED_WAVES = 8192;       // 16384 and half the run: the same, 32768: 5 % (fp32 batch) to 45 % (bf16 prompt) slower
 
 struct ConvArgs {
     SeqBatch q;
