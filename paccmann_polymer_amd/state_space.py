@@ -265,6 +265,10 @@ def _step_out(what, state, out, others):
     for t in others:
         if _overlap(t, out):
             raise ValueError(f'{what}: out shares memory with an input')
+    if out.requires_grad:
+        raise ValueError(f'{what}: out requires a gradient (training goes through the form for whole sequences)')
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)         # an autograd graph that saved it finds it changed
     return out
 
 

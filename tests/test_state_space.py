@@ -116,6 +116,13 @@ def test_step_out_may_be_the_state_and_nothing_else():
     state = torch.zeros(4, 3, D)
     assert S._step_out('f', state, None, ()).shape == state.shape
     assert S._step_out('f', state, state, ()) is state
+    seen = state._version
+    assert S._step_out('f', state, state, ()) is state and state._version == seen + 1
+    with torch.inference_mode():
+        frozen = torch.zeros(4, 3, D)
+    assert S._step_out('f', frozen, frozen, ()) is frozen
+    with pytest.raises(ValueError):
+        S._step_out('f', state, torch.zeros(4, 3, D, requires_grad=True), ())
     whole = torch.zeros(5, 3, D)
     for bad in (torch.zeros(4, 3, D + 1), torch.zeros(4, 3, D, dtype=torch.bfloat16), torch.zeros(4, D, 3).transpose(1, 2)):
         with pytest.raises(ValueError):
