@@ -17,10 +17,13 @@ using ppk::uni_len;
 using ppk::uniform;
 
 constexpr int TILE = 16;                     // steps between two kept states
-// Splits of the time axis: where the sequences and channels alone leave less than half of FWD_WAVES waves (BWD_BLOCKS blocks), a split takes
-// as many steps as make that many, and MIN_SPAN (BWD_MIN_SPAN) at least.  Measured: 1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with
-// 32, 50 with 16 (joining them eats the rest); 1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096;
-// 21 x 100 x 333 fp32 backward 45 us in one launch, 42 us in the three of a split.
+// Splits of the time axis: where the sequences and channels alone make less than a quarter of FWD_WAVES waves, one a SIMD (of BWD_BLOCKS blocks,
+// two a CU), a split takes as many steps as make that many, and MIN_SPAN (BWD_MIN_SPAN) at least.  Measured, 16 states:
+//   1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with 32, 50 with 16 (joining them eats the rest);
+//   64 x 256 x 1024 (1024 waves) fp32 forward 154 us in one piece, 170 in four splits; half the sequences 118 in one, 101 in eight;
+//   32 x 256 x 1024 (512 blocks) fp32 training 266 us with the backward pass in one piece, 321 in splits;
+//   1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096;
+//   21 x 100 x 333 fp32 backward 45 us in one launch, 42 in the three of a split.
 constexpr long long MIN_SPAN = 32, BWD_MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -75,18 +78,13 @@ template <int N> struct Scalars<bf16_t, N> {
         for (int n = 0; n < N / 2; ++n) v[n] = u[n]; }
     __device__ __forceinline__ float at(int n) const { return __uint_as_float(n & 1 ? v[n / 2] & 0xffff0000u : v[n / 2] << 16); }
 };
-// ... or any N at any alignment: lane n holds element n, zero from `count` on
-template <typename T, int N> struct Lanes {
-    float v;
-    __device__ __forceinline__ void load(const T* p, int lane, int count) { v = lane < count ? to_f32(p[lane]) : 0.f; }
-    __device__ __forceinline__ float at(int n) const { return lane_value(v, n); }
-};
-// SCALAR: a row's N == NP elements begin on 4 bytes everywhere
+// A step's B or C as the multiplications take it.  SCALAR: a row's N == NP elements begin on 4 bytes everywhere and are loaded as scalars, when
+// the step begins.  Otherwise any N at any alignment: lane n has loaded element n some steps ahead (the lanes from N on: zero) and hands it over.
 template <typename T, int NP, bool SCALAR> struct RowVec {
     Scalars<T, NP> s;
-    Lanes<T, NP> l;
-    __device__ __forceinline__ void load(const T* p, int lane, int count) { if constexpr (SCALAR) s.load(p); else l.load(p, lane, count); }
-    __device__ __forceinline__ float at(int n) const { if constexpr (SCALAR) return s.at(n); else return l.at(n); }
+    float v;
+    __device__ __forceinline__ void begin(const T* p, float ahead) { if constexpr (SCALAR) s.load(p); else v = ahead; }
+    __device__ __forceinline__ float at(int n) const { if constexpr (SCALAR) return s.at(n); else return lane_value(v, n); }
 };
 
 template <int NP> __device__ __forceinline__ void load_states(const float* p, int N, float (&h)[NP])
@@ -129,12 +127,10 @@ struct Item {
 };
 __device__ __forceinline__ long long carry_at(const ScanArgs& a, long long b, int s, int d) { return (b * a.splits + s) * a.D + d; }
 
-// Steps whose elements are loaded before those of the steps before them are used.  1 x 2048 x 1024 bf16, 16 states: 25.3 us with 2, 24.0 with 4,
-// 21.8 with 8; with more than 16 states eight steps' elements no longer fit beside the states.
-constexpr int ahead(int states) { return states <= 16 ? 8 : 4; }
+constexpr int AHEAD = 4;                       // steps whose elements are loaded before those of the steps before them are used (2: 5 % slower, 8: the same)
 
 // rows of AHEAD steps from t on, in direction dir, none behind `last`
-template <int AHEAD> __device__ __forceinline__ void rows_of(const SeqBatch& q, int t, int last, int dir, unsigned (&rows)[AHEAD])
+__device__ __forceinline__ void rows_of(const SeqBatch& q, int t, int last, int dir, unsigned (&rows)[AHEAD])
 {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) { const int u = t + dir * i; rows[i] = (unsigned)(dir > 0 ? (u < last ? u : last) : (u > last ? u : last)); }
@@ -148,7 +144,6 @@ template <int AHEAD> __device__ __forceinline__ void rows_of(const SeqBatch& q, 
 template <typename T, int NP, bool SCALAR, bool PART>
 __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 {
-    constexpr int AHEAD = ahead(NP);
     const Item it(a);
     const int lane = threadIdx.x, N = a.N;
     const int len = it.len, t0 = it.t0, t1 = it.t1;
@@ -169,12 +164,16 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     const Rows<T> Bs(a.Bm, it.b * a.Bs.b + it.g * a.Bg, a.Bs.t), Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t), ys(a.y, it.b * a.rows.b * a.D, a.rows.t * a.D);
     const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
     const bool gate = !PART && a.z;
-    T xv[AHEAD], rv[AHEAD], zv[AHEAD];
+    T xv[AHEAD], rv[AHEAD], zv[AHEAD], bv[AHEAD], cv[AHEAD];
     unsigned rows[AHEAD];
+    const unsigned own = (lane < N ? lane : 0) * (unsigned)sizeof(T);
     const auto fetch = [&](int t) {            // steps t, t + 1, ...; behind the last one, the last one
         rows_of(a.q, t, t1 - 1, 1, rows);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) { xv[i] = xs.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
+        if (!SCALAR)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) { bv[i] = Bs.get(rows[i], own); if (!PART) cv[i] = Cs.get(rows[i], own); }
         if (gate)
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) zv[i] = zs.get(rows[i], d);
@@ -183,16 +182,19 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; t += AHEAD) {
         if (!PART && kept && t % TILE == 0) { store_states<NP>(kept, N, h); kept += tile_size; }
-        float x[AHEAD], raw[AHEAD], z[AHEAD];
+        float x[AHEAD], raw[AHEAD], z[AHEAD], bl[AHEAD], cl[AHEAD];
         unsigned r[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) { x[i] = to_f32(xv[i]); raw[i] = to_f32(rv[i]) + bias; z[i] = gate ? to_f32(zv[i]) : 0.f; r[i] = rows[i]; }
+        for (int i = 0; i < AHEAD; ++i) {
+            bl[i] = !SCALAR && lane < N ? to_f32(bv[i]) : 0.f;
+            cl[i] = !SCALAR && !PART && lane < N ? to_f32(cv[i]) : 0.f;
+            x[i] = to_f32(xv[i]); raw[i] = to_f32(rv[i]) + bias; z[i] = gate ? to_f32(zv[i]) : 0.f; r[i] = rows[i]; }
         if (t + AHEAD < t1) fetch(t + AHEAD);
         const auto step = [&](int i) {
             __builtin_amdgcn_sched_barrier(0);     // one step's scalars at a time: those of all do not fit
             RowVec<T, NP, SCALAR> Bv, Cv;
-            Bv.load((const T*)Bs.row(r[i]), lane, N);
-            if (!PART) Cv.load((const T*)Cs.row(r[i]), lane, N);
+            Bv.begin((const T*)Bs.row(r[i]), bl[i]);
+            if (!PART) Cv.begin((const T*)Cs.row(r[i]), cl[i]);
             const float dt = a.softplus ? softplus(raw[i]) : raw[i], dx = dt * x[i];
             float y[4] = {skip * x[i], 0.f, 0.f, 0.f};
 #pragma unroll
@@ -225,7 +227,6 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 template <typename T, int NP, bool SCALAR>
 __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 {
-    constexpr int AHEAD = ahead(NP);
     const Item it(a);
     const int lane = threadIdx.x, N = a.N;
     const int t0 = it.t0, t1 = it.t1;
@@ -238,12 +239,13 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     const Rows<T> ds(a.dy, it.b * a.dys.b, a.dys.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
     const Rows<T> Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t);
     const unsigned d = (unsigned)it.d * (unsigned)sizeof(T);
-    T dv[AHEAD], rv[AHEAD], zv[AHEAD];
+    T dv[AHEAD], rv[AHEAD], zv[AHEAD], cv[AHEAD];
     unsigned rows[AHEAD];
+    const unsigned own = (lane < N ? lane : 0) * (unsigned)sizeof(T);
     const auto fetch = [&](int t) {            // steps t - 1, t - 2, ...; before the first one, the first one
         rows_of(a.q, t - 1, t0, -1, rows);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) { dv[i] = ds.get(rows[i], d); rv[i] = rs.get(rows[i], d); }
+        for (int i = 0; i < AHEAD; ++i) { dv[i] = ds.get(rows[i], d); rv[i] = rs.get(rows[i], d); if (!SCALAR) cv[i] = Cs.get(rows[i], own); }
         if (a.z)
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) zv[i] = zs.get(rows[i], d);
@@ -251,10 +253,11 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     float sum = 0.f;
     fetch(t1);
     for (int t = t1; t > t0; t -= AHEAD) {
-        float dy[AHEAD], raw[AHEAD];
+        float dy[AHEAD], raw[AHEAD], cl[AHEAD];
         unsigned r[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
+            cl[i] = !SCALAR && lane < N ? to_f32(cv[i]) : 0.f;
             const float z = a.z ? to_f32(zv[i]) : 0.f;
             dy[i] = to_f32(dv[i]) * (a.z ? z * sigmoid(z) : 1.0f);
             raw[i] = to_f32(rv[i]) + bias;
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
         const auto step = [&](int i) {
             __builtin_amdgcn_sched_barrier(0);
             RowVec<T, NP, SCALAR> Cv;
-            Cv.load((const T*)Cs.row(r[i]), lane, N);
+            Cv.begin((const T*)Cs.row(r[i]), cl[i]);
             const float dt = a.softplus ? softplus(raw[i]) : raw[i];
             sum += dt;
 #pragma unroll
@@ -607,7 +610,7 @@ int padded(long long N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; 
 long long span_of(long long T, long long units, long long want, long long least)
 {
     const long long all = ceil_div(T > 0 ? T : 1, TILE) * TILE;
-    if (units * 2 > want || all <= 2 * least) return all;
+    if (units * 4 >= want || all <= 2 * least) return all;
     const long long span = ceil_div(ceil_div(all * units, want), TILE) * TILE;
     return span > least ? span : least;
 }
