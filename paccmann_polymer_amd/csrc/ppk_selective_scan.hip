@@ -19,12 +19,13 @@ using ppk::uniform;
 constexpr int TILE = 16;                     // steps between two kept states
 // Splits of the time axis: where the sequences and channels alone make less than a quarter of FWD_WAVES waves, one a SIMD (of BWD_BLOCKS blocks,
 // two a CU), a split takes as many steps as make that many, and MIN_SPAN (BWD_MIN_SPAN) at least.  Measured, 16 states:
-//   1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 50 with 32, 50 with 16 (joining them eats the rest);
+//   1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 48 with 32, 47 with 16 (joining them eats the rest);
+//   21 x 100 x 333 fp32 forward 41 us with 32 steps at least, 28 with 16;
 //   64 x 256 x 1024 (1024 waves) fp32 forward 154 us in one piece, 170 in four splits; half the sequences 118 in one, 101 in eight;
 //   32 x 256 x 1024 (512 blocks) fp32 training 266 us with the backward pass in one piece, 321 in splits;
 //   1 x 16384 x 2048 bf16 training 1070 us with 1024 blocks, 1030 with 2048, 1050 with 4096;
 //   21 x 100 x 333 fp32 backward 45 us in one launch, 42 in the three of a split.
-constexpr long long MIN_SPAN = 32, BWD_MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
+constexpr long long MIN_SPAN = 16, BWD_MIN_SPAN = 64, FWD_WAVES = 4096, BWD_BLOCKS = 2048;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct ScanArgs {
@@ -87,14 +88,25 @@ template <typename T, int NP, bool SCALAR> struct RowVec {
     __device__ __forceinline__ float at(int n) const { if constexpr (SCALAR) return s.at(n); else return lane_value(v, n); }
 };
 
-template <int NP> __device__ __forceinline__ void load_states(const float* p, int N, float (&h)[NP])
+// a lane's N states; `wide`: N == NP and they begin on 16 bytes in every lane
+template <int NP> __device__ __forceinline__ void load_states(const float* p, int N, bool wide, float (&h)[NP])
 {
+    if (wide) {
 #pragma unroll
-    for (int n = 0; n < NP; ++n) h[n] = n < N ? p[n] : 0.f;
+        for (int n = 0; n < NP; n += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + n);
+            h[n] = v.x; h[n + 1] = v.y; h[n + 2] = v.z; h[n + 3] = v.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) h[n] = p[n < N ? n : 0];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) h[n] = n < N ? h[n] : 0.f;
 }
-template <int NP> __device__ __forceinline__ void store_states(float* p, int N, const float (&h)[NP])
+template <int NP> __device__ __forceinline__ void store_states(float* p, int N, bool wide, const float (&h)[NP])
 {
-    if (N == NP && ((uintptr_t)p & 15) == 0) {
+    if (wide) {
 #pragma unroll
         for (int n = 0; n < NP; n += 4) *reinterpret_cast<float4*>(p + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
         return;
@@ -103,6 +115,7 @@ template <int NP> __device__ __forceinline__ void store_states(float* p, int N, 
     for (int n = 0; n < NP; ++n)
         if (n < N) p[n] = h[n];
 }
+template <int NP> __device__ __forceinline__ bool wide_states(const void* p, int N) { return N == NP && ((uintptr_t)p & 15) == 0; }      // of an array's base
 
 // What a wave of the kernels with a lane a channel works on: 64 channels of a group of one sequence, one split of its steps
 struct Item {
@@ -150,15 +163,19 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     if (t0 >= len && it.s > 0) return;
     if (PART && t1 >= len) return;             // nothing enters a split behind the last
     float A2[NP], h[NP];
-    load_states<NP>(a.A + (long long)it.d * N, N, A2);
+    load_states<NP>(a.A + (long long)it.d * N, N, wide_states<NP>(a.A, N), A2);
     if (PART || (a.splits == 1 && !a.state)) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) h[n] = 0.f;
-    } else load_states<NP>(a.splits > 1 ? a.carry + carry_at(a, it.b, it.s, it.d) * N : a.state + (it.b * a.D + it.d) * N, N, h);
+    } else {
+        const float* from = a.splits > 1 ? a.carry : a.state;
+        load_states<NP>(from + (a.splits > 1 ? carry_at(a, it.b, it.s, it.d) : it.b * a.D + it.d) * N, N, wide_states<NP>(from, N), h);
+    }
 #pragma unroll
     for (int n = 0; n < NP; ++n) A2[n] = base2(A2[n]);
     const float skip = !PART && a.skip ? a.skip[it.d] : 0.f, bias = a.bias ? a.bias[it.d] : 0.f;
     const long long tile_size = (long long)a.D * N;
+    const bool kept_wide = wide_states<NP>(a.kept, N);
     float* kept = a.kept ? a.kept + ((first_tile(a, it.b) + t0 / TILE) * a.D + it.d) * N : nullptr;
     const Rows<T> xs(a.x, it.b * a.xs.b, a.xs.t), rs(a.raw, it.b * a.raws.b, a.raws.t), zs(a.z, it.b * a.zs.b, a.zs.t);
     const Rows<T> Bs(a.Bm, it.b * a.Bs.b + it.g * a.Bg, a.Bs.t), Cs(a.Cm, it.b * a.Cs.b + it.g * a.Cg, a.Cs.t), ys(a.y, it.b * a.rows.b * a.D, a.rows.t * a.D);
@@ -181,7 +198,7 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
     float sum = 0.f;
     if (t0 < t1) fetch(t0);
     for (int t = t0; t < t1; t += AHEAD) {
-        if (!PART && kept && t % TILE == 0) { store_states<NP>(kept, N, h); kept += tile_size; }
+        if (!PART && kept && t % TILE == 0) { store_states<NP>(kept, N, kept_wide, h); kept += tile_size; }
         float x[AHEAD], raw[AHEAD], z[AHEAD], bl[AHEAD], cl[AHEAD];
         unsigned r[AHEAD];
 #pragma unroll
@@ -217,9 +234,9 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
         }
     }
     if (PART) {
-        store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, h);
+        store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, wide_states<NP>(a.carry, N), h);
         a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
-    } else if (t1 == len) store_states<NP>(a.last + (it.b * a.D + it.d) * N, N, h);
+    } else if (t1 == len) store_states<NP>(a.last + (it.b * a.D + it.d) * N, N, wide_states<NP>(a.last, N), h);
 }
 
 // What the gradient of the state at the end of a split becomes at its beginning, without what enters at the end: g = a (g + dy' C),
@@ -232,7 +249,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
     const int t0 = it.t0, t1 = it.t1;
     if (t0 >= it.len || it.s == 0) return;     // nothing leaves the first
     float A2[NP], g[NP];
-    load_states<NP>(a.A + (long long)it.d * N, N, A2);
+    load_states<NP>(a.A + (long long)it.d * N, N, wide_states<NP>(a.A, N), A2);
 #pragma unroll
     for (int n = 0; n < NP; ++n) { A2[n] = base2(A2[n]); g[n] = 0.f; }
     const float bias = a.bias ? a.bias[it.d] : 0.f;
@@ -282,7 +299,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
                 if (t - 1 - i >= t0) step(i);
         }
     }
-    store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, g);
+    store_states<NP>(a.carry + carry_at(a, it.b, it.s, it.d) * N, N, wide_states<NP>(a.carry, N), g);
     a.sdt[carry_at(a, it.b, it.s, it.d)] = sum;
 }
 
@@ -301,23 +318,28 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
     float in = from ? from[b * dn + e] : 0.f;
     float* c = a.carry + b * a.splits * dn + e;
     const float* sd = a.sdt + b * a.splits * (long long)a.D + d;
-    constexpr int U = 8;
-    for (int k0 = 0; k0 < used; k0 += U) {
-        float own[U], sum[U];
+    // Parts of U splits are loaded together and their decays made before the chain that joins them, which is then a product, a sum and a store
+    // each.  The part of the last split on the way (forward the sequence's last, backward its first) is not made: nobody asks for it.
+    constexpr int U = 16;
+    const int dir = REV ? -1 : 1;
+    const long long cs = dir * dn, ss = dir * (long long)a.D;
+    if (REV) { c += (used - 1) * dn; sd += (long long)(used - 1) * a.D; }
+    int k0 = 0;
+    for (; k0 + U < used; k0 += U) {
+        float own[U], by[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            const int s = REV ? used - 1 - (k0 + i) : k0 + i;
-            const bool has = k0 + i < used && (REV ? s > 0 : s < used - 1);        // the last one's own part is not made
-            own[i] = has ? c[s * dn] : 0.f;
-            sum[i] = has ? sd[(long long)s * a.D] : 0.f;
-        }
+        for (int i = 0; i < U; ++i) { own[i] = c[i * cs]; by[i] = sd[i * ss]; }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            if (k0 + i >= used) break;
-            const int s = REV ? used - 1 - (k0 + i) : k0 + i;
-            c[s * dn] = in;
-            in = fmaf(exp2_(sum[i] * A2), in, own[i]);
-        }
+        for (int i = 0; i < U; ++i) by[i] = exp2_(by[i] * A2);
+#pragma unroll
+        for (int i = 0; i < U; ++i) { c[i * cs] = in; in = fmaf(by[i], in, own[i]); }
+        c += U * cs;
+        sd += U * ss;
+    }
+    for (; k0 < used; ++k0, c += cs, sd += ss) {
+        const float own = k0 + 1 < used ? *c : 0.f, decay = exp2_(k0 + 1 < used ? *sd * A2 : 0.f);
+        *c = in;
+        in = fmaf(decay, in, own);
     }
 }
 
