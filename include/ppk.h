@@ -290,7 +290,7 @@ int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void*
  * receives the state before every ppk_selective_scan_tile() steps of each sequence; tiles [B + 1] (device; NULL for a rectangular batch):
  * the first of them of each sequence and their number.
  * strides_host [16]: x, raw (two each), B, C (step, sequence, group), z (two), the outputs in ROWS of their width (two), dy (two).
- * Fewer than 2^31 steps and rows; the rows of a step's tensors fewer than 2^30 elements apart.
+ * Fewer than 2^30 steps and 2^31 rows; the rows of a step's tensors fewer than 2^30 elements apart.
  * y, dx, draw, dz [rows, D], dB, dC [rows, G, N].  bwd overwrites all its outputs; dskip, dbias, dstate may be NULL. */
 int64_t ppk_selective_scan_tile(void);
 size_t ppk_selective_scan_fwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G);      /* 0 where none is needed */

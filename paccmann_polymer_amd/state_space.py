@@ -27,6 +27,7 @@ _lib = _C.lib
 MAX_TAPS = 8
 MAX_STATES = 64
 FAR_ROWS = 1 << 30                 # the kernels take rows that are fewer elements apart; others are copied
+MAX_ROWS = 1 << 31                 # the kernels count rows in 32 bits
 
 
 class PackedRows(NamedTuple):
@@ -51,6 +52,8 @@ def packed_rows(batch_sizes, device, sequences: Optional[int] = None) -> PackedR
     B = int(bs[0]) if T else 0
     if T and (int(bs.min()) < 1 or bool((bs[1:] > bs[:-1]).any())):
         raise ValueError('packed_rows: batch sizes must be positive and must not increase')
+    if T and int(bs.sum()) >= MAX_ROWS:
+        raise ValueError(f'packed_rows: {int(bs.sum())} rows (fewer than 2^31 are supported)')
     if sequences is not None:
         if int(sequences) < B:
             raise ValueError(f'packed_rows: {int(sequences)} sequences, but {B} have a first step')

@@ -36,6 +36,13 @@ def test_packed_rows_refuses(sizes):
         S.packed_rows(torch.tensor([4, 2]), 'cpu', sequences=3)
 
 
+def test_packed_rows_refuses_more_rows_than_the_kernels_count():
+    with pytest.raises(ValueError, match='rows'):
+        S.packed_rows(torch.full((2,), 2 ** 30), 'cpu')
+    with pytest.raises(ValueError, match='rows'):
+        S.packed_rows(torch.full((2 ** 12,), 2 ** 20 + 1), 'cpu')
+
+
 def conv_args(**change):
     a = dict(x=torch.zeros(T, B, D), weight=torch.zeros(D, K), bias=torch.zeros(D))
     a.update(change)
