@@ -101,7 +101,7 @@ class _Batch:
             self.rows = self.T * self.B
             self.lead = (self.T, self.B)
             # outputs lie as x does: batch-first where a sequence's steps are next to each other
-            self.batch_first = data.stride(0) < data.stride(1)
+            self.batch_first = self.T == 1 or data.stride(0) < data.stride(1)
             self.out_rows = (1, self.T) if self.batch_first else (self.B, 1)
         self.D = data.shape[-1]
         if self.D < 1:
@@ -119,11 +119,13 @@ class _Batch:
         return t if s[0] < FAR_ROWS and s[1] < FAR_ROWS and (s[-1] == 1 or t.shape[-1] == 1) else t.contiguous()
 
     def strides(self, t):
-        """Of a step and of a sequence, in elements."""
+        """Of a step and of a sequence, in elements; of the only one, whatever the tensor says, 0."""
         if t is None:
             return 0, 0
         s = t.stride()
-        return (s[0], s[0]) if self.plan is not None else s[:2]
+        if self.plan is not None:
+            return (s[0], s[0]) if self.rows > 1 else (0, 0)
+        return s[0] if self.T > 1 else 0, s[1] if self.B > 1 else 0
 
     def new(self, tail, like):
         """An uninitialised per-step tensor of the type and device of `like`, laid out as x is."""

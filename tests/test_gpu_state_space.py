@@ -465,3 +465,34 @@ def test_infinities_stay_where_the_formula_has_them(T):
     w = torch.randn(20, 4, device=DEV)
     y4, y5 = causal_conv(c['x'], w, plan=lay.plan)[0], causal_conv(t['x'], w, plan=lay.plan)[0]
     assert torch.equal(y4[keep], y5[keep])
+
+
+@pytest.mark.parametrize('shape', [(1, 3), (4, 1), (1, 1)])
+def test_the_only_step_or_sequence_may_have_any_stride(shape):
+    """What a slice of one step (sequence) of a far larger tensor hands over; only the strides that are walked count."""
+    from paccmann_polymer_amd.state_space import causal_conv, selective_scan
+    g = torch.Generator(device=DEV).manual_seed(11)
+    T, B, D, N = *shape, 12, 8
+
+    def far(t):
+        s = list(t.stride())
+        for i in range(2):
+            if t.shape[i] == 1:
+                s[i] = 2 ** 33
+        return t.as_strided(t.shape, s)
+    x, dt, Bm, C, z = (randn(g, T, B, n, scale=0.5) for n in (D, D, N, N, D))
+    w, A = randn(g, D, 4), -randn(g, D, N).abs()
+    for near, away in zip(causal_conv(x, w), causal_conv(far(x), w)):
+        assert torch.equal(near, away)
+    near, away = [], []
+    for got, f in ((near, lambda t: t), (away, far)):
+        leaves = [v.detach().requires_grad_() for v in (x, dt, Bm, C, z)]
+        y, last = selective_scan(f(leaves[0]), f(leaves[1]), A, f(leaves[2]), f(leaves[3]), z=f(leaves[4]))
+        got += [y, last, *torch.autograd.grad(y.square().sum() + last.sum(), leaves)]
+    for a, b in zip(near, away):
+        assert torch.equal(a, b)
+    # rows of a packed batch of one row
+    from paccmann_polymer_amd.state_space import packed_rows
+    row = x[:1, 0]
+    plan = packed_rows(torch.ones(1, dtype=torch.int64), DEV)
+    assert torch.equal(causal_conv(row, w, plan=plan)[0], causal_conv(row.as_strided((1, D), (2 ** 33, 1)), w, plan=plan)[0])
