@@ -8,12 +8,13 @@
 namespace ppk {
 
 namespace {
-// grid (column block of 256, chunk of PS_ROWS rows)
-__global__ __launch_bounds__(256) void k_ps_part(const float* __restrict__ part, long long P, long long C, double* __restrict__ out)
+// a block: 256 columns of a chunk of PS_ROWS rows
+__global__ __launch_bounds__(256) void k_ps_part(const float* __restrict__ part, long long P, long long C, unsigned column_blocks, double* __restrict__ out)
 {
-    const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
+    const unsigned chunk = blockIdx.x / column_blocks;
+    const long long c = (long long)(blockIdx.x - chunk * column_blocks) * 256 + threadIdx.x;
     if (c >= C) return;
-    const long long p0 = (long long)blockIdx.y * PS_ROWS, p1 = p0 + PS_ROWS < P ? p0 + PS_ROWS : P;
+    const long long p0 = (long long)chunk * PS_ROWS, p1 = p0 + PS_ROWS < P ? p0 + PS_ROWS : P;
     double s = 0;
     long long p = p0;
     for (; p + 8 <= p1; p += 8) {
@@ -24,7 +25,7 @@ __global__ __launch_bounds__(256) void k_ps_part(const float* __restrict__ part,
         for (int k = 0; k < 8; ++k) s += (double)v[k];
     }
     for (; p < p1; ++p) s += (double)part[p * C + c];
-    out[(long long)blockIdx.y * C + c] = s;
+    out[(long long)chunk * C + c] = s;
 }
 __global__ __launch_bounds__(256) void k_ps_final(const double* __restrict__ part, int n, long long C, float* __restrict__ out)
 {
@@ -78,7 +79,7 @@ int partial_sums(const SumJob* jobs, int count, void* ws, hipStream_t stream)
         if (j.C <= 0 || !j.out) continue;
         if (j.P <= ONE_PASS_ROWS) { small.job[small.n++] = j; widest = j.C > widest ? j.C : widest; continue; }
         const unsigned cb = (unsigned)((j.C + 255) / 256), chunks = (unsigned)((j.P + PS_ROWS - 1) / PS_ROWS);
-        k_ps_part<<<dim3(cb, chunks), 256, 0, stream>>>(j.part, j.P, j.C, (double*)ws);
+        k_ps_part<<<cb * chunks, 256, 0, stream>>>(j.part, j.P, j.C, cb, (double*)ws);
         k_ps_final<<<cb, 256, 0, stream>>>((const double*)ws, (int)chunks, j.C, j.out);
     }
     if (small.n) k_ps_one<<<dim3((unsigned)((widest + 63) / 64), (unsigned)small.n), 1024, 0, stream>>>(small);

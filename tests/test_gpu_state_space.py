@@ -496,3 +496,21 @@ def test_the_only_step_or_sequence_may_have_any_stride(shape):
     row = x[:1, 0]
     plan = packed_rows(torch.ones(1, dtype=torch.int64), DEV)
     assert torch.equal(causal_conv(row, w, plan=plan)[0], causal_conv(row.as_strided((1, D), (2 ** 33, 1)), w, plan=plan)[0])
+
+
+def test_more_sequences_than_a_grid_has_rows():
+    """4.3 million sequences of a step each: their sums take more chunks than 65535."""
+    from paccmann_polymer_amd.state_space import selective_scan
+    g = torch.Generator(device=DEV).manual_seed(12)
+    B = 4_300_000
+    x, dt, Bm, C = (randn(g, 1, B, 1, scale=0.5) for _ in range(4))
+    A = torch.full((1, 1), -1.0, device=DEV, requires_grad=True)
+    D = torch.ones(1, device=DEV, requires_grad=True)
+    y, last = selective_scan(x, dt, A, Bm, C, D=D)
+    s = torch.nn.functional.softplus(dt.double())
+    h = s * x.double() * Bm.double()
+    close(y, C.double() * h + x.double(), 40 * H * (C.double() * h).abs() + 3 * H * x.double().abs())
+    dA, dD = torch.autograd.grad(y.sum(), (A, D))
+    assert float(dA) == 0.0                        # no state before the first step
+    xs = x.double()
+    assert abs(float(dD) - float(xs.sum())) <= 2 * H * float(xs.abs().sum())
