@@ -354,6 +354,9 @@ template <int LPC> __device__ __forceinline__ float sum_slices(float v)
 }
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+// Parts of a tile: a sequence's last tile is worked on as far as the part that its last step is in.  2048 sequences of 20 to 100 steps, 512 channels,
+// 16 states, fp32: 1175 us, 1223 with whole tiles; 21 of 1 to 100 steps, 333 channels: 43 and 46.  Five and eight parts: the same.
+constexpr int NPARTS = 3, PARTS[NPARTS + 1] = {0, 5, 10, TILE};
 
 // The backward pass.  A block takes 256 / LPC channels of a group of one sequence and walks a split's tiles backwards; a thread holds the
 // four states 4 slice .. of a channel.  In a wave, lane % 16 = slice * (16 / LPC) + low bits of the channel, lane / 16 = its high bits:
@@ -469,53 +472,61 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
         locate(next);
         __syncthreads();
 #pragma unroll
-        for (int t = 0; t < TILE; ++t) {
-            const float dtv = s_dt[t][ch], dxv = s_dx[t][ch];
-            const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]);
+        for (int part = 0; part < NPARTS; ++part) {
+            if (PARTS[part] >= steps) break;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                av[t][j] = exp2_(dtv * A2[j]);
-                h[t + 1][j] = fmaf(av[t][j], h[t][j], dxv * Bv[j]);
+            for (int t = PARTS[part]; t < PARTS[part + 1]; ++t) {
+                const float dtv = s_dt[t][ch], dxv = s_dx[t][ch];
+                const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    av[t][j] = exp2_(dtv * A2[j]);
+                    h[t + 1][j] = fmaf(av[t][j], h[t][j], dxv * Bv[j]);
+                }
             }
         }
         asm volatile("" ::: "memory");           // the steps' values are read from LDS again: kept, they would be 96 registers
 #pragma unroll
-        for (int t = TILE - 1; t >= 0; --t) {
-            if (t == TILE - 6) fetch(next);                                     // where the registers of five steps are free again
-            const float dtv = s_dt[t][ch], dxv = s_dx[t][ch], dyv = s_dy[t][ch];
-            const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]), Cv = *reinterpret_cast<const f32x4*>(&s_BC[t][NP + ns * 4]);
-            float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
+        for (int part = NPARTS - 1; part >= 0; --part) {
+            if (part == NPARTS - 2) fetch(next);                                // where the registers of a part's steps are free again
+            if (PARTS[part] >= steps) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                dh[j] = fmaf(dyv, Cv[j], dh[j]);
-                q1 = fmaf(dh[j], Bv[j], q1);
-                v[j] = dh[j] * dxv;
-                v[4 + j] = dyv * h[t + 1][j];
-                q3 = fmaf(Cv[j], h[t + 1][j], q3);
-                dh[j] *= av[t][j];
-                const float da = dh[j] * h[t][j];
-                q2 = fmaf(da, A2[j], q2);
-                dA[j] = fmaf(da, dtv, dA[j]);
-            }
-            q1 = sum_slices<LPC>(q1);
-            q2 = sum_slices<LPC>(q2);
-            q3 = sum_slices<LPC>(q3);
-            s_q[ns & 3][t][ch] = (ns & 3) == 0 ? q1 : (ns & 3) == 1 ? q2 : q3;   // every slice holds all three: the fourth writes nobody's
-            // over the wave's channels: two exchanges of halves leave a lane the sums of two of the eight values (bit 5 of the lane: dC,
-            // bit 4: the upper two states), the low bits of the channel follow within a row of 16
-            float u[4], w[2];
+            for (int t = PARTS[part + 1] - 1; t >= PARTS[part]; --t) {
+                const float dtv = s_dt[t][ch], dxv = s_dx[t][ch], dyv = s_dy[t][ch];
+                const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]), Cv = *reinterpret_cast<const f32x4*>(&s_BC[t][NP + ns * 4]);
+                float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(v[k + 4]), false, false);
-                u[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-            }
+                for (int j = 0; j < 4; ++j) {
+                    dh[j] = fmaf(dyv, Cv[j], dh[j]);
+                    q1 = fmaf(dh[j], Bv[j], q1);
+                    v[j] = dh[j] * dxv;
+                    v[4 + j] = dyv * h[t + 1][j];
+                    q3 = fmaf(Cv[j], h[t + 1][j], q3);
+                    dh[j] *= av[t][j];
+                    const float da = dh[j] * h[t][j];
+                    q2 = fmaf(da, A2[j], q2);
+                    dA[j] = fmaf(da, dtv, dA[j]);
+                }
+                q1 = sum_slices<LPC>(q1);
+                q2 = sum_slices<LPC>(q2);
+                q3 = sum_slices<LPC>(q3);
+                s_q[ns & 3][t][ch] = (ns & 3) == 0 ? q1 : (ns & 3) == 1 ? q2 : q3;   // every slice holds all three: the fourth writes nobody's
+                // over the wave's channels: two exchanges of halves leave a lane the sums of two of the eight values (bit 5 of the lane: dC,
+                // bit 4: the upper two states), the low bits of the channel follow within a row of 16
+                float u[4], w[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[k + 2]), false, false);
-                w[k] = lanes_sum<CL>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+                for (int k = 0; k < 4; ++k) {
+                    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[k]), __float_as_uint(v[k + 4]), false, false);
+                    u[k] = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(u[k]), __float_as_uint(u[k + 2]), false, false);
+                    w[k] = lanes_sum<CL>(__uint_as_float(p[0]) + __uint_as_float(p[1]));
+                }
+                // CL lanes hold the same two sums and store them to the same place
+                *reinterpret_cast<f32x2*>(&s_red[t][wave][(lane >> 5) * NP + ns * 4 + ((lane >> 4) & 1) * 2]) = f32x2{w[0], w[1]};
             }
-            // CL lanes hold the same two sums and store them to the same place
-            *reinterpret_cast<f32x2*>(&s_red[t][wave][(lane >> 5) * NP + ns * 4 + ((lane >> 4) & 1) * 2]) = f32x2{w[0], w[1]};
         }
         __syncthreads();
 #pragma unroll
