@@ -305,41 +305,61 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 
 // Joins the splits of a sequence: carry[s] holds what split s gives alone and receives what enters it.  Forward from the state before
 // the first step, backward (REV) from the gradient of the state behind the last; a thread a state.
-template <bool REV>
+constexpr int JOIN_STATES = 32;
+template <bool REV, int U>
 __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
 {
-    const long long dn = (long long)a.D * a.N, e = (long long)blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
-    if (e >= dn) return;
+    constexpr int S = 256 / JOIN_STATES;                             // slices of the splits; U of a slice's are held at once
+    __shared__ float s_end[S][JOIN_STATES], s_decay[S][JOIN_STATES];
+    const int slice = threadIdx.x / JOIN_STATES, el = threadIdx.x % JOIN_STATES;
+    const long long dn = (long long)a.D * a.N, e0 = (long long)blockIdx.x * JOIN_STATES + el, b = blockIdx.y;
+    const bool live = e0 < dn;
+    const long long e = live ? e0 : 0;
     const int d = (int)(e / a.N);
     const float A2 = base2(a.A[e]);
     const float* from = REV ? a.dlast : a.state;
     const long long len = uni_len(a.q, b);
     const int used = len > 0 ? (int)((len + a.span - 1) / a.span) : 1;          // no steps: the first split still hands on what enters it
     float in = from ? from[b * dn + e] : 0.f;
-    float* c = a.carry + b * a.splits * dn + e;
-    const float* sd = a.sdt + b * a.splits * (long long)a.D + d;
-    // Parts of U splits are loaded together and their decays made before the chain that joins them, which is then a product, a sum and a store
-    // each.  The part of the last split on the way (forward the sequence's last, backward its first) is not made: nobody asks for it.
-    constexpr int U = 16;
-    const int dir = REV ? -1 : 1;
-    const long long cs = dir * dn, ss = dir * (long long)a.D;
-    if (REV) { c += (used - 1) * dn; sd += (long long)(used - 1) * a.D; }
-    int k0 = 0;
-    for (; k0 + U < used; k0 += U) {
-        float own[U], by[U];
+    const long long dir = REV ? -1 : 1, first = b * a.splits + (REV ? used - 1 : 0);
+    float* c = a.carry + first * dn + e;
+    const float* sd = a.sdt + first * a.D + d;
+    for (int k0 = 0; k0 < used; k0 += S * U) {
+        const int many = used - k0 < S * U ? used - k0 : S * U, per = (many + S - 1) / S, k1 = k0 + slice * per;
+        const int n = many - slice * per < per ? many - slice * per : per;      // 0 or less: nothing left for this slice
+        float own[U], by[U], end = 0.f, decay = 1.f;
+        // The part of the last split on the way (forward the sequence's last, backward its first) is not made: nobody asks for it.  Loads are
+        // not masked, so that all of them fly together: one behind the last made is that one again.
+        const int last = used > 1 ? used - 2 : 0;
 #pragma unroll
-        for (int i = 0; i < U; ++i) { own[i] = c[i * cs]; by[i] = sd[i * ss]; }
+        for (int i = 0; i < U; ++i) {
+            const int k = k1 + i < last ? k1 + i : last;
+            own[i] = c[dir * k * dn];
+            by[i] = sd[dir * k * a.D];
+        }
 #pragma unroll
-        for (int i = 0; i < U; ++i) by[i] = exp2_(by[i] * A2);
+        for (int i = 0; i < U; ++i) {
+            const bool made = i < n && k1 + i + 1 < used;
+            own[i] = made ? own[i] : 0.f;
+            by[i] = made ? exp2_(by[i] * A2) : 1.f;
+            end = fmaf(by[i], end, own[i]);
+            decay *= by[i];
+        }
+        s_end[slice][el] = end;
+        s_decay[slice][el] = decay;
+        __syncthreads();
+        float mine = in;
 #pragma unroll
-        for (int i = 0; i < U; ++i) { c[i * cs] = in; in = fmaf(by[i], in, own[i]); }
-        c += U * cs;
-        sd += U * ss;
-    }
-    for (; k0 < used; ++k0, c += cs, sd += ss) {
-        const float own = k0 + 1 < used ? *c : 0.f, decay = exp2_(k0 + 1 < used ? *sd * A2 : 0.f);
-        *c = in;
-        in = fmaf(decay, in, own);
+        for (int k = 0; k < S; ++k) {
+            if (k == slice) mine = in;
+            in = fmaf(s_decay[k][el], in, s_end[k][el]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (live && i < n) c[dir * (k1 + i) * dn] = mine;
+            mine = fmaf(by[i], mine, own[i]);
+        }
+        __syncthreads();
     }
 }
 
@@ -694,6 +714,12 @@ template <typename T> void run_bwd_part(const ScanArgs& a, unsigned blocks, hipS
         default: k_scan_bwd_part<T, 64, false><<<blocks, 64, 0, st>>>(a);
     }
 }
+template <bool REV> void join(const ScanArgs& a, long long B, hipStream_t st)
+{
+    const dim3 grid((unsigned)ceil_div((long long)a.D * a.N, JOIN_STATES), (unsigned)B);
+    if (a.splits <= 4 * 256 / JOIN_STATES) k_scan_join<REV, 4><<<grid, 256, 0, st>>>(a);
+    else k_scan_join<REV, 16><<<grid, 256, 0, st>>>(a);
+}
 template <typename T> void run_bwd(const ScanArgs& a, unsigned blocks, hipStream_t st)
 {
     switch (bwd_slices(a.N)) {
@@ -804,7 +830,7 @@ int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
         a.sdt = (float*)cur;
         if (dtype == PPK_F32) run_fwd<float>(a, true, (unsigned)blocks, st);
         else run_fwd<bf16_t>(a, true, (unsigned)blocks, st);
-        k_scan_join<false><<<dim3((unsigned)ceil_div(D * N, 256), (unsigned)B), 256, 0, st>>>(a);
+        join<false>(a, B, st);
     }
     if (dtype == PPK_F32) run_fwd<float>(a, false, (unsigned)blocks, st);
     else run_fwd<bf16_t>(a, false, (unsigned)blocks, st);
@@ -862,7 +888,7 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
             const unsigned pb = (unsigned)(items * G * part.blocks_per_group);
             if (dtype == PPK_F32) run_bwd_part<float>(part, pb, st);
             else run_bwd_part<bf16_t>(part, pb, st);
-            k_scan_join<true><<<dim3((unsigned)ceil_div(D * N, 256), (unsigned)B), 256, 0, st>>>(a);
+            join<true>(a, B, st);
         }
         if (dtype == PPK_F32) run_bwd<float>(a, (unsigned)blocks, st);
         else run_bwd<bf16_t>(a, (unsigned)blocks, st);
