@@ -19,7 +19,7 @@ using ppk::uniform;
 constexpr int TILE = 16;                     // steps between two kept states
 // Splits of the time axis: where the sequences and channels alone make less than a quarter of FWD_WAVES waves, one a SIMD (of BWD_BLOCKS blocks,
 // two a CU), a split takes as many steps as make that many, and MIN_SPAN (BWD_MIN_SPAN) at least.  Measured, 16 states:
-//   1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 48 with 32, 47 with 16 (joining them eats the rest);
+//   1 x 2048 x 1024 bf16 forward 65 us with 64 steps at least, 48 with 32, 41 with 16;
 //   21 x 100 x 333 fp32 forward 41 us with 32 steps at least, 28 with 16;
 //   64 x 256 x 1024 (1024 waves) fp32 forward 154 us in one piece, 170 in four splits; half the sequences 118 in one, 101 in eight;
 //   32 x 256 x 1024 (512 blocks) fp32 training 266 us with the backward pass in one piece, 321 in splits;
@@ -304,7 +304,9 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 }
 
 // Joins the splits of a sequence: carry[s] holds what split s gives alone and receives what enters it.  Forward from the state before
-// the first step, backward (REV) from the gradient of the state behind the last; a thread a state.
+// the first step, backward (REV) from the gradient of the state behind the last.  h' = decay h + own is associative: a block takes
+// JOIN_STATES states and as many slices of the splits as make 256 threads, each slice joins its own, then the slices.  Bound by the latency of its
+// loads: 128 splits of 1024 channels x 16 states 7.8 us (a thread a state, one split after the other: 12; 16 states a block: 12, 64: 9.0).
 constexpr int JOIN_STATES = 32;
 template <bool REV, int U>
 __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
