@@ -107,10 +107,16 @@ class _Batch:
         if self.D < 1:
             raise ValueError(f'{what}: x has no channels')
 
+    def data_of(self, name, t):
+        """The rows of a per-step PackedSequence, which has to be packed as x is."""
+        if self.plan is None or not torch.equal(t.batch_sizes, self.plan.batch_sizes):
+            raise ValueError(f'{self.what}: {name} is packed in another way than x')
+        return t.data
+
     def take(self, name, t, tail, dtype):
         """A per-step tensor [lead, tail], the elements of its last dimension next to each other."""
         if isinstance(t, PackedSequence):
-            t = t.data
+            t = self.data_of(name, t)
         if not isinstance(t, torch.Tensor) or t.shape != self.lead + tail:
             raise ValueError(f'{self.what}: {name} must be {[*self.lead, *tail]}, not {list(t.shape) if isinstance(t, torch.Tensor) else t}')
         if t.dtype != dtype:
@@ -381,8 +387,6 @@ def _scan_params(what, A, D, dt_bias, width):
 
 def _grouped(what, name, t, lead, width, N):
     """B or C as [..., groups, N]."""
-    if isinstance(t, PackedSequence):
-        t = t.data
     if not isinstance(t, torch.Tensor) or t.dim() not in (len(lead) + 1, len(lead) + 2) or t.shape[-1] != N:
         raise ValueError(f'{what}: {name} must be [..., groups, {N}] or [..., {N}]')
     t = t.unsqueeze(-2) if t.dim() == len(lead) + 1 else t
@@ -407,6 +411,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, plan: Optional[
     N = _scan_params(what, A, D, dt_bias, width)
     raw = batch.take('dt', dt, (width,), data.dtype)
     gate = None if z is None else batch.take('z', z, (width,), data.dtype)
+    B, C = (batch.data_of(n, v) if isinstance(v, PackedSequence) else v for n, v in (('B', B), ('C', C)))
     Bg, Cg = _grouped(what, 'B', B, batch.lead, width, N), _grouped(what, 'C', C, batch.lead, width, N)
     if Bg.shape != Cg.shape:
         raise ValueError(f'{what}: B has {Bg.shape[-2]} groups, C has {Cg.shape[-2]}')

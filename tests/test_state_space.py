@@ -185,3 +185,17 @@ def test_plan_of_another_packing_is_refused():
     assert other.rows == 5
     with pytest.raises(ValueError, match='another packing'):
         S.causal_conv(packed, torch.zeros(D, K), plan=other)
+
+
+@pytest.mark.parametrize('name', ['dt', 'z', 'B', 'C'])
+def test_per_step_inputs_of_another_packing_are_refused(name):
+    """As many rows, but other lengths: row for row they would belong to other steps."""
+    x = pack_sequence([torch.zeros(3, D), torch.zeros(2, D)])
+    args = dict(x=x, dt=x, A=torch.zeros(D, N), B=pack_sequence([torch.zeros(3, N), torch.zeros(2, N)]), C=torch.zeros(5, N), z=x)
+    args[name] = pack_sequence([torch.zeros(4, D if name in 'dtz' else N), torch.zeros(1, D if name in 'dtz' else N)])
+    with pytest.raises(ValueError, match=f'{name} is packed in another way'):
+        S.selective_scan(**args)
+    flat = dict(args, x=torch.zeros(1, 5, D), dt=torch.zeros(1, 5, D), z=None, B=torch.zeros(1, 5, N), C=torch.zeros(1, 5, N))
+    flat[name] = args[name]
+    with pytest.raises(ValueError, match=f'{name} is packed in another way'):
+        S.selective_scan(**flat)
