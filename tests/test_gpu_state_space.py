@@ -514,3 +514,26 @@ def test_more_sequences_than_a_grid_has_rows():
     assert float(dA) == 0.0                        # no state before the first step
     xs = x.double()
     assert abs(float(dD) - float(xs.sum())) <= 2 * H * float(xs.abs().sum())
+
+
+@pytest.mark.parametrize('N', [8, 16, 32])
+@pytest.mark.parametrize('T', [5, 100])
+def test_states_and_parameters_anywhere_in_memory(T, N):
+    """A, the state and its gradient from an address that is no multiple of 16 bytes: other accesses, the same sums."""
+    from paccmann_polymer_amd.state_space import selective_scan, selective_scan_step
+    g = torch.Generator(device=DEV).manual_seed(13)
+    B, D = 3, 20
+
+    def shifted(t):
+        room = t.new_empty(t.numel() + 1)
+        return room[1:].view(t.shape).copy_(t)
+    x, dt, Bm, C = (randn(g, T, B, n, scale=0.5) for n in (D, D, N, N))
+    A, state, dlast = -randn(g, D, N).abs(), randn(g, B, D, N), randn(g, B, D, N)
+    results = []
+    for f in (torch.clone, shifted):
+        leaves = [x.clone().requires_grad_(), f(A).detach().requires_grad_(), f(state).detach().requires_grad_()]
+        y, last = selective_scan(leaves[0], dt, leaves[1], Bm, C, state=leaves[2])
+        step = selective_scan_step(x[0], dt[0], f(A), Bm[0], C[0], f(state))
+        results.append([y, last, *torch.autograd.grad((y, last), leaves, (x, f(dlast))), *step])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
