@@ -153,29 +153,28 @@ template <int CL> struct Run {
 };
 template <int CL> __device__ __forceinline__ unsigned row_of(const SeqBatch& q, long long t) { return CL == 64 ? ppk::uni_row(q, t) : (unsigned)q.row(t); }
 
-// the input of step t, which is of the state before the first step
-template <typename T, int VEC, int CL>
+// the input of step t >= -(K - 1), which is of the state before the first step
+template <typename T, int VEC, int K, int CL>
 __device__ __forceinline__ void input_at(const ConvArgs& a, const Rows<T>& xs, long long t, long long b, int c, float (&v)[VEC])
 {
     if (t >= 0) { widen<T, VEC>(xs.template get_as<Vec<T, VEC>>(row_of<CL>(a.q, t), c * (unsigned)sizeof(T)), v); return; }
-    const long long i = t + a.K - 1;
-    if (i >= 0 && a.state) { load_vec<T, VEC>((const T*)a.state + (b * (a.K - 1) + i) * a.D + c, v); return; }
+    if (a.state) { load_vec<T, VEC>((const T*)a.state + (b * (K - 1) + t + K - 1) * a.D + c, v); return; }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = 0.f;
 }
-// KP taps, K of them the operator's: the first KP - K are zero
-template <int VEC, int KP> __device__ __forceinline__ void load_taps(const ConvArgs& a, int c, float (&w)[KP][VEC], float (&bias)[VEC])
+template <int VEC, int K> __device__ __forceinline__ void load_taps(const ConvArgs& a, int c, float (&w)[K][VEC], float (&bias)[VEC])
 {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         bias[e] = a.bias ? a.bias[c + e] : 0.f;
 #pragma unroll
-        for (int j = 0; j < KP; ++j) w[j][e] = j >= KP - a.K ? a.weight[(long long)(c + e) * a.K + j - (KP - a.K)] : 0.f;
+        for (int j = 0; j < K; ++j) w[j][e] = a.weight[(long long)(c + e) * K + j];
     }
 }
 
-// block 256 = 256 / CL runs x CL lanes of VEC channels
-template <typename T, int VEC, int KP, int CL>
+// block 256 = 256 / CL runs x CL lanes of VEC channels.  Compiled for each K: more taps with weights of zero would multiply inputs that the
+// operator does not reach, and 0 times an infinity is NaN.
+template <typename T, int VEC, int K, int CL>
 __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a, int channel_blocks)
 {
     const int c = ((int)(blockIdx.x % channel_blocks) * CL + threadIdx.x % CL) * VEC;
@@ -193,10 +192,10 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a, int channel_blocks
         for (int i = 0; i < AHEAD; ++i) next[i] = xs.template get_as<Vec<T, VEC>>(rows[i], cb);
     };
     if (t0 < t1) fetch(t0);
-    float w[KP][VEC], bias[VEC], win[KP][VEC];
-    load_taps<VEC, KP>(a, c, w, bias);
+    float w[K][VEC], bias[VEC], win[K][VEC];
+    load_taps<VEC, K>(a, c, w, bias);
 #pragma unroll
-    for (int j = 0; j < KP - 1; ++j) input_at<T, VEC, CL>(a, xs, t0 - (KP - 1) + j, b, c, win[j]);
+    for (int j = 0; j < K - 1; ++j) input_at<T, VEC, K, CL>(a, xs, t0 - (K - 1) + j, b, c, win[j]);
     for (long long t = t0; t < t1; t += AHEAD) {
         float x[AHEAD][VEC];
 #pragma unroll
@@ -208,24 +207,23 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs a, int channel_blocks
             float out[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                win[KP - 1][e] = x[i][e];
+                win[K - 1][e] = x[i][e];
                 float s = bias[e];
 #pragma unroll
-                for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+                for (int j = 0; j < K; ++j) s = fmaf(w[j][e], win[j][e], s);
                 out[e] = a.silu ? s * sigmoid(s) : s;
 #pragma unroll
-                for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+                for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
             }
             ys.template put_as<Vec<T, VEC>>(r[i], cb, narrow<T, VEC>(out));
         }
     }
     if (t1 == run.len && a.last)
 #pragma unroll
-        for (int j = 0; j < KP - 1; ++j)
-            if (j >= KP - a.K) store_vec<T, VEC>((T*)a.last + (b * (a.K - 1) + j - (KP - a.K)) * a.D + c, win[j]);
+        for (int j = 0; j < K - 1; ++j) store_vec<T, VEC>((T*)a.last + (b * (K - 1) + j) * a.D + c, win[j]);
 }
 
-template <typename T, int VEC, int KP, int CL>
+template <typename T, int VEC, int K, int CL>
 __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks)
 {
     constexpr int IL = 256 / CL;
@@ -233,15 +231,15 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks
     const int cl = threadIdx.x % CL, il = threadIdx.x / CL, c = ((int)(blockIdx.x % channel_blocks) * CL + cl) * VEC;
     const long long first_block = blockIdx.x / channel_blocks, blocks = gridDim.x / channel_blocks;
     const unsigned cb = c * (unsigned)sizeof(T);
-    float dw[KP][VEC] = {}, db[VEC] = {};
+    float dw[K][VEC] = {}, db[VEC] = {};
     if (c < a.D) {
-        float w[KP][VEC], bias[VEC];
-        load_taps<VEC, KP>(a, c, w, bias);
+        float w[K][VEC], bias[VEC];
+        load_taps<VEC, K>(a, c, w, bias);
         const long long items = a.q.B * a.runs;
         for (long long item = first_block * IL + il; item < items; item += blocks * IL) {
             const Run<CL> run(a, item);
             if (!run.any) continue;
-            const long long b = run.b, t0 = run.t0, t1 = run.t1, len = run.len, first = t0 == 0 ? -(long long)(a.K - 1) : t0;
+            const long long b = run.b, t0 = run.t0, t1 = run.t1, len = run.len, first = t0 == 0 ? -(long long)(K - 1) : t0;
             const Rows<T> xs(a.x, b * a.xs.b, a.xs.t), dys(a.dy, b * a.dys.b, a.dys.t), dxs(a.dx, b * a.ys.b, a.ys.t);
             Vec<T, VEC> nx[AHEAD], nd[AHEAD];
             const auto fetch = [&](long long t) {            // behind the sequence's last step, that one again
@@ -252,14 +250,14 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks
                 for (int i = 0; i < AHEAD; ++i) { nx[i] = xs.template get_as<Vec<T, VEC>>(rows[i], cb); nd[i] = dys.template get_as<Vec<T, VEC>>(rows[i], cb); }
             };
             if (len > 0) fetch(t0);
-            float win[KP][VEC], dp[KP][VEC];                 // inputs t - KP + 1 .. t; dp[j] = dpre of step t - j
+            float win[K][VEC], dp[K][VEC];                   // inputs t - K + 1 .. t; dp[j] = dpre of step t - j
 #pragma unroll
-            for (int j = 0; j < KP - 1; ++j) input_at<T, VEC, CL>(a, xs, t0 - (KP - 1) + j, b, c, win[j]);
+            for (int j = 0; j < K - 1; ++j) input_at<T, VEC, K, CL>(a, xs, t0 - (K - 1) + j, b, c, win[j]);
 #pragma unroll
-            for (int j = 0; j < KP; ++j)
+            for (int j = 0; j < K; ++j)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) dp[j][e] = 0.f;
-            const long long te = t1 + KP - 1;
+            const long long te = t1 + K - 1;
             for (long long tg = t0; tg < te; tg += AHEAD) {
                 float x[AHEAD][VEC], dy[AHEAD][VEC];
 #pragma unroll
@@ -270,7 +268,7 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks
                     const long long t = tg + i;
                     if (t >= te) break;
 #pragma unroll
-                    for (int j = KP - 1; j > 0; --j)
+                    for (int j = K - 1; j > 0; --j)
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) dp[j][e] = dp[j - 1][e];
 #pragma unroll
@@ -278,58 +276,56 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs a, int channel_blocks
                     if (t < len) {
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) {
-                            win[KP - 1][e] = x[i][e];
+                            win[K - 1][e] = x[i][e];
                             float s = bias[e], d = dy[i][e];
 #pragma unroll
-                            for (int j = 0; j < KP; ++j) s = fmaf(w[j][e], win[j][e], s);
+                            for (int j = 0; j < K; ++j) s = fmaf(w[j][e], win[j][e], s);
                             if (a.silu) { const float g = sigmoid(s); d *= g * fmaf(s, 1.0f - g, 1.0f); }
                             dp[0][e] = d;
                             if (t < t1) {
                                 db[e] += d;
 #pragma unroll
-                                for (int j = 0; j < KP; ++j) dw[j][e] = fmaf(d, win[j][e], dw[j][e]);
+                                for (int j = 0; j < K; ++j) dw[j][e] = fmaf(d, win[j][e], dw[j][e]);
                             }
 #pragma unroll
-                            for (int j = 0; j < KP - 1; ++j) win[j][e] = win[j + 1][e];
+                            for (int j = 0; j < K - 1; ++j) win[j][e] = win[j + 1][e];
                         }
                     }
-                    const long long tt = t - (KP - 1);       // the step whose input's gradient is complete
+                    const long long tt = t - (K - 1);        // the step whose input's gradient is complete
                     if (tt < first || tt >= t1) continue;
                     float dx[VEC];
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         dx[e] = 0.f;
 #pragma unroll
-                        for (int j = 0; j < KP; ++j) dx[e] = fmaf(w[j][e], dp[j][e], dx[e]);
+                        for (int j = 0; j < K; ++j) dx[e] = fmaf(w[j][e], dp[j][e], dx[e]);
                     }
-                    const long long k = tt - (len - (a.K - 1));
+                    const long long k = tt - (len - (K - 1));
                     if (k >= 0 && a.dlast) {                 // the last K - 1 inputs are the new state too
                         float g[VEC];
-                        load_vec<T, VEC>((const T*)a.dlast + (b * (a.K - 1) + k) * a.D + c, g);
+                        load_vec<T, VEC>((const T*)a.dlast + (b * (K - 1) + k) * a.D + c, g);
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) dx[e] += g[e];
                     }
                     if (tt >= 0) dxs.template put_as<Vec<T, VEC>>(row_of<CL>(a.q, tt), cb, narrow<T, VEC>(dx));
-                    else if (a.dstate) store_vec<T, VEC>((T*)a.dstate + (b * (a.K - 1) + tt + a.K - 1) * a.D + c, dx);
+                    else if (a.dstate) store_vec<T, VEC>((T*)a.dstate + (b * (K - 1) + tt + K - 1) * a.D + c, dx);
                 }
             }
         }
     }
     // the items of a block, in order, one column of the partial sums at a time
 #pragma unroll
-    for (int j = 0; j <= KP; ++j) {
-        if (j < KP && j < KP - a.K) continue;
+    for (int j = 0; j <= K; ++j) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) red[il][cl][e] = j < KP ? dw[j < KP ? j : 0][e] : db[e];
+        for (int e = 0; e < VEC; ++e) red[il][cl][e] = j < K ? dw[j < K ? j : 0][e] : db[e];
         __syncthreads();
         if (il == 0 && c < a.D) {
-            const int col = j < KP ? j - (KP - a.K) : a.K;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 float s = red[0][cl][e];
                 for (int i = 1; i < IL; ++i) s += red[i][cl][e];
-                a.part[(first_block * (a.K + 1) + col) * a.D + c + e] = s;
+                a.part[(first_block * (K + 1) + j) * a.D + c + e] = s;
             }
         }
     }
@@ -360,22 +356,27 @@ __global__ __launch_bounds__(256) void k_conv_step(long long B, int D, int K, co
 
 int taps(long long K) { return K <= 2 ? 2 : K <= 4 ? 4 : 8; }
 
-template <typename T, int VEC, int KP, int CL> void launch_conv(const ConvArgs& a, bool bwd, unsigned blocks, hipStream_t st)
+template <typename T, int VEC, int K, int CL> void launch_conv(const ConvArgs& a, bool bwd, unsigned blocks, hipStream_t st)
 {
     const int cb = (a.D + CL * VEC - 1) / (CL * VEC);
-    if (bwd) k_conv_bwd<T, VEC, KP, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
-    else k_conv_fwd<T, VEC, KP, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
+    if (bwd) k_conv_bwd<T, VEC, K, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
+    else k_conv_fwd<T, VEC, K, CL><<<blocks * (unsigned)cb, 256, 0, st>>>(a, cb);
 }
-template <typename T, int VEC, int KP> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
+template <typename T, int VEC, int K> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
 {
-    if (cl == 16) launch_conv<T, VEC, KP, 16>(a, bwd, blocks, st);
-    else launch_conv<T, VEC, KP, 64>(a, bwd, blocks, st);
+    if (cl == 16) launch_conv<T, VEC, K, 16>(a, bwd, blocks, st);
+    else launch_conv<T, VEC, K, 64>(a, bwd, blocks, st);
 }
 template <typename T, int VEC> void launch_conv(const ConvArgs& a, bool bwd, int cl, unsigned blocks, hipStream_t st)
 {
-    switch (taps(a.K)) {
+    switch (a.K) {
+        case 1: launch_conv<T, VEC, 1>(a, bwd, cl, blocks, st); break;
         case 2: launch_conv<T, VEC, 2>(a, bwd, cl, blocks, st); break;
+        case 3: launch_conv<T, VEC, 3>(a, bwd, cl, blocks, st); break;
         case 4: launch_conv<T, VEC, 4>(a, bwd, cl, blocks, st); break;
+        case 5: launch_conv<T, VEC, 5>(a, bwd, cl, blocks, st); break;
+        case 6: launch_conv<T, VEC, 6>(a, bwd, cl, blocks, st); break;
+        case 7: launch_conv<T, VEC, 7>(a, bwd, cl, blocks, st); break;
         default: launch_conv<T, VEC, 8>(a, bwd, cl, blocks, st);
     }
 }

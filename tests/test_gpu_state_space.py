@@ -537,3 +537,65 @@ def test_states_and_parameters_anywhere_in_memory(T, N):
         results.append([y, last, *torch.autograd.grad((y, last), leaves, (x, f(dlast))), *step])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def same_kind(got, want, what=''):
+    """NaN and infinities (with their signs) stand where the 64-bit definition has them."""
+    want = want.to(got.dtype)
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(want)), (what, kind.__name__, int((kind(got) != kind(want)).sum()))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('silu', [False, True])
+@pytest.mark.parametrize('D', [8, 5, 72, 70])                    # rows of 16 lanes and whole waves, four channels a lane and one
+@pytest.mark.parametrize('K', range(1, 9))
+def test_causal_conv_infinite_inputs_reach_k_steps(K, D, silu, dtype):
+    """An infinite input and a NaN in the middle of two sequences, and an infinite upstream gradient: what a tap does not reach is as without."""
+    from paccmann_polymer_amd.state_space import causal_conv, causal_conv_step
+    lay = Layout([40, 40, 40, 21], 'packed')
+    g = torch.Generator(device=DEV).manual_seed(K * 100 + D)
+    x, dy = lay.tensor(g, D, dtype=dtype), lay.tensor(g, D, dtype=dtype)
+    w, bias = torch.rand(D, K, generator=g, device=DEV) + 0.1, randn(g, D, scale=0.3)
+    state, dlast = randn(g, lay.B, K - 1, D, dtype=dtype), randn(g, lay.B, K - 1, D, dtype=dtype)
+
+    def run(x, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w, bias, state)]
+        y, last = causal_conv(leaves[0], leaves[1], leaves[2], plan=lay.plan, state=leaves[3], activation='silu' if silu else None)
+        return (y.detach(), last.detach(), *torch.autograd.grad((y, last), leaves, (dy, dlast)))
+
+    def want(x, dy):
+        leaves = [t.detach().double().requires_grad_() for t in (x, w, bias, state)]
+        y, last = conv_definition(lay, *leaves, False)
+        y = torch.nn.functional.silu(y) if silu else y          # its derivative as one factor: as a sum of two, an infinite dy makes inf - inf of it
+        used = [y, last] if K > 1 else [y]
+        gr = torch.autograd.grad(used, leaves, (dy.double(), dlast.double())[:len(used)], allow_unused=True)
+        return (y.detach(), last.detach(), *(torch.zeros_like(t) if d is None else d for t, d in zip(leaves, gr)))
+
+    clean = run(x, dy)
+    inf, at = float('inf'), 13
+    rows = torch.stack([lay.off[t] + torch.arange(lay.B) if n == lay.B else torch.cat([lay.off[t] + torch.arange(n), torch.full((lay.B - n,), lay.rows)])
+                        for t, n in enumerate(lay.bs)])                                       # [T, B]: a sequence's rows; behind its last, none
+    for field, values in (('x', ((1, 2, inf), (2, 4, float('nan')))), ('dy', ((1, 2, inf), (0, 3, -inf)))):
+        xs, ds = x.clone(), dy.clone()
+        hit_y, hit_dx = (torch.zeros(lay.rows + 1, D, dtype=torch.bool, device=DEV) for _ in range(2))
+        for b, c, value in values:
+            (xs if field == 'x' else ds)[rows[at, b], c] = value
+            if field == 'x':
+                hit_y[rows[at:at + K, b], c] = True
+                if silu:
+                    hit_dx[rows[at - K + 1:at + K, b], c] = True
+            else:
+                hit_dx[rows[at - K + 1:at + 1, b], c] = True
+        got, expected = run(xs, ds), want(xs, ds)
+        for name, a, b in zip(('y', 'last', 'dx', 'dw', 'dbias', 'dstate'), got, expected):
+            same_kind(a, b, (field, name))
+        assert torch.equal(got[0][~hit_y[:-1]], clean[0][~hit_y[:-1]])
+        assert torch.equal(got[2][~hit_dx[:-1]], clean[2][~hit_dx[:-1]])
+        assert torch.equal(got[5], clean[5])                                                  # nothing reaches the state before the first step
+        if field == 'x':
+            s = state
+            for t in range(40):
+                n = lay.bs[t]
+                out, s = causal_conv_step(xs[lay.off[t]:lay.off[t + 1]], s[:n], w, bias, 'silu' if silu else None)
+                same_kind(out, got[0][lay.off[t]:lay.off[t + 1]].double(), ('step', t))
