@@ -377,8 +377,9 @@ template <int LPC> __device__ __forceinline__ float sum_slices(float v)
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Parts of a tile: a sequence's last tile is worked on as far as the part that its last step is in.  2048 sequences of 20 to 100 steps, 512 channels,
-// 16 states, fp32: 1175 us, 1223 with whole tiles; 21 of 1 to 100 steps, 333 channels: 43 and 46.  Five and eight parts: the same.
-constexpr int NPARTS = 3, PARTS[NPARTS + 1] = {0, 5, 10, TILE};
+// 16 states, fp32: 1170 us, 1223 with whole tiles, 1177 with three parts; 1 x 16384 x 2048 bf16: 540, 530 with three; 21 sequences of 1 to 100
+// steps, 333 channels: 44, 46 with whole tiles, 42 with three.  Parts of two steps: only their second can be one that does not exist.
+constexpr int NPARTS = 8, PART = TILE / NPARTS, FETCH_PART = 4;
 
 // The backward pass.  A block takes 256 / LPC channels of a group of one sequence and walks a split's tiles backwards; a thread holds the
 // four states 4 slice .. of a channel.  In a wave, lane % 16 = slice * (16 / LPC) + low bits of the channel, lane / 16 = its high bits:
@@ -495,9 +496,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
         __syncthreads();
 #pragma unroll
         for (int part = 0; part < NPARTS; ++part) {
-            if (PARTS[part] >= steps) break;
+            if (part * PART >= steps) break;
 #pragma unroll
-            for (int t = PARTS[part]; t < PARTS[part + 1]; ++t) {
+            for (int t = part * PART; t < (part + 1) * PART; ++t) {
                 const float dtv = s_dt[t][ch], dxv = s_dx[t][ch];
                 const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]);
 #pragma unroll
@@ -510,10 +511,10 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
         asm volatile("" ::: "memory");           // the steps' values are read from LDS again: kept, they would be 96 registers
 #pragma unroll
         for (int part = NPARTS - 1; part >= 0; --part) {
-            if (part == NPARTS - 2) fetch(next);                                // where the registers of a part's steps are free again
-            if (PARTS[part] >= steps) continue;
+            if (part == FETCH_PART) fetch(next);                                // where the registers of the parts behind it are free again
+            if (part * PART >= steps) continue;
 #pragma unroll
-            for (int t = PARTS[part + 1] - 1; t >= PARTS[part]; --t) {
+            for (int t = (part + 1) * PART - 1; t >= part * PART; --t) {
                 const float dtv = s_dt[t][ch], dxv = s_dx[t][ch], dyv = s_dy[t][ch];
                 const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s_BC[t][ns * 4]), Cv = *reinterpret_cast<const f32x4*>(&s_BC[t][NP + ns * 4]);
                 float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
@@ -527,7 +528,8 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
                     dh[j] *= av[t][j];
                     const float da = dh[j] * h[t][j];
                     q2 = fmaf(da, A2[j], q2);
-                    dA[j] = fmaf(da, dtv, dA[j]);
+                    // a step that does not exist has a dt of 0, but an infinite state may enter it; nothing has been added before the sequence's last step
+                    dA[j] = t == part * PART || t < steps ? fmaf(da, dtv, dA[j]) : 0.f;
                 }
                 q1 = sum_slices<LPC>(q1);
                 q2 = sum_slices<LPC>(q2);

@@ -599,3 +599,27 @@ def test_causal_conv_infinite_inputs_reach_k_steps(K, D, silu, dtype):
                 n = lay.bs[t]
                 out, s = causal_conv_step(xs[lay.off[t]:lay.off[t + 1]], s[:n], w, bias, 'silu' if silu else None)
                 same_kind(out, got[0][lay.off[t]:lay.off[t + 1]].double(), ('step', t))
+
+
+@pytest.mark.parametrize('T', [1, 3, 5, 7, 16, 23, 200])
+@pytest.mark.parametrize('N', [16, 11, 32])
+def test_gradients_of_an_infinite_last_input(N, T):
+    """The state that it makes is read by no step: gradients of A, x and the first state are those of any other input there."""
+    from paccmann_polymer_amd.state_space import selective_scan
+    lay, t, dy, dlast = scan_case([T, T, max(T - 1, 1)], 'packed', 20, N, 1, torch.float32, True, True, True, True, True)
+    row = int(lay.off[T - 1] + 1)                                       # the last step of sequence 1
+
+    def grads(t):
+        leaves = {k: v.detach().requires_grad_() for k, v in t.items()}
+        y, last = selective_scan(**leaves, plan=lay.plan)
+        return dict(zip(t, torch.autograd.grad((y, last), list(leaves.values()), (dy, dlast))))
+
+    clean = grads(t)
+    bad = {k: v.clone() for k, v in t.items()}
+    bad['x'][row, 7] = float('inf')
+    got = grads(bad)
+    for k in ('A', 'x', 'state'):
+        assert torch.equal(got[k], clean[k]), k
+    want = scan_reference(lay, bad, dy, dlast, True, False)[2]
+    for k in ('dt', 'B', 'C', 'D', 'dt_bias'):
+        same_kind(got[k], want[k], k)
