@@ -213,10 +213,11 @@ __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
             Bv.begin((const T*)Bs.row(r[i]), bl[i]);
             if (!PART) Cv.begin((const T*)Cs.row(r[i]), cl[i]);
             const float dt = a.softplus ? softplus(raw[i]) : raw[i], dx = dt * x[i];
-            float y[4] = {skip * x[i], 0.f, 0.f, 0.f};
+            float y[4] = {!PART && a.skip ? skip * x[i] : 0.f, 0.f, 0.f, 0.f};     // no D: no term, which an infinite x would make NaN of
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 h[n] = fmaf(exp2_(dt * A2[n]), h[n], dx * Bv.at(n));
+                if (!SCALAR && !PART) h[n] = n < N ? h[n] : 0.f;               // an infinite dx makes NaN of a state that does not exist
                 if (!PART) y[n & 3] = fmaf(h[n], Cv.at(n), y[n & 3]);
             }
             if (PART) { sum += dt; return; }
@@ -389,7 +390,10 @@ constexpr int NPARTS = 8, PART = TILE / NPARTS, FETCH_PART = 4;
 //   256 vector instructions, and slower: 1574 against 1222 us on 2048 sequences of 20 to 100 steps, 512 channels, 16 states, fp32, where the
 //   matrix unit and the vector unit were busy for 80 % of the time together, one after the other.
 // Elements of a tile are loaded while the tile behind it is worked on, and what the tile's end needs of them waits in LDS.
-template <typename T, int LPC>
+// FULL: N is 4 LPC and the channels of a group are whole blocks.  Otherwise states and channels that do not exist are kept at zero: their products
+// with an infinite input, B, C or gradient would be NaN, and sums over states and channels take them in (21 sequences, 333 channels of three
+// groups, 11 states: 46 us, 44 without).
+template <typename T, int LPC, bool FULL>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 {
     constexpr int NP = 4 * LPC, BC = 256 / LPC, PE = TILE * BC / 256, CL = 16 / LPC, BCE = TILE * 2 * NP / 256;
@@ -411,14 +415,17 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
     const long long len = uni_len(a.q, b), end = (s + 1) * a.span < len ? (s + 1) * a.span : len;
     const long long tile0 = first_tile(a, b);
     float A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, dh[4];
+    bool exists[4];
     const float* into = a.splits > 1 && s * a.span < len ? a.carry + carry_at(a, b, s, d) * N : (a.dlast ? a.dlast + (b * a.D + d) * N : nullptr);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int n = ns * 4 + j;
-        A2[j] = live && n < N ? base2(a.A[(long long)d * N + n]) : 0.f;
-        dh[j] = live && n < N && into ? into[n] : 0.f;
+        exists[j] = live && n < N;
+        A2[j] = live ? base2(a.A[(long long)d * N + (n < N ? n : 0)]) : 0.f;          // a state that does not exist decays as one that does
+        dh[j] = exists[j] && into ? into[n] : 0.f;
     }
     const float skip = a.skip && plive ? a.skip[pd] : 0.f, bias = a.bias && plive ? a.bias[pd] : 0.f;
+    const bool has_skip = a.skip != nullptr;
     float dskip = 0.f, dbias = 0.f;
 
     const Rows<T> xs(a.x, b * a.xs.b, a.xs.t), rs(a.raw, b * a.raws.b, a.raws.t), ds(a.dy, b * a.dys.b, a.dys.t);
@@ -504,7 +511,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     av[t][j] = exp2_(dtv * A2[j]);
-                    h[t + 1][j] = fmaf(av[t][j], h[t][j], dxv * Bv[j]);
+                    h[t + 1][j] = fmaf(av[t][j], h[t][j], FULL || exists[j] ? dxv * Bv[j] : 0.f);
                 }
             }
         }
@@ -520,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
                 float q1 = 0.f, q2 = 0.f, q3 = 0.f, v[8];                           // v: dB of the four states, then dC
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    dh[j] = fmaf(dyv, Cv[j], dh[j]);
+                    dh[j] = FULL || exists[j] ? fmaf(dyv, Cv[j], dh[j]) : 0.f;
                     q1 = fmaf(dh[j], Bv[j], q1);
                     v[j] = dh[j] * dxv;
                     v[4 + j] = dyv * h[t + 1][j];
@@ -560,9 +567,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
             const unsigned r = BC >= 64 ? uni_row(a.q, t0 + t) : (unsigned)a.q.row(t0 + t);
             const float q1 = s_q[0][t][pc], x = s_x[t][pc], dy = s_dy[t][pc];
             const float dr = fmaf(x, q1, s_q[1][t][pc] * LN2) * s_slope[t][pc];
-            dxs.put(r, pb, from_f32<T>(fmaf(s_dt[t][pc], q1, skip * dy)));
+            dxs.put(r, pb, from_f32<T>(fmaf(s_dt[t][pc], q1, skip * (has_skip ? dy : 0.f))));
             drs.put(r, pb, from_f32<T>(dr));
-            if (a.z) dzs.put(r, pb, from_f32<T>(s_gz[t][pc] * fmaf(skip, x, s_q[2][t][pc])));
+            if (a.z) dzs.put(r, pb, from_f32<T>(s_gz[t][pc] * fmaf(skip, has_skip ? x : 0.f, s_q[2][t][pc])));
             dskip = fmaf(dy, x, dskip);
             dbias += dr;
         }
@@ -640,12 +647,14 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
         }
     const float x = to_f32(((const T*)a.x)[b * a.xs.b + d]);
     const float raw = to_f32(((const T*)a.raw)[b * a.raws.b + d]) + (a.bias ? a.bias[d] : 0.f);
-    const float z = a.z ? to_f32(((const T*)a.z)[b * a.zs.b + d]) : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    const float z = a.z ? to_f32(((const T*)a.z)[b * a.zs.b + d]) : 0.f;
+    const float skip = (a.skip ? a.skip : a.A)[d];                             // no D: any of A's, unused; behind a branch the load is late (15.0 -> 15.6 us)
     const float dt = a.softplus ? softplus(raw) : raw, dx = dt * x;
     float y = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         h[j] = fmaf(exp2_(dt * base2(A[j])), h[j], dx * Bv[j]);
+        if (!WIDE) h[j] = ns * 4 + j < N ? h[j] : 0.f;                         // an infinite dx makes NaN of a state that does not exist
         y = fmaf(h[j], Cv[j], y);
     }
     if (WIDE) *reinterpret_cast<float4*>(next + at_h) = make_float4(h[0], h[1], h[2], h[3]);
@@ -653,7 +662,7 @@ __global__ __launch_bounds__(256) void k_scan_step(ScanArgs a, const float* stat
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (ns * 4 + j < N) next[at_h + j] = h[j];
-    y = lanes_sum<LPC>(y) + skip * x;
+    y = lanes_sum<LPC>(y) + (a.skip ? skip * x : 0.f);
     if (a.z) y *= z * sigmoid(z);
     if (ns == 0) ((T*)a.y)[bd] = from_f32<T>(y);
 }
@@ -724,12 +733,17 @@ template <bool REV> void join(const ScanArgs& a, long long B, hipStream_t st)
     if (a.splits <= 4 * 256 / JOIN_STATES) k_scan_join<REV, 4><<<grid, 256, 0, st>>>(a);
     else k_scan_join<REV, 16><<<grid, 256, 0, st>>>(a);
 }
+template <typename T, int LPC> void launch_bwd(const ScanArgs& a, unsigned blocks, hipStream_t st)
+{
+    if (a.N == 4 * LPC && a.per % (256 / LPC) == 0) k_scan_bwd<T, LPC, true><<<blocks, 256, 0, st>>>(a);
+    else k_scan_bwd<T, LPC, false><<<blocks, 256, 0, st>>>(a);
+}
 template <typename T> void run_bwd(const ScanArgs& a, unsigned blocks, hipStream_t st)
 {
     switch (bwd_slices(a.N)) {
-        case 4: k_scan_bwd<T, 4><<<blocks, 256, 0, st>>>(a); break;
-        case 8: k_scan_bwd<T, 8><<<blocks, 256, 0, st>>>(a); break;
-        default: k_scan_bwd<T, 16><<<blocks, 256, 0, st>>>(a);
+        case 4: launch_bwd<T, 4>(a, blocks, st); break;
+        case 8: launch_bwd<T, 8>(a, blocks, st); break;
+        default: launch_bwd<T, 16>(a, blocks, st);
     }
 }
 template <typename T, int LPC> void launch_step(const ScanArgs& a, unsigned blocks, const float* state, float* next, hipStream_t st)

@@ -623,3 +623,52 @@ def test_gradients_of_an_infinite_last_input(N, T):
     want = scan_reference(lay, bad, dy, dlast, True, False)[2]
     for k in ('dt', 'B', 'C', 'D', 'dt_bias'):
         same_kind(got[k], want[k], k)
+
+
+def positive(t):
+    """The same case without cancelling infinities: what is not a decay is positive."""
+    return {k: v if v is None or k in ('A', 'dt', 'dt_bias') else v.abs() + 0.1 for k, v in t.items()}
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('skip,gate', [(False, False), (False, True), (True, True)])
+@pytest.mark.parametrize('T', [4, 21, 70])
+@pytest.mark.parametrize('N', [1, 3, 5, 8, 11, 16, 17, 33, 50, 64])
+def test_selective_scan_infinities_are_the_definitions(N, T, skip, gate, dtype):
+    """An infinity in x, dt, B, C or the upstream gradient: states, channels and steps that do not exist turn no infinite result into NaN, and no finite
+    one into anything else."""
+    from paccmann_polymer_amd.state_space import selective_scan
+    D, inf, at = 20, float('inf'), T // 2
+    lay, t, dy, dlast = scan_case([T, T], 'time', D, N, 2, dtype, gate, skip, True, True, True)
+    t, dy, dlast = positive(t), dy.abs() + 0.1, dlast.abs() + 0.1
+    names = [k for k, v in t.items() if v is not None]
+    for field in ('x', 'dt', 'B', 'C', 'dy'):
+        p, up = {k: None if v is None else v.clone() for k, v in t.items()}, dy.clone()
+        if field in ('B', 'C'):
+            p[field][at, 1, 0, N // 2] = inf
+        else:
+            (up if field == 'dy' else p['x'])[at, 1, 7] = inf
+        leaves = {k: None if v is None else v.detach().requires_grad_() for k, v in p.items()}
+        y, last = selective_scan(**leaves)
+        got = dict(zip(names, torch.autograd.grad((y, last), [leaves[k] for k in names], (up, dlast))))
+        yw, lw, want = scan_reference(lay, p, up, dlast, True, False)
+        same_kind(y.detach(), yw, (field, 'y'))
+        same_kind(last.detach(), lw, (field, 'last'))
+        for k in names:
+            same_kind(got[k], want[k], (field, k))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('skip', [False, True])
+@pytest.mark.parametrize('N', [1, 3, 4, 11, 16, 30, 33, 64])
+def test_selective_scan_step_infinities_are_the_definitions(N, skip, dtype):
+    from paccmann_polymer_amd.state_space import selective_scan_step
+    lay, t, _, _ = scan_case([1, 1], 'time', 20, N, 2, dtype, True, skip, True, True, True)
+    t = positive(t)
+    for field in ('x', 'dt', 'B', 'C'):
+        p = {k: None if v is None else v.clone() for k, v in t.items()}
+        p[field].view(2, -1)[1, 0] = float('inf')
+        y, s = selective_scan_step(p['x'][0], p['dt'][0], p['A'], p['B'][0], p['C'][0], p['state'], D=p['D'], z=p['z'][0], dt_bias=p['dt_bias'])
+        yw, sw = scan_definition(lay, 2, *(None if p[k] is None else p[k].double() for k in ('x', 'dt', 'dt', 'A', 'B', 'C', 'D', 'z', 'dt_bias', 'dt_bias', 'state')), True)
+        same_kind(y, yw[0], (field, 'y'))
+        same_kind(s, sw, (field, 'state'))
