@@ -134,9 +134,10 @@ class _Batch:
         return s[0] if self.T > 1 else 0, s[1] if self.B > 1 else 0
 
     def new(self, tail, like):
-        """An uninitialised per-step tensor of the type and device of `like`, laid out as x is."""
+        """An uninitialised per-step tensor of the type and device of `like`, laid out as x is; no view: a caller may change it in place."""
         if self.plan is None and self.batch_first:
-            return like.new_empty((self.B, self.T, *tail)).transpose(0, 1)
+            n = tail[0] if len(tail) == 1 else tail[0] * tail[1]
+            return like.new_empty_strided(self.lead + tail, (n, self.T * n, *tail[1:], 1))
         return like.new_empty(self.lead + tail)
 
     def pointers(self):

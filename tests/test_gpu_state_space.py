@@ -672,3 +672,31 @@ def test_selective_scan_step_infinities_are_the_definitions(N, skip, dtype):
         yw, sw = scan_definition(lay, 2, *(None if p[k] is None else p[k].double() for k in ('x', 'dt', 'dt', 'A', 'B', 'C', 'D', 'z', 'dt_bias', 'dt_bias', 'state')), True)
         same_kind(y, yw[0], (field, 'y'))
         same_kind(s, sw, (field, 'state'))
+
+
+@pytest.mark.parametrize('shape,batch_first', [((6, 3), True), ((6, 3), False), ((1, 3), False), ((1, 3), True), ((6, 1), True)])
+def test_results_may_be_changed_in_place(shape, batch_first):
+    """A residual added to y where it lies, in every layout, before the backward pass."""
+    from paccmann_polymer_amd.state_space import causal_conv, selective_scan
+    g = torch.Generator(device=DEV).manual_seed(21)
+    T, B, D, N = *shape, 12, 8
+    x = randn(g, B, T, D).transpose(0, 1) if batch_first else randn(g, T, B, D)
+    bc, A, w = randn(g, T, B, N), -randn(g, D, N).abs(), randn(g, D, 4)
+
+    def run(inplace):
+        leaf = x.detach().requires_grad_()
+        y, last = selective_scan(leaf, x, A, bc, bc)
+        c, cl = causal_conv(leaf, w)
+        for i, t in enumerate((y, c)):
+            assert t.stride() == x.stride() or 1 in shape                # laid out as x is
+        if inplace:
+            y += x
+            c.mul_(2.0)
+            last.add_(1.0)
+            cl.zero_()
+        else:
+            y, c, last = y + x, c * 2.0, last + 1.0
+        return y.detach(), c.detach(), torch.autograd.grad((y.square().sum() + c.square().sum() + last.square().sum()), leaf)[0]
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
