@@ -92,14 +92,13 @@ def _policy_call(code, x, t, old, adv, ref, args, want_grad):
     clip_low, clip_high, kl_coef, ignore_index, temperature = args
     dev = x.device
     with _C.on_device(dev):
-        out = torch.empty(4, dtype=torch.float32, device=dev)
-        loss, stats = out[:1], out[1:]
+        loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(3, dtype=torch.float32, device=dev)     # no views: callers change them in place
         d = torch.empty(rows, V, dtype=x.dtype, device=dev) if want_grad else None
         wsb = _lib.ppk_policy_loss_workspace_bytes(rows)
         ws = torch.empty(max(int(wsb), 256), dtype=torch.uint8, device=dev)
         _C.check(_lib.ppk_policy_loss(code, _C.addr(x), _ld(x), _C.addr(t), rows, V, ignore_index, temperature, _C.addr(old), _C.addr(adv), _C.addr(ref),
                                       clip_low, clip_high, kl_coef, _C.addr(loss), _C.addr(stats), _C.addr(d), V, _C.addr(ws), wsb, _C.stream_on(x.device)))
-    return loss.reshape(()), stats, d
+    return loss, stats, d
 
 
 class _PolicyLoss(torch.autograd.Function):
