@@ -117,8 +117,9 @@ __device__ __forceinline__ double log_sum(float s)
     return s != s || s == INFINITY ? (double)s : fma((double)k, 0.69314718055994530942, 2.0 * r * p);
 }
 
-// e^d - d - 1: its series where the sum would cancel (|d| < 1/4: nine terms, the first left out 1e-10 of the whole), itself elsewhere
-__device__ __forceinline__ float kl_of(float d)
+// e^d - d - 1 and, in `em1`, e^d - 1: the first by its series where the sum would cancel (|d| < 1/4: eight terms, the first left out 8e-12 of
+// the whole), the second as its sum with d there.  Each by itself elsewhere: -(e^d - d - 1) - d rounds at the size of d, where e^d - 1 is at most 1.
+__device__ __forceinline__ float kl_of(float d, float& em1)
 {
     float p = fmaf(d, 1.0f / 362880, 1.0f / 40320);
     p = fmaf(d, p, 1.0f / 5040);
@@ -127,7 +128,10 @@ __device__ __forceinline__ float kl_of(float d)
     p = fmaf(d, p, 1.0f / 24);
     p = fmaf(d, p, 1.0f / 6);
     p = fmaf(d, p, 0.5f);
-    return fabsf(d) < 0.25f ? d * d * p : expf(d) - d - 1.0f;
+    const float kl = d * d * p, e = expf(d) - 1.0f;
+    const bool near = fabsf(d) < 0.25f;
+    em1 = near ? kl + d : e;
+    return near ? kl : e - d;
 }
 
 // The terms of one row.  lp is fp64 (above); the differences that it enters are rounded once.  Returns dloss / dlp (before the division by n).
@@ -142,8 +146,9 @@ __device__ __forceinline__ float policy_terms(const RowArgs& a, float old, float
     kl = 0.0f;
     if (a.ref) {
         const float d = (float)((double)ref - lp);
-        kl = kl_of(d);
-        if (a.beta != 0.0f) g = fmaf(-a.beta, kl + d, g);         // 1 - e^d = -(kl + d); no KL term: nor what it could overflow to
+        float em1;
+        kl = kl_of(d, em1);
+        if (a.beta != 0.0f) g = fmaf(-a.beta, em1, g);            // no KL term: nor what it could overflow to
     }
     return g;
 }

@@ -284,3 +284,24 @@ def test_loss_may_be_changed_in_place():
     (d,) = torch.autograd.grad(loss, x)
     assert torch.equal(d, want) and torch.equal(stats, keep) and loss.dim() == 0
     stats.zero_()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('off', [-float('inf'), -1e9, -200.0, -20.0, -3.0, -0.26, -0.24, 0.24, 0.26, 3.0, 20.0])
+def test_kl_gradient_far_from_the_reference(off, dtype):
+    """1 - e^d of a reference that all but forbids the taken token, and on both sides of where its series ends."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(12, 33, dtype, 6, ignored=0.0)
+    lp, p = definition(logits, tgt, 1.0)
+    old, adv = lp.float(), torch.zeros(12, device='cuda')
+    ref = (lp + 0.05).float()
+    ref[4] = float(lp[4]) + off
+    x = logits.detach().requires_grad_()
+    loss, _ = policy_loss(x, tgt, old, adv, ref, kl_coef=0.5)
+    (d,) = torch.autograd.grad(loss, x)
+    grad_w = policy_definition(logits, tgt, old, adv, ref, 0.2, 0.2, 0.5, 1.0)[2]
+    e = torch.exp(ref.double() - lp)
+    # the row's factor 0.5 (1 - e^d) / n: e^d is off by 130 H of itself (d is off by what lp is) and by H d, and the difference is rounded once
+    size = 0.5 / 12 * (e * (130 + (ref.double() - lp).abs().clamp(max=100)) + (e - 1).abs() * (140 * p.amax(1) + 12))
+    close(d, grad_w, (size * H)[:, None].expand_as(grad_w), dtype)
+    assert bool(torch.isfinite(d).all()) and bool(d[4].any())
