@@ -137,9 +137,10 @@ __device__ __forceinline__ float kl_of(float d, float& em1)
 // The terms of one row.  lp is fp64 (above); the differences that it enters are rounded once.  Returns dloss / dlp (before the division by n).
 __device__ __forceinline__ float policy_terms(const RowArgs& a, float old, float adv, float ref, double lp, float& pg, float& kl, float& clipped)
 {
-    const float ratio = expf((float)(lp - (double)old));
+    const float lr = (float)(lp - (double)old), ratio = expf(lr);
     const float held_r = ratio < a.low ? a.low : (ratio > a.high ? a.high : ratio);
-    const float free_ = ratio * adv, held = held_r * adv;
+    // a ratio that is finite but beyond fp32, times no advantage: nothing
+    const float free_ = adv == 0.0f && lr < INFINITY ? adv : ratio * adv, held = held_r * adv;
     pg = -(free_ <= held ? free_ : (free_ != free_ ? free_ : held));
     clipped = held < free_ ? 1.0f : 0.0f;
     float g = free_ <= held ? -free_ : 0.0f;

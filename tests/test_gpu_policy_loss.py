@@ -305,3 +305,19 @@ def test_kl_gradient_far_from_the_reference(off, dtype):
     size = 0.5 / 12 * (e * (130 + (ref.double() - lp).abs().clamp(max=100)) + (e - 1).abs() * (140 * p.amax(1) + 12))
     close(d, grad_w, (size * H)[:, None].expand_as(grad_w), dtype)
     assert bool(torch.isfinite(d).all()) and bool(d[4].any())
+
+
+def test_no_advantage_and_a_ratio_beyond_fp32():
+    """e^(lp - old) overflows; times an advantage of zero it is zero, in the loss and in the gradient."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(9, 21, torch.float32, 3, ignored=0.0)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    old[2], adv[2] = -120.0, 0.0
+    old[5], adv[5] = -120.0, -0.0
+    x = logits.detach().requires_grad_()
+    loss, stats = policy_loss(x, tgt, old, adv, ref, kl_coef=0.1)
+    (d,) = torch.autograd.grad(loss, x)
+    want = policy_definition(logits, tgt, old, adv, ref, 0.2, 0.2, 0.1, 1.0)
+    assert abs(float(loss.detach() - want[0])) <= 130 * H * float(want[3] + 1) + H
+    assert bool(((stats.double() - want[1]).abs() <= 130 * H * (want[3] + 1) + H).all())
+    assert float((d.double() - want[2]).abs().max()) <= 1e-6
