@@ -121,6 +121,10 @@ __device__ __forceinline__ double log_sum(float s)
 // the whole), the second as its sum with d there.  Each by itself elsewhere: -(e^d - d - 1) - d rounds at the size of d, where e^d - 1 is at most 1.
 __device__ __forceinline__ float kl_of(float d, float& em1)
 {
+    if (!(fabsf(d) < 0.25f)) {
+        em1 = expf(d) - 1.0f;
+        return em1 - d;
+    }
     float p = fmaf(d, 1.0f / 362880, 1.0f / 40320);
     p = fmaf(d, p, 1.0f / 5040);
     p = fmaf(d, p, 1.0f / 720);
@@ -128,10 +132,9 @@ __device__ __forceinline__ float kl_of(float d, float& em1)
     p = fmaf(d, p, 1.0f / 24);
     p = fmaf(d, p, 1.0f / 6);
     p = fmaf(d, p, 0.5f);
-    const float kl = d * d * p, e = expf(d) - 1.0f;
-    const bool near = fabsf(d) < 0.25f;
-    em1 = near ? kl + d : e;
-    return near ? kl : e - d;
+    p *= d * d;
+    em1 = p + d;
+    return p;
 }
 
 // The terms of one row.  lp is fp64 (above); the differences that it enters are rounded once.  Returns dloss / dlp (before the division by n).
