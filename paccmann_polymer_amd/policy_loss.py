@@ -112,7 +112,7 @@ class _PolicyLoss(torch.autograd.Function):
         loss, stats, d = _policy_call(code, x, targets, old, adv, ref, args, want_grad)
         if d is not None:
             ctx.save_for_backward(x, targets, old, adv, ref)
-            ctx.grad, ctx.code, ctx.args = d, code, args
+            ctx.grad, ctx.code, ctx.args, ctx.captured = d, code, args, torch.cuda.is_current_stream_capturing()
         ctx.mark_non_differentiable(stats)
         return loss, stats
 
@@ -120,7 +120,8 @@ class _PolicyLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss, _dstats):
         d, ctx.grad = ctx.grad, None                        # it is handed on and may be changed: a second backward pass makes its own
-        if d is None:
+        # so does one that is captured behind an eager forward pass: each replay would multiply the same memory once more
+        if d is None or (not ctx.captured and torch.cuda.is_current_stream_capturing()):
             x, targets, old, adv, ref = ctx.saved_tensors
             d = _policy_call(ctx.code, x, targets, old, adv, ref, ctx.args, True)[2]
         dev = d.device

@@ -321,3 +321,17 @@ def test_no_advantage_and_a_ratio_beyond_fp32():
     assert abs(float(loss.detach() - want[0])) <= 130 * H * float(want[3] + 1) + H
     assert bool(((stats.double() - want[1]).abs() <= 130 * H * (want[3] + 1) + H).all())
     assert float((d.double() - want[2]).abs().max()) <= 1e-6
+
+
+def test_backward_captured_behind_an_eager_forward_pass(monkeypatch):
+    """A graph replays its multiplication by the upstream gradient: what the eager forward pass wrote once must not be its operand."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(30, 20, torch.float32, 4)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    x = logits.detach().requires_grad_()
+    loss, _ = policy_loss(x, tgt, old, adv, ref, kl_coef=0.1)
+    held = loss.grad_fn.grad
+    keep = held.clone()
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    (d,) = torch.autograd.grad(loss * 4.0, x)
+    assert torch.equal(held, keep) and torch.equal(d, keep * 4.0)
