@@ -266,6 +266,13 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _no_gradient(what, **tensors):
+    """A step's results are part of no autograd graph: an input that wants a gradient is refused, or it would be lost without a word."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f'{what}: {name} requires a gradient (training goes through the form for whole sequences; call this one under torch.no_grad())')
+
+
 def _step_out(what, state, out, others):
     """Where a step writes its new state: `out`, or fresh memory.  `out` may be the state itself, but share memory with nothing else."""
     if out is None:
@@ -286,7 +293,7 @@ def _step_out(what, state, out, others):
 
 def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
     """One token of each of B sequences: x [B, D], state [B, K - 1, D] -> (y [B, D], new state).  `out`: where the new state goes
-    (it may be `state`: updated in place).  Inference only: training goes through `causal_conv`."""
+    (it may be `state`: updated in place).  Inference only, an input that wants a gradient is refused: training goes through `causal_conv`."""
     what = 'causal_conv_step'
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f'{what}: x must be [B, D]')
@@ -298,6 +305,8 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
         raise ValueError(f'{what}: state must be {[B, K - 1, D]}')
     if state.dtype != x.dtype:
         raise TypeError(f'{what}: state must be {x.dtype}, as x is')
+    if torch.is_grad_enabled():
+        _no_gradient(what, x=x, state=state, weight=weight, bias=bias)
     dev = _C.one_device(x, state, weight, bias)
     with _C.on_device(dev):
         ld, unit = x.stride()
@@ -430,8 +439,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, plan: Optional[
 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=True, out=None):
     """One token of each of B sequences: x, dt, z [B, channels], B, C [B, groups, N] or [B, N], state [B, channels, N] fp32 -> (y [B, channels],
-    new state).  `out`: where the new state goes (it may be `state`: updated in place).  Inference only: training goes through
-    `selective_scan`."""
+    new state).  `out`: where the new state goes (it may be `state`: updated in place).  Inference only, an input that wants a gradient is refused:
+    training goes through `selective_scan`."""
     what = 'selective_scan_step'
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f'{what}: x must be [B, channels]')
@@ -453,6 +462,8 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
         rows.append(v if v.stride(-1) == 1 or shape[-1] == 1 else v.contiguous())
     x, dt, z, B, C = rows
     _param(what, 'state', state, (n, width, N))
+    if torch.is_grad_enabled():
+        _no_gradient(what, x=x, dt=dt, A=A, B=B, C=C, state=state, D=D, z=z, dt_bias=dt_bias)
     dev = _C.one_device(x, dt, A, B, C, D, z, dt_bias, state)
     with _C.on_device(dev):
         A, D, dt_bias = A.contiguous(), _contiguous(D), _contiguous(dt_bias)

@@ -199,3 +199,25 @@ def test_per_step_inputs_of_another_packing_are_refused(name):
     flat[name] = args[name]
     with pytest.raises(ValueError, match=f'{name} is packed in another way'):
         S.selective_scan(**flat)
+
+
+@pytest.mark.parametrize('name', ['x', 'state', 'weight', 'bias'])
+def test_causal_conv_step_refuses_what_wants_a_gradient(name):
+    """Its results are no part of an autograd graph: a gradient would be lost without a word."""
+    a = dict(x=torch.zeros(B, D), state=torch.zeros(B, K - 1, D), weight=torch.zeros(D, K), bias=torch.zeros(D))
+    a[name].requires_grad_()
+    with pytest.raises(ValueError, match=f'{name} requires a gradient'):
+        S.causal_conv_step(**a)
+    with torch.no_grad(), pytest.raises(_C.PPKError):                            # all in order, but on the CPU
+        S.causal_conv_step(**a)
+
+
+@pytest.mark.parametrize('name', ['x', 'dt', 'A', 'B', 'C', 'state', 'D', 'z', 'dt_bias'])
+def test_selective_scan_step_refuses_what_wants_a_gradient(name):
+    a = dict(x=torch.zeros(B, D), dt=torch.zeros(B, D), A=torch.zeros(D, N), B=torch.zeros(B, N), C=torch.zeros(B, N), state=torch.zeros(B, D, N),
+             D=torch.zeros(D), z=torch.zeros(B, D), dt_bias=torch.zeros(D))
+    a[name].requires_grad_()
+    with pytest.raises(ValueError, match=f'{name} requires a gradient'):
+        S.selective_scan_step(**a)
+    with torch.no_grad(), pytest.raises(_C.PPKError):
+        S.selective_scan_step(**a)
