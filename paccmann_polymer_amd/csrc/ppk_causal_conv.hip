@@ -415,17 +415,19 @@ int conv_check(const char* what, int dtype, long long T, long long B, long long 
     if (T < 0 || B < 0 || D < 1 || D > (1 << 20) || K < 1) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld K=%lld", what, T, B, D, K);
     if (K > 8) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld taps (at most 8)", what, K);
     if (!strides || !w || (B > 0 && T > 0 && !x)) PPK_FAIL(PPK_ERR_NULL, "%s: null pointer", what);
-    if (T >= 1LL << 31 || B >= 1LL << 31 || conv_cut(T, B, D, false, false).blocks * conv_cut(T, B, D, false, false).channel_blocks > 0x7fffffffLL)
-        PPK_FAIL(PPK_ERR_UNSUP, "%s: T=%lld B=%lld D=%lld", what, T, B, D);
+    if (T >= 1LL << 31 || B >= 1LL << 31) PPK_FAIL(PPK_ERR_UNSUP, "%s: T=%lld B=%lld D=%lld", what, T, B, D);
     for (int i = 0; i < nstrides; i += 2)
         if (strides[i] < 0 || strides[i] >= 1LL << 30) PPK_FAIL(PPK_ERR_UNSUP, "%s: rows 2^30 elements or more apart", what);
     return PPK_OK;
 }
 
+// row blocks of the launch, or an error
 template <typename T> int conv_run(ConvArgs a, bool bwd, hipStream_t st)
 {
     const bool vec = conv_vec(a, (int)sizeof(T));
     const ConvCut k = conv_cut(a.q.T, a.q.B, a.D, vec, bwd);
+    if (!ppk_grid_fits(k.blocks * k.channel_blocks, 256))
+        PPK_FAIL(PPK_ERR_UNSUP, "causal_conv: T=%lld B=%lld D=%d takes %lld blocks, more than a launch has", a.q.T, a.q.B, a.D, k.blocks * k.channel_blocks);
     a.run = k.run;
     a.runs = (int)k.runs;
     if (vec) launch_conv<T, WIDE>(a, bwd, k.lanes, (unsigned)k.blocks, st);
@@ -450,8 +452,8 @@ int ppk_causal_conv_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
     a.D = (int)D; a.K = (int)K;
     a.x = x; a.state = state; a.weight = weight; a.bias = bias; a.y = y; a.last = K > 1 ? new_state : nullptr; a.silu = silu;
     a.xs = {strides_host[0], strides_host[1]}; a.ys = {strides_host[2], strides_host[3]};
-    if (dtype == PPK_F32) conv_run<float>(a, false, (hipStream_t)stream);
-    else conv_run<bf16_t>(a, false, (hipStream_t)stream);
+    rc = dtype == PPK_F32 ? conv_run<float>(a, false, (hipStream_t)stream) : conv_run<bf16_t>(a, false, (hipStream_t)stream);
+    if (rc < 0) return rc;
     PPK_CHECK_LAUNCH("causal_conv_fwd");
     return PPK_OK;
 }
@@ -483,6 +485,7 @@ int ppk_causal_conv_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t K, c
     a.xs = {strides_host[0], strides_host[1]}; a.dys = {strides_host[2], strides_host[3]}; a.ys = {strides_host[4], strides_host[5]};
     int blocks = 0;
     if (B > 0) blocks = dtype == PPK_F32 ? conv_run<float>(a, true, st) : conv_run<bf16_t>(a, true, st);
+    if (blocks < 0) return blocks;
     const ppk::SumJob job = {a.part, blocks, cols, dweight, (int)K, dbias};
     rc = ppk::partial_sums(&job, 1, nullptr, st);
     if (rc) return rc;
@@ -496,7 +499,8 @@ int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void*
     if (dtype != PPK_F32 && dtype != PPK_BF16) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: type %d (fp32 and bf16 are supported)", dtype);
     if (B < 0 || D < 1 || K < 1 || ldx < 0) PPK_FAIL(PPK_ERR_SHAPE, "causal_conv_step: B=%lld D=%lld K=%lld", (long long)B, (long long)D, (long long)K);
     if (K > 8) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: %lld taps (at most 8)", (long long)K);
-    if (B * D > 0xffffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: B=%lld D=%lld", (long long)B, (long long)D);
+    if (B >= 1LL << 32 || D >= 1LL << 31 || !ppk_grid_fits((B * D + 255) / 256, 256))
+        PPK_FAIL(PPK_ERR_UNSUP, "causal_conv_step: B=%lld D=%lld, more channels than a launch has threads", (long long)B, (long long)D);
     if (B == 0) return PPK_OK;
     if (!x || !weight || !y || (K > 1 && (!state || !new_state))) PPK_FAIL(PPK_ERR_NULL, "causal_conv_step: null pointer");
     const unsigned blocks = (unsigned)((B * D + 255) / 256);

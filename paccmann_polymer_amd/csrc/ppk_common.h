@@ -38,6 +38,9 @@ void ppk_set_error(const char* fmt, ...);
         if (e__ != hipSuccess) PPK_FAIL(PPK_ERR_HIP, "%s: %s", #call, hipGetErrorString(e__)); \
     } while (0)
 
+// A launch holds fewer than 2^32 threads.
+static inline bool ppk_grid_fits(long long blocks, int threads) { return blocks <= 0xffffffffLL / threads; }
+
 static inline size_t ppk_align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // carve `bytes` (256-B aligned) out of a workspace cursor

@@ -777,7 +777,7 @@ int scan_check(const char* what, int dtype, long long T, long long B, long long 
     if (T < 0 || B < 0 || D < 1 || N < 1 || G < 1 || D % G) PPK_FAIL(PPK_ERR_SHAPE, "%s: T=%lld B=%lld D=%lld N=%lld G=%lld", what, T, B, D, N, G);
     if (N > 64) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld states a channel (at most 64)", what, N);
     if (D > (1 << 20)) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld channels", what, D);
-    if (T >= 1LL << 30) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld steps", what, T);
+    if (T >= 1LL << 30 || B >= 1LL << 31) PPK_FAIL(PPK_ERR_UNSUP, "%s: %lld steps of B=%lld sequences", what, T, B);
     return PPK_OK;
 }
 
@@ -839,7 +839,8 @@ int ppk_selective_scan_fwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
     a.y = y; a.last = last_state; a.kept = kept;
     set_strides(a, strides_host);
     const long long blocks = B * p.splits * G * a.blocks_per_group;
-    if (blocks > 0x7fffffffLL || (p.splits > 1 && B > 65535)) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_fwd: B=%lld D=%lld", (long long)B, (long long)D);
+    if (!ppk_grid_fits(blocks, 64) || (p.splits > 1 && B > 65535))
+        PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_fwd: B=%lld D=%lld takes %lld blocks, more than a launch has", (long long)B, (long long)D, blocks);
     hipStream_t st = (hipStream_t)stream;
     if (p.splits > 1) {
         if (ws_bytes < carry_bytes(B, D, N, p.splits) || !workspace) PPK_FAIL(PPK_ERR_WS, "selective_scan_fwd: workspace of %zu bytes", ws_bytes);
@@ -897,8 +898,9 @@ int ppk_selective_scan_bwd(int dtype, int64_t T, int64_t B, int64_t D, int64_t N
     a.dx = dx; a.draw = draw; a.dz = dz; a.kept = const_cast<float*>(kept); a.dstate = dstate; a.nrows = rows;
     set_strides(a, strides_host);
     const long long blocks = items * G * a.blocks_per_group, bc = rows * G * 2 * N;
-    if (blocks > 0x7fffffffLL || ceil_div(bc, 256) > 0x7fffffffLL || (w.p.splits > 1 && B > 65535))
-        PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_bwd: B=%lld D=%lld rows=%lld", (long long)B, (long long)D, (long long)rows);
+    if (!ppk_grid_fits(blocks, 256) || !ppk_grid_fits(ceil_div(bc, 256), 256) || (w.p.splits > 1 && B > 65535))
+        PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_bwd: B=%lld D=%lld rows=%lld takes %lld and %lld blocks, more than a launch has", (long long)B, (long long)D, (long long)rows,
+                 blocks, ceil_div(bc, 256));
     if (blocks > 0) {
         if (w.p.splits > 1) {
             ScanArgs part = a;
@@ -937,7 +939,7 @@ int ppk_selective_scan_step(int dtype, int64_t B, int64_t D, int64_t N, int64_t 
     a.x = x; a.raw = raw; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.skip = skip; a.bias = bias; a.softplus = softplus; a.y = y;
     set_strides(a, strides_host);
     const long long blocks = ceil_div(B * D * slices(N), 256);
-    if (blocks > 0x7fffffffLL) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_step: B=%lld D=%lld", (long long)B, (long long)D);
+    if (!ppk_grid_fits(blocks, 256)) PPK_FAIL(PPK_ERR_UNSUP, "selective_scan_step: B=%lld D=%lld takes %lld blocks, more than a launch has", (long long)B, (long long)D, blocks);
     if (dtype == PPK_F32) run_step<float>(a, (unsigned)blocks, state, new_state, (hipStream_t)stream);
     else run_step<bf16_t>(a, (unsigned)blocks, state, new_state, (hipStream_t)stream);
     PPK_CHECK_LAUNCH("selective_scan_step");

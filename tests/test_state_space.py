@@ -221,3 +221,17 @@ def test_selective_scan_step_refuses_what_wants_a_gradient(name):
         S.selective_scan_step(**a)
     with torch.no_grad(), pytest.raises(_C.PPKError):
         S.selective_scan_step(**a)
+
+
+@pytest.mark.parametrize('call', [
+    lambda L: L.ppk_causal_conv_fwd(0, 1, (1 << 31) - 1, 8, 4, None, None, 16, 16, None, None, 1, 16, None, strides(4), None),
+    lambda L: L.ppk_causal_conv_step(0, (1 << 32) - 1, 1, 4, 16, 1, 16, 16, None, 1, 16, 16, None),
+    lambda L: L.ppk_selective_scan_fwd(0, 1, 1 << 26, 8, 4, 1, None, None, None, *[16] * 5, *[None] * 4, 1, 16, 16, None, strides(16), None, 0, None),
+    lambda L: L.ppk_selective_scan_bwd(0, 1, 1 << 24, 8, 4, 1, 1 << 24, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 1 << 60, None),
+    lambda L: L.ppk_selective_scan_bwd(0, 32, 1 << 20, 8, 64, 1, 1 << 25, None, None, None, *[16] * 5, *[None] * 3, 1, 16, 16, None, *[16] * 5, *[None] * 4, strides(16), 256, 1 << 60, None),
+    lambda L: L.ppk_selective_scan_step(0, 1 << 28, 16, 4, 1, *[16] * 5, *[None] * 3, 16, 1, 16, 16, strides(16), None),
+])
+def test_more_threads_than_a_launch_has_are_refused(call):
+    """A grid holds fewer than 2^32 threads: said before anything is launched, with the sizes."""
+    assert call(_C.lib) == -4
+    assert b'B=' in _C.lib.ppk_last_error()
