@@ -309,6 +309,12 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 // JOIN_STATES states and as many slices of the splits as make 256 threads, each slice joins its own, then the slices.  Bound by the latency of its
 // loads: 128 splits of 1024 channels x 16 states 7.8 us (a thread a state, one split after the other: 12; 16 states a block: 12, 64: 9.0).
 constexpr int JOIN_STATES = 32;
+// decay x + own.  No step's decay is 0 or infinite, but that of many steps may be beyond fp32: a state of 0 stays 0 and an infinite one infinite all the same.
+__device__ __forceinline__ float carried(float decay, float x, float own)
+{
+    constexpr int ZERO_OR_INF = 0x264;
+    return __builtin_amdgcn_classf(x, ZERO_OR_INF) ? x + own : fmaf(decay, x, own);
+}
 template <bool REV, int U>
 __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
 {
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
     for (int k0 = 0; k0 < used; k0 += S * U) {
         const int many = used - k0 < S * U ? used - k0 : S * U, per = (many + S - 1) / S, k1 = k0 + slice * per;
         const int n = many - slice * per < per ? many - slice * per : per;      // 0 or less: nothing left for this slice
-        float own[U], by[U], end = 0.f, decay = 1.f;
+        float own[U], by[U], end = 0.f, decay = 0.f;                             // decay: its exponent
         // The part of the last split on the way (forward the sequence's last, backward its first) is not made: nobody asks for it.  Loads are
         // not masked, so that all of them fly together: one behind the last made is that one again.
         const int last = used > 1 ? used - 2 : 0;
@@ -344,23 +350,24 @@ __global__ __launch_bounds__(256) void k_scan_join(ScanArgs a)
         for (int i = 0; i < U; ++i) {
             const bool made = i < n && k1 + i + 1 < used;
             own[i] = made ? own[i] : 0.f;
-            by[i] = made ? exp2_(by[i] * A2) : 1.f;
-            end = fmaf(by[i], end, own[i]);
-            decay *= by[i];
+            by[i] = made ? by[i] * A2 : 0.f;
+            decay += by[i];
+            by[i] = exp2_(by[i]);
+            end = carried(by[i], end, own[i]);
         }
         s_end[slice][el] = end;
-        s_decay[slice][el] = decay;
+        s_decay[slice][el] = exp2_(decay);
         __syncthreads();
         float mine = in;
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             if (k == slice) mine = in;
-            in = fmaf(s_decay[k][el], in, s_end[k][el]);
+            in = carried(s_decay[k][el], in, s_end[k][el]);
         }
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (live && i < n) c[dir * (k1 + i) * dn] = mine;
-            mine = fmaf(by[i], mine, own[i]);
+            mine = carried(by[i], mine, own[i]);
         }
         __syncthreads();
     }

@@ -700,3 +700,46 @@ def test_results_may_be_changed_in_place(shape, batch_first):
 
     for a, b in zip(run(True), run(False)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('T,A,dt', [(2048, 1.0, 1.0), (2048, -1.0, -1.0), (700, 4.0, 1.0)])
+def test_states_that_grow_from_zero(T, A, dt):
+    """Decays above one over more steps than fp32 holds the product of, with nothing to multiply: a state (a gradient) of zero stays zero, in one
+    piece and in splits."""
+    from paccmann_polymer_amd.state_space import selective_scan
+    D, N, few = 8, 16, 10
+    g = torch.Generator(device=DEV).manual_seed(T)
+    lay = Layout([T], 'time')
+    t = dict(x=torch.zeros(T, 1, D, device=DEV), dt=torch.full((T, 1, D), dt, device=DEV), A=torch.full((D, N), A, device=DEV),
+             B=randn(g, T, 1, 1, N), C=randn(g, T, 1, 1, N), D=None, z=None, dt_bias=None, state=torch.zeros(1, D, N, device=DEV))
+    t['x'][T - few:] = randn(g, few, 1, D)
+    dy, dlast = torch.zeros(T, 1, D, device=DEV), torch.zeros(1, D, N, device=DEV)
+    dy[:few] = randn(g, few, 1, D)
+    names = [k for k, v in t.items() if v is not None]
+    leaves = {k: None if v is None else v.detach().requires_grad_() for k, v in t.items()}
+    y, last = selective_scan(**leaves, dt_softplus=False)
+    got = dict(zip(names, torch.autograd.grad((y, last), [leaves[k] for k in names], (dy, dlast))))
+    yw, lw, want = scan_reference(lay, t, dy, dlast, False, False)
+    yc, lc, comp = scan_reference(lay, t, dy, dlast, False, True)
+    # dt has one sign here, which the companion keeps: all of its terms have the same one, and their magnitude is what bounds an error
+    yc, lc, comp = yc.abs(), lc.abs(), {k: v.abs() for k, v in comp.items()}
+    # |dt A| <= 4 here: twice what a step of the other tests loses
+    close(y.detach(), yw, (80 * (few + 2) + N) * H * yc + 1e-37, 'y')
+    close(last.detach(), lw, 80 * (few + 2) * H * lc + 1e-37, 'last')
+    for k in names:
+        close(got[k], want[k], (160 * (few + 2) + N + (D if k in ('B', 'C') else 0)) * H * 3 * comp[k] + 1e-37, k)
+
+
+def test_an_infinite_state_stays_infinite_across_splits():
+    """Its decay over thousands of steps is below what fp32 holds; no step's is."""
+    from paccmann_polymer_amd.state_space import selective_scan
+    T, D, N = 4096, 8, 16
+    lay = Layout([T], 'time')
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, dt, bc = randn(g, T, 1, D), torch.full((T, 1, D), 0.5, device=DEV), randn(g, T, 1, 1, N).abs()
+    A, state = torch.full((D, N), -1.0, device=DEV), torch.zeros(1, D, N, device=DEV)
+    state[0, 3] = float('inf')
+    y, last = selective_scan(x, dt, A, bc, bc, state=state, dt_softplus=False)
+    assert bool(torch.isposinf(y[:, 0, 3]).all()) and bool(torch.isposinf(last[0, 3]).all())
+    keep = [i for i in range(D) if i != 3]
+    assert bool(torch.isfinite(y[:, :, keep]).all())
