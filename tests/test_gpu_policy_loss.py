@@ -335,3 +335,49 @@ def test_backward_captured_behind_an_eager_forward_pass(monkeypatch):
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
     (d,) = torch.autograd.grad(loss * 4.0, x)
     assert torch.equal(held, keep) and torch.equal(d, keep * 4.0)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,V', [(12001, 300), (45003, 9), (4201, 3001), (6001, 700)])
+def test_more_rows_than_a_launch_holds_at_once(rows, V, dtype):
+    """Blocks that go from row to row: what is loaded ahead, a last round that not every group has a row of, sums carried across rows, and
+    rows of 256 threads that use their LDS again."""
+    test_token_log_probs(rows, V, dtype)
+    test_policy_loss(rows, V, dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,V,ld,offset', [(40, 575, 577, 1), (6, 2050, 2053, 3), (1500, 33, 35, 1), (3, 9001, 9003, 5), (1, 140001, 140001, 1)])
+def test_policy_gradient_of_a_slice(rows, V, ld, offset, dtype):
+    """Logits whose rows begin at other offsets from 16 bytes than the gradient's: the same results as of a copy that lies as the gradient does."""
+    from paccmann_polymer_amd.policy_loss import policy_loss
+    logits, tgt, g = make(rows, V, dtype, rows + V, ld=ld, offset=offset)
+    old, adv, ref = policy_inputs(logits, tgt, g, 0.2, 0.2)
+    lp, p = definition(logits, tgt, 1.0)
+    loss_w, stats_w, grad_w, size = policy_definition(logits, tgt, old, adv, ref, 0.2, 0.2, 0.05, 1.0)
+    x = logits.detach().requires_grad_()
+    assert x.data_ptr() % 16 == offset * x.element_size() % 16
+    loss, stats = policy_loss(x, tgt, old, adv, ref, kl_coef=0.05)
+    (d,) = torch.autograd.grad(loss, x)
+    tol = 130 * H * (size + 0.5 + 0.1) + H                              # as in test_policy_loss
+    assert abs(float(loss.detach() - loss_w)) <= float(tol) + H * abs(float(loss_w))
+    use = (tgt != 0)[:, None]
+    gmax = torch.exp(lp - old.double()) * adv.double().abs() + 0.05 * torch.exp(ref.double() - lp)
+    close(d, grad_w, torch.where(use, gmax[:, None] / max(1, int(use.sum())) * (p * 272 + 140) * H, 0.0), dtype)
+
+
+def test_rows_beyond_32_bits():
+    """Rows of logits further than 2^32 bytes apart in all: read where they lie, with the results of rows that begin as far from 16 bytes."""
+    from paccmann_polymer_amd.policy_loss import policy_loss, token_log_probs
+    rows, V, far = 5, 70, 2 ** 30 + 3
+    values, tgt, g = make(rows, V, torch.bfloat16, 9, ignored=0.0)
+    logits, near = (torch.empty((rows - 1) * ld + V, dtype=torch.bfloat16, device='cuda').as_strided((rows, V), (ld, 1)).copy_(values) for ld in (far, 72 + 3))
+    old, adv, ref = policy_inputs(near, tgt, g, 0.2, 0.2)
+    out = []
+    for t in (logits, near):
+        x, y = t.detach().requires_grad_(), t.detach().requires_grad_()
+        lp = token_log_probs(x, tgt)
+        loss, stats = policy_loss(y, tgt, old, adv, ref, kl_coef=0.1)
+        out.append((lp.detach(), loss.detach(), stats, *torch.autograd.grad((lp, loss), (x, y), (adv, torch.ones_like(loss)))))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)

@@ -743,3 +743,49 @@ def test_an_infinite_state_stays_infinite_across_splits():
     assert bool(torch.isposinf(y[:, 0, 3]).all()) and bool(torch.isposinf(last[0, 3]).all())
     keep = [i for i in range(D) if i != 3]
     assert bool(torch.isfinite(y[:, :, keep]).all())
+
+
+MANY = [100 - b * 80 // 2047 for b in range(2048)]                      # 2048 sequences of 100 to 20 steps
+
+
+@pytest.mark.parametrize('lengths,kind,D,K,wide', [
+    (MANY, 'packed', 32, 4, 0),                  # more items than a backward launch has room for: its blocks take several, one after the other
+    (MANY, 'packed', 256, 3, 8),                 # runs of 32 steps
+    (MANY, 'packed', 512, 4, 0),                 # runs of 64
+    (MANY[::8], 'packed', 512, 4, 1),            # runs of 16, a channel a lane
+    ([100] * 40, 'batch', 4100, 4, 0)])          # at most 64 blocks for each of 17 blocks of channels
+@pytest.mark.parametrize('dtype', TYPES)
+def test_causal_conv_of_many_runs(lengths, kind, D, K, wide, dtype):
+    test_causal_conv(D, K, wide, True, True, True, lengths, kind, dtype)
+
+
+@pytest.mark.parametrize('walk', ['steps', 'sequences'])
+def test_offsets_beyond_32_bits_reach_the_kernels(walk):
+    """Steps (sequences) just under 2^30 elements apart: taken as they lie, and their offsets pass 2^32 bytes."""
+    from paccmann_polymer_amd import state_space as S
+    g = torch.Generator(device=DEV).manual_seed(12)
+    far, D, N = 2 ** 30 - 64, 64, 16
+    T, B = (5, 2) if walk == 'steps' else (2, 5)
+    base = torch.empty(4 * far + 16 * D, dtype=torch.bfloat16, device=DEV)
+
+    def view(k, *tail):
+        n = (1 if len(tail) == 1 else tail[1])
+        near = 8 * D
+        t = torch.as_strided(base, (T, B, *tail), (*((far, near) if walk == 'steps' else (near, far)), *([n, 1] if len(tail) == 2 else [1])), k * D)
+        t.copy_(randn(g, T, B, *tail, dtype=torch.bfloat16))
+        return t
+    x, dt, z, dy, dc = (view(k, D) for k in range(5))
+    B_, C_ = view(5, 1, N), view(6, 1, N)
+    for name, t in (('x', x), ('dt', dt), ('z', z), ('dy', dy), ('dc', dc), ('B', B_), ('C', C_)):
+        batch = S._Batch('test', x, None)
+        assert batch.take(name, t, tuple(t.shape[2:]), t.dtype).data_ptr() == t.data_ptr()
+    A, w = -torch.rand(D, N, generator=g, device=DEV), randn(g, D, 4)
+
+    def both(x, dt, z, B, C, dy, dc):
+        leaves = [t.detach().requires_grad_() for t in (x, dt, z, B, C)]
+        y, last = S.selective_scan(leaves[0], leaves[1], A, leaves[3], leaves[4], z=leaves[2])
+        c, cl = S.causal_conv(leaves[0], w)
+        return (y, last, c, cl, *torch.autograd.grad((y, c), leaves, (dy, dc)))
+
+    for a, b in zip(both(x, dt, z, B_, C_, dy, dc), both(*(t.contiguous() for t in (x, dt, z, B_, C_, dy, dc)))):
+        assert torch.equal(a, b)
