@@ -305,7 +305,7 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu', out=None):
         raise ValueError(f'{what}: state must be {[B, K - 1, D]}')
     if state.dtype != x.dtype:
         raise TypeError(f'{what}: state must be {x.dtype}, as x is')
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (x.requires_grad or state.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         _no_gradient(what, x=x, state=state, weight=weight, bias=bias)
     dev = _C.one_device(x, state, weight, bias)
     with _C.on_device(dev):
@@ -462,7 +462,9 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
         rows.append(v if v.stride(-1) == 1 or shape[-1] == 1 else v.contiguous())
     x, dt, z, B, C = rows
     _param(what, 'state', state, (n, width, N))
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (
+            x.requires_grad or dt.requires_grad or A.requires_grad or B.requires_grad or C.requires_grad or state.requires_grad or (D is not None and D.requires_grad)
+            or (z is not None and z.requires_grad) or (dt_bias is not None and dt_bias.requires_grad)):
         _no_gradient(what, x=x, dt=dt, A=A, B=B, C=C, state=state, D=D, z=z, dt_bias=dt_bias)
     dev = _C.one_device(x, dt, A, B, C, D, z, dt_bias, state)
     with _C.on_device(dev):
