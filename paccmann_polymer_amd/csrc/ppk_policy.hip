@@ -14,9 +14,11 @@ namespace {
 constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int COUNT_BLOCK = 1024;                // targets per partial count
 constexpr long long COUNT_INLINE = 2048;         // up to so many rows, every block counts them itself: cheaper than a launch of their own
-// Blocks of the policy modes that hold several rows at once: what is resident together (five waves a SIMD), each loading its next rows while it
-// works on the ones before.  122880 x 575 fp32 with the gradient: 129 us, 142 with 2048 blocks, 137 with 4096, 140 with 4096 and nothing
-// loaded ahead.  Scores alone have eight waves a SIMD and need neither: 59 us with 4096 blocks, 71 with 1280.
+// Blocks of the policy modes that hold several rows at once, each loading its next rows while it works on the ones before: what is resident
+// together of 122880 x 575 fp32 rows (five waves a SIMD), where the kernel takes 129 us, 142 with 2048 blocks, 137 with 4096, 140 with 4096 and
+// nothing loaded ahead.  Other rows would take more: whole passes with 1280, 2560 and 4096 blocks, 1000000 x 64 fp32 203, 202, 211 us, bf16 229, 212,
+// 206; 122880 x 575 bf16 229, 214, 208; 70000 x 1000 fp32 153, 132-153, 131-136; 3000000 x 9 fp32 436, 404, 383.  Scores alone have eight waves a
+// SIMD and need neither: 59 us with 4096 blocks, 71 with 1280.
 constexpr int RESIDENT_BLOCKS = 1280;
 constexpr int MAX_BLOCKS = 4096;                 // row blocks of a launch, and rows of its partial sums
 

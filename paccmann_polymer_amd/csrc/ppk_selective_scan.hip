@@ -153,7 +153,8 @@ __device__ __forceinline__ void rows_of(const SeqBatch& q, int t, int last, int 
 }
 
 // The forward pass: a lane a channel with its NP >= N states in registers, B and C of a step in scalar registers (SCALAR) or handed over
-// from lanes.  PART: only the state at the end of a split that begins with none, and the sum of its dt.
+// from lanes (at 32 states three waves a SIMD and 30 to 44 scalar registers spilled, at 64 one wave and 204 to 208: 64 x 256 x 1024 fp32 151 us at 16
+// states, 252 at 32, 452 at 64; 17 and 33 do the work of 32 and 64).  PART: only the state at the end of a split that begins with none, and the sum of its dt.
 template <typename T, int NP, bool SCALAR, bool PART>
 __global__ __launch_bounds__(64) void k_scan_fwd(ScanArgs a)
 {
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(64) void k_scan_bwd_part(ScanArgs a)
 // Joins the splits of a sequence: carry[s] holds what split s gives alone and receives what enters it.  Forward from the state before
 // the first step, backward (REV) from the gradient of the state behind the last.  h' = decay h + own is associative: a block takes
 // JOIN_STATES states and as many slices of the splits as make 256 threads, each slice joins its own, then the slices.  Bound by the latency of its
-// loads: 128 splits of 1024 channels x 16 states 7.8 us (a thread a state, one split after the other: 12; 16 states a block: 12, 64: 9.0).
+// loads: 128 splits of 1024 channels x 16 states 8.2 us (a thread a state, one split after the other: 12; 16 states a block: 12, 64: 9.0).
 constexpr int JOIN_STATES = 32;
 // decay x + own.  No step's decay is 0 or infinite, but that of many steps may be beyond fp32: a state of 0 stays 0 and an infinite one infinite all the same.
 __device__ __forceinline__ float carried(float decay, float x, float own)
@@ -384,9 +385,9 @@ template <int LPC> __device__ __forceinline__ float sum_slices(float v)
 }
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-// Parts of a tile: a sequence's last tile is worked on as far as the part that its last step is in.  2048 sequences of 20 to 100 steps, 512 channels,
-// 16 states, fp32: 1170 us, 1223 with whole tiles, 1177 with three parts; 1 x 16384 x 2048 bf16: 540, 530 with three; 21 sequences of 1 to 100
-// steps, 333 channels: 44, 46 with whole tiles, 42 with three.  Parts of two steps: only their second can be one that does not exist.
+// Parts of a tile: a sequence's last tile is worked on as far as the part that its last step is in.  Least times of 2048 sequences of 20 to 100
+// steps, 512 channels, 16 states, fp32: 1130-1170 us with parts of two steps, 1177 with three parts, 1223 with whole tiles; 1 x 16384 x 2048 bf16
+// (whole tiles only): 535-550, 530 with three.  Parts of two steps: only their second can be one that does not exist.
 constexpr int NPARTS = 8, PART = TILE / NPARTS, FETCH_PART = 4;
 
 // The backward pass.  A block takes 256 / LPC channels of a group of one sequence and walks a split's tiles backwards; a thread holds the
@@ -399,7 +400,9 @@ constexpr int NPARTS = 8, PART = TILE / NPARTS, FETCH_PART = 4;
 // Elements of a tile are loaded while the tile behind it is worked on, and what the tile's end needs of them waits in LDS.
 // FULL: N is 4 LPC and the channels of a group are whole blocks.  Otherwise states and channels that do not exist are kept at zero: their products
 // with an infinite input, B, C or gradient would be NaN, and sums over states and channels take them in (21 sequences, 333 channels of three
-// groups, 11 states: 46 us, 44 without).
+// groups, 11 states: 47 us, 44 without).
+// Bound by the vector unit at two waves a SIMD: 16 steps of states and decays are 132 of 256 registers, and at 16 states 4 more and 70 to 76 scalar
+// ones are spilled (up to 84 bytes of scratch a lane).
 template <typename T, int LPC, bool FULL>
 __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanArgs a)
 {
