@@ -292,8 +292,8 @@ int ppk_causal_conv_step(int dtype, int64_t B, int64_t D, int64_t K, const void*
  * strides_host [16]: x, raw (two each), B, C (step, sequence, group), z (two), the outputs in ROWS of their width (two), dy (two).
  * Fewer than 2^30 steps and 2^31 rows; the rows of a step's tensors fewer than 2^30 elements apart; fewer than 2^32 threads in any launch:
  * fwd 64 for each 64 channels of a group of each sequence (and split of its steps), bwd 256 for each 64 (N <= 16), 32 or 16 (N > 32) of
- * them, and rows G 2 N for dB and dC, step B D ceil(N / 4); the convolution 256 for a run's group of up to 256 channels, step B D.  A call
- * beyond is PPK_ERR_UNSUP, and nothing is launched.
+ * them, and rows G 2 N for dB and dC, step B D times 1, 2, 4, 8 or 16 (N to 4, 8, 16, 32, 64); the convolution 256 for every four runs of 64 steps
+ * and 256 channels (64 where rows allow no 4-element accesses), step B D.  A call beyond is PPK_ERR_UNSUP, and nothing is launched.
  * y, dx, draw, dz [rows, D], dB, dC [rows, G, N].  bwd overwrites all its outputs; dskip, dbias, dstate may be NULL. */
 int64_t ppk_selective_scan_tile(void);
 size_t ppk_selective_scan_fwd_workspace_bytes(int64_t T, int64_t B, int64_t D, int64_t N, int64_t G);      /* 0 where none is needed */
